@@ -55,6 +55,13 @@ _SIGNATURES = {
     "mm_launch_count": (c_int64, []),
     "mm_fp8_w8a8_mega_moe_static": (c_int, [c_void_p] * 10 + [c_int] * 5 + [c_float, c_void_p]),
     "mm_fp8_w8a8_mega_moe_static_status": (c_int, [c_void_p, POINTER(c_int32)]),
+    "mm_cast_block128": (c_int, [c_void_p, c_int, c_int64, c_int, c_int64, c_void_p, c_void_p, c_void_p]),
+    "mm_cast_weight_block128": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "mm_fp8_gemm_block128": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int64, c_int,
+                                     c_int64, c_int, c_int, c_void_p]),
+    "mm_norm_gate_residual": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_void_p, c_int, c_void_p, c_int, c_int64, c_int, c_void_p,
+                                      c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_float, c_float, c_void_p]),
+    "mm_block128_read_status": (c_int, [c_void_p, POINTER(c_int32)]),
     "mm_set_stage_timing": (c_int, [c_int]),
     "mm_get_stage_times": (c_int, [POINTER(c_float), c_int]),
 }

@@ -260,6 +260,9 @@ int stage_end(int id, cudaStream_t stream) {
 
 // lets the other translation units of the library report through mm_last_error
 void mm_detail_set_error(const char* msg) { snprintf(g_err, sizeof(g_err), "%s", msg); }
+// and share its launch counter and the limit of its in-kernel waits
+void mm_detail_count_launch() { g_launches.fetch_add(1); }
+uint64_t mm_detail_pipe_timeout_ns() { return (uint64_t)g_pipe_ms.load() * 1000000ull; }
 
 extern "C" {
 

@@ -1,0 +1,379 @@
+// Products of e4m3 operands with a scale for each block of 128 (tcgen05, accumulators in TMEM, operands by TMA).
+//
+//   d[m, n] = sum over kb of ( sum over k in block kb of a[m, k] b[e][n, k] ) * sa[m, kb] * sb[e][n / 128, kb]
+//
+// The tensor core sums one block of 128 k exactly as it would any product; the scales change from block to block, so each
+// block's accumulator is read back from TMEM, multiplied and added to fp32 sums in registers, while the tensor core works on
+// the next block in another TMEM buffer.  For a 128 x 256 tile that is 32768 values for each 512 cycles of MMA at the e4m3
+// rate: 8 epilogue warps hold 128 sums per thread and take two of them with each fma.rn.f32x2.
+//
+// One CTA per SM, 384 threads: warp 0 = TMA, warp 1 = MMA, warp 2 owns TMEM, warps 4-11 = epilogue (registers moved to them).
+// kSplit > 1: the CTAs of a cluster share one tile and divide its k blocks; the fp32 parts meet in distributed shared memory
+// and are added in rank order, so the result does not depend on timing.
+#pragma once
+#include <cuda_bf16.h>
+#include "layout.h"
+#include "pack.cuh"
+#include "ptx.cuh"
+
+namespace mm {
+
+constexpr int kB128Threads = 384;
+constexpr int kB128EpiThreads = 256;
+
+struct B128GemmParams {
+    int m, n, k_blocks;
+    int m_tiles, n_tiles;              // of 128 rows and BN columns
+    int a_box_rows;
+    int n_sf;                          // 128-blocks of weight rows for each expert
+    int experts;
+    int tiled;                         // weights as [expert][n block][k block][256 rows][128]: a 2-D map, else [expert][n][k]: a 3-D map
+    int tiled_n_blocks;
+    const float* sa; int64_t sa_stride;        // [m][k_blocks]
+    const float* sb;                           // [experts][n_sf][k_blocks]
+    const int* m_indices;                      // grouped: expert of each row (-1: padding, not written), else null
+    void* out; int64_t out_stride;             // elements
+    int out_fp32;
+    int out_vec32;                             // rows and base are multiples of 32 bytes
+    int* status;
+    uint64_t timeout_ns;
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap* map, int32_t c0, int32_t c1, int32_t c2, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+}
+template <int kRegs> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
+template <int kRegs> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
+
+// Two fp32 sums at a time.
+__device__ __forceinline__ uint64_t pack_f32x2(uint32_t lo, uint32_t hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+    return v;
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ void fma_f32x2(uint64_t& acc, uint64_t a, uint64_t b) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
+}
+__device__ __forceinline__ void st_global_32b(void* p, const uint32_t (&v)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+__device__ __forceinline__ float4 ld_shared_cluster_f4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+template <int kBN> struct B128Shape {
+    static constexpr int kStages = kBN == 256 ? 4 : 6;
+    static constexpr int kAccs = 512 / kBN;                          // TMEM accumulators in turn
+    static constexpr int kABytes = 128 * 128;
+    static constexpr int kBBytes = kBN * 128;
+    static constexpr int kStageBytes = kABytes + kBBytes;
+    static constexpr int kStagingBytes = 8 * 32 * 33 * 4;            // a 32 x 32 fp32 piece for each epilogue warp
+    static constexpr int kBarBytes = 256;
+    static constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + kBarBytes;
+    static_assert(kSmemBytes <= 232448, "exceeds the 227 KiB of shared memory a CTA can have");
+    static_assert(128 * (kBN + 4) * 4 <= kStages * kStageBytes, "the fp32 part of a split tile fits in the operand ring");
+};
+
+// Tile number -> (m tile, n tile): eight m tiles at a time run through all n tiles, so that the operands that CTAs of one wave
+// read stay few.
+__device__ __forceinline__ void b128_tile(const B128GemmParams& p, int tile, int& mt, int& nt) {
+    const int per_group = 8 * p.n_tiles;
+    const int g = tile / per_group, r = tile - g * per_group;
+    const int gm = min(8, p.m_tiles - g * 8);
+    nt = r / gm;
+    mt = g * 8 + r - nt * gm;
+}
+
+// Adds one k block's accumulator (kCols columns of this warp's 32 lanes at `taddr`) times `s` to the sums.
+template <int kCols>
+__device__ __forceinline__ void b128_promote(uint64_t (&acc)[kCols / 2], uint32_t taddr, float s, uint32_t free_bar, int lane) {
+    const uint64_t s2 = pack_f32x2(__float_as_uint(s), __float_as_uint(s));
+#pragma unroll
+    for (int c = 0; c < kCols; c += 64) {
+        uint32_t v0[32], v1[32];
+        tmem_ld_32x32(taddr + c, v0);
+        tmem_ld_32x32(taddr + c + 32, v1);
+        tmem_ld_wait();
+        if (c + 64 >= kCols) {                       // all of it is in registers: the tensor core may have the buffer back
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(free_bar);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) fma_f32x2(acc[c / 2 + j], pack_f32x2(v0[2 * j], v0[2 * j + 1]), s2);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) fma_f32x2(acc[c / 2 + 16 + j], pack_f32x2(v1[2 * j], v1[2 * j + 1]), s2);
+    }
+}
+
+template <int kBN, bool kSplit>
+__global__ void __launch_bounds__(kB128Threads, 1)
+block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const B128GemmParams p) {
+    using S = B128Shape<kBN>;
+    constexpr int kStages = S::kStages, kAccs = S::kAccs;
+    constexpr int kCols = kBN / 2;                               // columns of a tile that one epilogue thread sums
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const uint32_t smem_base = smem_u32(smem);
+    uint8_t* staging = smem + kStages * S::kStageBytes;
+    const uint32_t bars = smem_base + kStages * S::kStageBytes + S::kStagingBytes;
+    auto full_bar = [&](int s) { return bars + 8u * s; };
+    auto empty_bar = [&](int s) { return bars + 8u * (kStages + s); };
+    auto tfull_bar = [&](int a) { return bars + 8u * (2 * kStages + a); };
+    auto tempty_bar = [&](int a) { return bars + 8u * (2 * kStages + kAccs + a); };
+    constexpr int kTail = 8 * (2 * kStages + 2 * kAccs);
+    static_assert(kTail + 16 <= S::kBarBytes, "barriers");
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(staging + S::kStagingBytes + kTail);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(staging + S::kStagingBytes + kTail + 8);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int split = 1, part = 0;
+    if (kSplit) {
+        asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(split));
+        part = static_cast<int>(cluster_ctarank());
+    }
+    const int num_tiles = p.m_tiles * p.n_tiles;
+    const int first_tile = blockIdx.x / split, tile_step = gridDim.x / split;
+    // the k blocks of this CTA
+    const int kb0 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * part / split);
+    const int kb1 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (part + 1) / split);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+        for (int a = 0; a < kAccs; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), 8); }
+        *abort_flag = 0;
+        fence_barrier_init();
+        prefetch_tensormap(&tm_a);
+        prefetch_tensormap(&tm_b);
+    }
+    if (warp == 2) {
+        tmem_alloc(smem_u32(tmem_slot), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    // expert of an m tile (grouped: of its first row), or -1 when there is nothing to do; every role asks and skips alike
+    auto tile_expert = [&](int mt) {
+        if (p.m_indices == nullptr) return 0;
+        const int e = p.m_indices[mt * 128];
+        return e < p.experts ? e : -1;
+    };
+
+    if (warp < 4) {
+        regs_dec<88>();
+        if (warp == 0 && lane == 0) {
+            // ------------------------------------------------------------------ TMA
+            int stage = 0; uint32_t phase = 0;
+            bool alive = true;
+            const uint32_t bytes = static_cast<uint32_t>(p.a_box_rows) * 128 + S::kBBytes;
+            for (int tile = first_tile; tile < num_tiles && alive; tile += tile_step) {
+                int mt, nt;
+                b128_tile(p, tile, mt, nt);
+                const int e = tile_expert(mt);
+                if (e < 0) continue;
+                const int64_t tiled0 = (static_cast<int64_t>(e) * p.tiled_n_blocks + (nt * kBN) / 256) * p.k_blocks;
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
+                    const uint32_t a_dst = smem_base + stage * S::kStageBytes;
+                    mbar_arrive_expect_tx(full_bar(stage), bytes);
+                    if (p.tiled) tma_load_2d(a_dst + S::kABytes, &tm_b, 0, static_cast<int32_t>((tiled0 + kb) * 256 + (nt * kBN) % 256), full_bar(stage));
+                    else tma_load_3d(a_dst + S::kABytes, &tm_b, kb * 128, nt * kBN, e, full_bar(stage));
+                    tma_load_2d(a_dst, &tm_a, kb * 128, mt * 128, full_bar(stage));
+                    if (++stage == kStages) { stage = 0; phase ^= 1u; }
+                }
+            }
+        } else if (warp == 1 && lane == 0) {
+            // ------------------------------------------------------------------ MMA
+            constexpr uint32_t idesc = umma_idesc_f8(128, kBN);
+            int stage = 0; uint32_t phase = 0;
+            int acc = 0; uint32_t acc_phase = 0;
+            bool alive = true;
+            for (int tile = first_tile; tile < num_tiles && alive; tile += tile_step) {
+                int mt, nt;
+                b128_tile(p, tile, mt, nt);
+                if (tile_expert(mt) < 0) continue;
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
+                    if (!mbar_wait(full_bar(stage), phase, abort_flag, p.timeout_ns)) { alive = false; break; }
+                    tc_fence_after();
+                    const uint64_t da = umma_desc_k_sw128(smem_base + stage * S::kStageBytes);
+                    const uint64_t db = umma_desc_k_sw128(smem_base + stage * S::kStageBytes + S::kABytes);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) umma_f8(tmem_base + acc * kBN, da + 2u * k, db + 2u * k, idesc, k != 0 ? 1u : 0u);
+                    umma_commit(empty_bar(stage));
+                    umma_commit(tfull_bar(acc));
+                    if (++stage == kStages) { stage = 0; phase ^= 1u; }
+                    if (++acc == kAccs) { acc = 0; acc_phase ^= 1u; }
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---------------------------------------------------------------------- epilogue
+        regs_inc<208>();
+        const int q = warp & 3;                              // TMEM lane quarter of this warp
+        const int half = (warp - 4) >> 2;                    // which half of the columns
+        const int et = q * 32 + lane;                        // row of the tile
+        float* my_staging = reinterpret_cast<float*>(staging) + (warp - 4) * 32 * 33;
+        int acc = 0; uint32_t acc_phase = 0;
+        bool alive = true;
+        for (int tile = first_tile; tile < num_tiles && alive; tile += tile_step) {
+            int mt, nt;
+            b128_tile(p, tile, mt, nt);
+            const int e = tile_expert(mt);
+            if (p.m_indices != nullptr) {
+                // rows of another expert than the block's first one, or behind padding, are a mistake in the layout: reported, not written
+                const int first = p.m_indices[mt * 128];
+                const int own = p.m_indices[mt * 128 + et];
+                if ((first >= p.experts || (own >= 0 && own != first)) && atomicCAS(p.status, 0, MM_ERR_BAD_GROUP_LAYOUT) == 0) {
+                    p.status[1] = 0; p.status[2] = mt; p.status[3] = first; p.status[4] = own;
+                }
+            }
+            if (e < 0) continue;
+            const int row = mt * 128 + et;
+            bool row_ok = row < p.m;
+            if (row_ok && p.m_indices != nullptr) row_ok = p.m_indices[row] == e;
+            const float* sa = p.sa + static_cast<int64_t>(row < p.m ? row : 0) * p.sa_stride;
+            const int n_block = min(nt * (kBN / 128) + (kBN == 256 ? half : 0), p.n_sf - 1);
+            const float* sb = p.sb + (static_cast<int64_t>(e) * p.n_sf + n_block) * p.k_blocks;
+            uint64_t sum[kCols / 2];
+#pragma unroll
+            for (int j = 0; j < kCols / 2; ++j) sum[j] = 0ull;
+            float s_next = sa[kb0] * sb[kb0];
+            for (int kb = kb0; kb < kb1; ++kb) {
+                const float s = s_next;
+                if (kb + 1 < kb1) s_next = sa[kb + 1] * sb[kb + 1];
+                if (!mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.timeout_ns)) { alive = false; break; }
+                tc_fence_after();
+                b128_promote<kCols>(sum, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * kBN + half * kCols, s, tempty_bar(acc), lane);
+                if (++acc == kAccs) { acc = 0; acc_phase ^= 1u; }
+            }
+            if (!alive) break;
+            if (kSplit) {
+                // this CTA's part of the tile, for the cluster to add up: the operand ring is idle now (the last accumulator
+                // was complete, so every copy and every MMA of this CTA is done)
+                float* mine = reinterpret_cast<float*>(smem) + et * (kBN + 4) + half * kCols;
+#pragma unroll
+                for (int j = 0; j < kCols / 2; j += 2) {
+                    float4 f;
+                    unpack_f32x2(sum[j], f.x, f.y);
+                    unpack_f32x2(sum[j + 1], f.z, f.w);
+                    *reinterpret_cast<float4*>(mine + 2 * j) = f;
+                }
+                continue;
+            }
+            const int col0 = nt * kBN + half * kCols;
+            if (p.out_vec32 && col0 + kCols <= p.n) {
+                if (row_ok) {
+                    if (p.out_fp32) {
+                        float* o = static_cast<float*>(p.out) + row * p.out_stride + col0;
+#pragma unroll
+                        for (int j = 0; j < kCols / 2; j += 4) {
+                            uint32_t v[8];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) { float a, b; unpack_f32x2(sum[j + i], a, b); v[2 * i] = __float_as_uint(a); v[2 * i + 1] = __float_as_uint(b); }
+                            st_global_32b(o + 2 * j, v);
+                        }
+                    } else {
+                        __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + row * p.out_stride + col0;
+#pragma unroll
+                        for (int j = 0; j < kCols / 2; j += 8) {
+                            uint32_t v[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) { float a, b; unpack_f32x2(sum[j + i], a, b); v[i] = pack_bf16x2(a, b); }
+                            st_global_32b(o + 2 * j, v);
+                        }
+                    }
+                }
+            } else {
+                // any number of columns and any alignment: 32 columns at a time through shared memory, so that a warp writes
+                // neighbouring columns of one row
+#pragma unroll
+                for (int c = 0; c < kCols; c += 32) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) unpack_f32x2(sum[c / 2 + j], my_staging[lane * 33 + 2 * j], my_staging[lane * 33 + 2 * j + 1]);
+                    __syncwarp();
+                    const unsigned rows_ok = __ballot_sync(0xffffffffu, row_ok);
+                    const int col = col0 + c + lane;
+                    for (int r = 0; r < 32; ++r) {
+                        if (!((rows_ok >> r) & 1u) || col >= p.n) continue;
+                        const int64_t at = (mt * 128 + q * 32 + r) * p.out_stride + col;
+                        if (p.out_fp32) static_cast<float*>(p.out)[at] = my_staging[r * 33 + lane];
+                        else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16(my_staging[r * 33 + lane]);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    }
+
+    if (kSplit) {
+        __syncwarp();
+        cluster_sync_all();                                  // every part of the tile is in shared memory
+        if (warp >= 4 && *abort_flag == 0 && first_tile < num_tiles) {
+            int mt, nt;
+            b128_tile(p, first_tile, mt, nt);
+            const int e = tile_expert(mt);
+            const int rows = e < 0 ? 0 : min(128, p.m - mt * 128);
+            constexpr int kPer = kBN / 32;                   // columns of a lane: 4 at a time
+            for (int r = part + (warp - 4) * split; r < rows; r += 8 * split) {
+                const int row = mt * 128 + r;
+                if (p.m_indices != nullptr && p.m_indices[row] != e) continue;
+#pragma unroll
+                for (int c0 = 0; c0 < kPer; c0 += 4) {
+                    const int c = (c0 / 4) * 128 + lane * 4;
+                    const uint32_t at = smem_base + static_cast<uint32_t>(r * (kBN + 4) + c) * 4;
+                    float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int i = 0; i < split; ++i) {
+                        const float4 v = ld_shared_cluster_f4(mapa_shared(at, i));
+                        t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w;
+                    }
+                    const int col = nt * kBN + c;
+                    const float f[4] = {t.x, t.y, t.z, t.w};
+                    const int64_t o = row * p.out_stride + col;
+                    if (p.out_vec32 && col + 4 <= p.n) {
+                        if (p.out_fp32) *reinterpret_cast<float4*>(static_cast<float*>(p.out) + o) = t;
+                        else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + o) = make_uint2(pack_bf16x2(t.x, t.y), pack_bf16x2(t.z, t.w));
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if (col + j >= p.n) continue;
+                            if (p.out_fp32) static_cast<float*>(p.out)[o + j] = f[j];
+                            else static_cast<__nv_bfloat16*>(p.out)[o + j] = __float2bfloat16(f[j]);
+                        }
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        cluster_sync_all();                                  // nobody leaves while its part may still be read
+    }
+
+    if (*abort_flag != 0) {
+        // a bounded wait expired: give copies that may still be in flight time to land, then report
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 1000000ull) __nanosleep(1000);
+        if (threadIdx.x == 0 && atomicCAS(p.status, 0, MM_ERR_PIPE_TIMEOUT) == 0) {
+            p.status[1] = 20; p.status[2] = blockIdx.x; p.status[3] = num_tiles; p.status[4] = 0;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 2) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
+    }
+}
+
+}  // namespace mm

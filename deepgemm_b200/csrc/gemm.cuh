@@ -16,6 +16,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include "layout.h"
+#include "pack.cuh"
 #include "ptx.cuh"
 
 namespace mm {
@@ -76,15 +77,6 @@ __device__ __forceinline__ uint8_t* combine_row_ptr(const GemmParams& p, int src
     if (src_rank < 0 || src_rank >= p.R || slot >= p.K || src_token < 0 || src_token >= p.T) return nullptr;
     return reinterpret_cast<uint8_t*>(p.peers[src_rank]) + p.combine_off +
            (static_cast<int64_t>(src_token) * p.K + slot) * p.H * 2;
-}
-
-// x * sigmoid(x) with the fast exponential and reciprocal units, as the reference does
-// (deep_gemm/include/deep_gemm/common/mega_moe_dcu.cuh:90-99: exp2 and rcp intrinsics)
-__device__ __forceinline__ float silu_f(float x) { return __fdividef(x, 1.0f + __expf(-x)); }
-
-__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
-    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&v);
 }
 
 // Epilogue arithmetic of one output tile for one epilogue warp: read this warp's share of the accumulator from TMEM,

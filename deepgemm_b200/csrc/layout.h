@@ -25,6 +25,7 @@ enum {
     MM_ERR_PIPE_TIMEOUT = 2,
     MM_ERR_POOL_OVERFLOW = 3,
     MM_ERR_GRID_BARRIER_TIMEOUT = 4,
+    MM_ERR_BAD_GROUP_LAYOUT = 5,     // a 128-row block of an m-grouped GEMM mixes experts or has a hole
 };
 
 struct MmStatus {       // first bytes of the scratch buffer

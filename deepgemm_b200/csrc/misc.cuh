@@ -3,25 +3,11 @@
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include "layout.h"
+#include "pack.cuh"
 #include "ptx.cuh"
 #include "route.cuh"
 
 namespace mm {
-
-__device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
-__device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
-
-__device__ __forceinline__ uint32_t pack4_e4m3(float a, float b, float c, float d) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-    return lo | (hi << 16);
-}
-
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
 
 // Per-row FP8 quantisation, bit-exact with megamoe/__init__.py:51-56 (cast_to_fp8_channelwise):
 //   scale = max(amax|x|, 1e-4) / 448 ; q = e4m3_rne(float(x) / scale)   (true IEEE divisions, as torch does).

@@ -15,8 +15,6 @@
 
 namespace mm {
 
-constexpr int MM_ERR_BAD_GROUP_LAYOUT = 5;     // a 128-row block of an m-grouped GEMM mixes experts or has a hole
-
 // One warp per 128-row block.  work: [0..15] status words (MmStatus), [16..31] plan ([16] = number of blocks),
 // [32 .. 32+blocks) expert of the block, [32+blocks .. 32+2*blocks) valid rows of the block.
 __global__ void __launch_bounds__(256) mgroup_plan_kernel(const int* __restrict__ m_indices, int rows, int num_experts, int* __restrict__ work) {

@@ -738,6 +738,11 @@ def swiglu_quant_channelwise_out(x: torch.Tensor, topk_weights: Optional[torch.T
     return out_fp8, out_scale_view
 
 
+from .block128 import (  # noqa: E402  (the modules share this package's library, not each other's names)
+    NormOutputs, cast_to_fp8_block128, cast_weight_to_fp8_block128, check_block128_status, fp8_gemm_nt_block128,
+    m_grouped_fp8_gemm_nt_contiguous_block128, norm_gate_residual,
+)
+
 __all__ = [
     "SymmBuffer",
     "cast_to_fp8_channelwise",
@@ -756,4 +761,11 @@ __all__ = [
     "fp8_w8a8_mega_moe",
     "fill_inputs_from_router",
     "RECIPE_UE8M0_PER32",
+    "NormOutputs",
+    "cast_to_fp8_block128",
+    "cast_weight_to_fp8_block128",
+    "check_block128_status",
+    "fp8_gemm_nt_block128",
+    "m_grouped_fp8_gemm_nt_contiguous_block128",
+    "norm_gate_residual",
 ]

@@ -1,0 +1,297 @@
+"""Operators in FP8 e4m3 with one fp32 scale for each block of 128 values, and the norms that feed them.
+
+Activations carry a scale for each 128 values of a row ([rows, ceil(K/128)]), weights one for each 128 x 128 block
+([.., ceil(N/128), ceil(K/128)]).  The channelwise layer (`fp8_mega_moe`) has one scale per row and per output channel instead; a
+checkpoint quantised by blocks cannot be converted to that without a second rounding, so it is served by these:
+
+  cast_to_fp8_block128, cast_weight_to_fp8_block128      bf16 / fp16 / fp32 -> codes and scales
+  fp8_gemm_nt_block128                                   dense product
+  m_grouped_fp8_gemm_nt_contiguous_block128              product of rows grouped by expert
+  norm_gate_residual                                     norms around a block with its gate, scaled residual and either cast
+
+Calls are asynchronous on the current stream of the tensors' device, keep nothing between calls and may be captured into a CUDA
+graph.  `check_block128_status()` reports what a kernel could not (a bounded wait that expired, a grouped layout that mixes experts).
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from .. import _lib
+
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_E4M3 = torch.float8_e4m3fn
+
+
+def _blocks(n: int) -> int:
+    return (n + 127) // 128
+
+
+def _call(device: torch.device, fn, *args) -> None:
+    """Run a library call (its last argument, the stream, is added here) with `device` current."""
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if rc != 0:
+        _lib.check(rc)
+
+
+def _require_cuda(name: str, *tensors: Optional[torch.Tensor]) -> torch.device:
+    device = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f"{name} needs CUDA tensors (this package has no CPU path)")
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise RuntimeError(f"{name}: tensors are on different devices ({device} and {t.device})")
+    return device
+
+
+def _rows_of(t: torch.Tensor, align: int) -> torch.Tensor:
+    """`t` [rows, k] as it is if its rows are dense and start on `align`-byte boundaries, else a contiguous copy."""
+    size = t.element_size()
+    if t.stride(1) == 1 and t.stride(0) >= t.size(1) and (t.stride(0) * size) % align == 0 and t.data_ptr() % align == 0:
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % align == 0 else t.clone()
+
+
+def cast_to_fp8_block128(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows [.., K] of bf16, fp16 or fp32 (K a multiple of 8) -> (e4m3 [.., K], fp32 scales [.., ceil(K/128)]).
+
+    For each 128 values of a row: top = max(amax, 1e-4), scale = top / 448, code = e4m3(448 x / top), ties to even.  A block that
+    holds an infinity or a NaN gets NaN codes and a scale that is not finite."""
+    if x.dim() < 1 or x.dtype not in _TYPES:
+        raise TypeError("cast_to_fp8_block128 expects a bfloat16, float16 or float32 tensor with at least one dimension")
+    k = x.shape[-1]
+    if k == 0 or k % 8 != 0:
+        raise ValueError("the row length must be a positive multiple of 8")
+    device = _require_cuda("cast_to_fp8_block128", x)
+    rows2d = x if x.dim() == 2 else x.reshape(-1, k)
+    rows2d = _rows_of(rows2d, 16)
+    rows = rows2d.shape[0]
+    q = torch.empty(x.shape, dtype=_E4M3, device=device)
+    sf = torch.empty((*x.shape[:-1], (k + 127) // 128), dtype=torch.float32, device=device)
+    if rows:
+        _call(device, _lib.lib().mm_cast_block128, rows2d.data_ptr(), _TYPES[x.dtype], rows, k, rows2d.stride(0), q.data_ptr(), sf.data_ptr())
+    return q, sf
+
+
+def cast_weight_to_fp8_block128(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Weights [N, K] or [E, N, K] (K a multiple of 8) -> (e4m3 of the same shape, fp32 scales [.., ceil(N/128), ceil(K/128)]):
+    the cast of `cast_to_fp8_block128` with one scale for each 128 x 128 block."""
+    if w.dim() not in (2, 3) or w.dtype not in _TYPES:
+        raise TypeError("cast_weight_to_fp8_block128 expects a 2D or 3D bfloat16, float16 or float32 tensor")
+    n, k = w.shape[-2:]
+    if k == 0 or k % 8 != 0:
+        raise ValueError("the row length must be a positive multiple of 8")
+    device = _require_cuda("cast_weight_to_fp8_block128", w)
+    w = w.contiguous()
+    if w.data_ptr() % 16 != 0:
+        w = w.clone()
+    q = torch.empty(w.shape, dtype=_E4M3, device=device)
+    sf = torch.empty((*w.shape[:-2], _blocks(n), _blocks(k)), dtype=torch.float32, device=device)
+    if w.numel():
+        _call(device, _lib.lib().mm_cast_weight_block128, w.data_ptr(), _TYPES[w.dtype], w.shape[0] if w.dim() == 3 else 1, n, k, q.data_ptr(), sf.data_ptr())
+    return q, sf
+
+
+def _check_operands(name, a, a_sf, b, b_sf, n, k):
+    if a.dtype != _E4M3 or b.dtype != _E4M3:
+        raise RuntimeError(f"{name} expects e4m3 operands")
+    if a_sf.dtype != torch.float32 or b_sf.dtype != torch.float32:
+        raise RuntimeError(f"{name} expects fp32 scales")
+    if k == 0 or k % 16 != 0:
+        raise RuntimeError(f"{name}: K must be a positive multiple of 16")
+    if a.dim() != 2 or a.shape[1] != k or tuple(a_sf.shape) != (a.shape[0], _blocks(k)):
+        raise RuntimeError(f"{name} expects a [M, K] with scales [M, ceil(K/128)], got {tuple(a.shape)} and {tuple(a_sf.shape)}")
+    if tuple(b_sf.shape[-2:]) != (_blocks(n), _blocks(k)):
+        raise RuntimeError(f"{name} expects weight scales [.., ceil(N/128), ceil(K/128)], got {tuple(b_sf.shape)}")
+
+
+def _scale_rows(sf: torch.Tensor) -> torch.Tensor:
+    return sf if sf.stride(1) == 1 and sf.stride(0) >= sf.shape[1] else sf.contiguous()
+
+
+def fp8_gemm_nt_block128(a: Tuple[torch.Tensor, torch.Tensor], b: Tuple[torch.Tensor, torch.Tensor], out: Optional[torch.Tensor] = None,
+                         out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """out[M, N] = a [M, K] . b [N, K]^T with a = (e4m3, scales [M, ceil(K/128)]), b = (e4m3, scales [ceil(N/128), ceil(K/128)]).
+
+    K is a multiple of 16 and may end inside a block; M and N are any.  Rows of `a` and of `out` may be strided.  The sums are fp32;
+    the output is bf16 or fp32 (`out`'s type, else `out_dtype`, else bf16)."""
+    (a_q, a_sf), (b_q, b_sf) = a, b
+    name = "fp8_gemm_nt_block128"
+    device = _require_cuda(name, a_q, a_sf, b_q, b_sf, out)
+    if b_q.dim() != 2 or b_sf.dim() != 2:
+        raise RuntimeError(f"{name} expects b [N, K] with 2D scales")
+    n, k = b_q.shape
+    _check_operands(name, a_q, a_sf, b_q, b_sf, n, k)
+    m = a_q.shape[0]
+    if out is None:
+        out = torch.empty((m, n), dtype=torch.bfloat16 if out_dtype is None else out_dtype, device=device)
+    elif tuple(out.shape) != (m, n) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n) or (out_dtype is not None and out.dtype != out_dtype):
+        raise RuntimeError(f"{name}: out must be [{m}, {n}] with dense rows (and of out_dtype, if that is given)")
+    if out.dtype not in (torch.bfloat16, torch.float32):
+        raise RuntimeError(f"{name}: the output is bfloat16 or float32")
+    if m == 0 or n == 0:
+        return out
+    a_q, b_q = _rows_of(a_q, 16), b_q.contiguous()
+    if b_q.data_ptr() % 16 != 0:
+        b_q = b_q.clone()
+    a_sf, b_sf = _scale_rows(a_sf), b_sf.contiguous()
+    _call(device, _lib.lib().mm_fp8_gemm_block128, a_q.data_ptr(), max(a_q.stride(0), k), a_sf.data_ptr(), max(a_sf.stride(0), _blocks(k)), b_q.data_ptr(),
+          b_sf.data_ptr(), 1, 0, None, out.data_ptr(), max(out.stride(0), n), out.dtype == torch.float32, m, n, k)
+    return out
+
+
+def m_grouped_fp8_gemm_nt_contiguous_block128(a: Tuple[torch.Tensor, torch.Tensor], b: Tuple[torch.Tensor, torch.Tensor], d: torch.Tensor,
+                                              m_indices: torch.Tensor, check: bool = False) -> torch.Tensor:
+    """d[row] = a[row] . b[e]^T with e = m_indices[row], as `m_grouped_fp8_gemm_nt_contiguous` with scales by blocks.
+
+    a = (e4m3 [rows, K], scales [rows, ceil(K/128)]), b = (e4m3 [E, N, K] or tiled (`pack_weights_tiled(w, "l2")`), scales
+    [E, ceil(N/128), ceil(K/128)]), d bf16 or fp32.  Rows are grouped by expert, groups padded to 128 rows; rows with m_indices -1 are
+    left as they were.  check=True synchronises and raises if a 128-row block mixed experts (such rows are not written)."""
+    (a_q, a_sf), (w, w_sf) = a, b
+    name = "m_grouped_fp8_gemm_nt_contiguous_block128"
+    device = _require_cuda(name, a_q, a_sf, w, w_sf, d, m_indices)
+    if w_sf.dim() != 3 or w.dim() not in (3, 5) or w.shape[0] != w_sf.shape[0]:
+        raise RuntimeError(f"{name} expects weights [E, N, K] (or tiled) with scales [E, ceil(N/128), ceil(K/128)]")
+    k = a_q.shape[-1]
+    n = d.shape[-1]
+    tiled = w.dim() == 5
+    if tiled and (n % 128 != 0 or k % 128 != 0 or tuple(w.shape[1:]) != ((n + 255) // 256, k // 128, 256, 128)):
+        raise RuntimeError(f"{name}: tiled weights of shape {tuple(w.shape)} do not match N = {n}, K = {k}")
+    if not tiled and tuple(w.shape[1:]) != (n, k):
+        raise RuntimeError(f"{name}: weights of shape {tuple(w.shape)} do not match N = {n}, K = {k}")
+    _check_operands(name, a_q, a_sf, w, w_sf, n, k)
+    rows = a_q.shape[0]
+    if tuple(d.shape) != (rows, n) or not d.is_contiguous() or d.dtype not in (torch.bfloat16, torch.float32):
+        raise RuntimeError(f"{name}: d must be a contiguous bfloat16 or float32 [{rows}, {n}]")
+    if m_indices.dtype != torch.int32 or tuple(m_indices.shape) != (rows,):
+        raise RuntimeError(f"{name} expects int32 m_indices [{rows}]")
+    if rows % _lib.BLOCK_M != 0:
+        raise RuntimeError(f"{name}: rows must be a multiple of {_lib.BLOCK_M} (groups padded to it)")
+    if rows and n and w.shape[0] == 0:
+        raise RuntimeError(f"{name}: no experts")
+    if rows and n:
+        a_q, w = _rows_of(a_q, 16), w.contiguous()
+        if w.data_ptr() % 16 != 0:
+            w = w.clone()
+        a_sf, w_sf, m_indices = _scale_rows(a_sf), w_sf.contiguous(), m_indices.contiguous()
+        _call(device, _lib.lib().mm_fp8_gemm_block128, a_q.data_ptr(), max(a_q.stride(0), k), a_sf.data_ptr(), max(a_sf.stride(0), _blocks(k)), w.data_ptr(),
+              w_sf.data_ptr(), w.shape[0], tiled, m_indices.data_ptr(), d.data_ptr(), n, d.dtype == torch.float32, rows, n, k)
+    if check:
+        check_block128_status(device)
+    return d
+
+
+def check_block128_status(device: Optional[torch.device] = None) -> None:
+    """Synchronise the current stream and raise if a kernel of this module has reported a failure on `device` since the last call."""
+    out = (ctypes.c_int32 * 5)()
+    with torch.cuda.device(device):
+        _lib.check(_lib.lib().mm_block128_read_status(torch.cuda.current_stream().cuda_stream, out))
+    if out[0] != 0:
+        raise _lib.MegaMoeError(f"device status {out[0]} ({_lib.STATUS_NAMES.get(out[0], '?')}): phase={out[1]} block={out[2]} "
+                                f"expected={out[3]} observed={out[4]}")
+
+
+class NormOutputs(NamedTuple):
+    """Outputs of norm_gate_residual; None where nothing was asked for."""
+    residual: torch.Tensor
+    normed: Optional[torch.Tensor]
+    codes: Optional[torch.Tensor]
+    scales: Optional[torch.Tensor]
+
+
+def norm_gate_residual(y: Optional[torch.Tensor], residual: torch.Tensor, *, post_weight: Optional[torch.Tensor] = None,
+                       gate: Optional[torch.Tensor] = None, residual_scale: float = 1.0, pre_weight: Optional[torch.Tensor] = None,
+                       eps: float = 1e-6, weight_offset: float = 0.0, quant: Optional[str] = None, out_normed: bool = True,
+                       out_codes: Optional[torch.Tensor] = None, out_scales: Optional[torch.Tensor] = None) -> NormOutputs:
+    """What stands between two blocks of a model, in one pass over [T, H]:
+
+        residual' = residual_scale * residual + gate * RMSNorm(y; post_weight)
+        normed    = RMSNorm(residual'; pre_weight)          (and its e4m3 codes)
+
+    with RMSNorm(v; w) = v * rsqrt(mean v^2 + eps) * (w + weight_offset).  y is the block's output; without it (before the first block)
+    the residual is only normed and returned as it is.  Without post_weight y is not normed, without gate it is not gated, without
+    pre_weight (after the last block) nothing but residual' comes back.  gate is [H], [T, 1] or [T, H].  quant: None, "block128" (scales
+    [T, ceil(H/128)], for the products of this module) or "channelwise" (scales [T], as `fp8_mega_moe` reads them; out_codes and
+    out_scales may be views of a SymmBuffer, `sb.x[:T]` and `sb.x_sf[:T]`).
+
+    y, residual, weights and gate are bf16, fp16 or fp32, each in its own type; residual' has residual's type, normed is bf16 (fp32 where
+    residual is fp16, never narrower than the range of the stream).  Arithmetic is fp32 throughout and each output is rounded once.  H is a
+    multiple of 8, at most 16384."""
+    name = "norm_gate_residual"
+    device = _require_cuda(name, y, residual, post_weight, gate, pre_weight, out_codes, out_scales)
+    for t in (y, residual, post_weight, gate, pre_weight):
+        if t is not None and t.dtype not in _TYPES:
+            raise TypeError(f"{name} expects bfloat16, float16 or float32 tensors")
+    if residual.dim() != 2:
+        raise ValueError(f"{name} expects a residual [T, H]")
+    t, h = residual.shape
+    if h == 0 or h % 8 != 0 or h > 16384:
+        raise ValueError(f"{name}: H must be a multiple of 8, at most 16384")
+    if y is None and (post_weight is not None or gate is not None or residual_scale != 1.0):
+        raise ValueError(f"{name}: post_weight, gate and residual_scale need y")
+    if y is not None and tuple(y.shape) != (t, h):
+        raise ValueError(f"{name}: y must be [{t}, {h}]")
+    for w in (post_weight, pre_weight):
+        if w is not None and tuple(w.shape) != (h,):
+            raise ValueError(f"{name}: norm weights must be [{h}]")
+    if quant not in (None, "block128", "channelwise"):
+        raise ValueError(f"{name}: quant must be None, 'block128' or 'channelwise'")
+    if pre_weight is None and quant is not None:
+        raise ValueError(f"{name}: codes need pre_weight")
+    if quant is None and (out_codes is not None or out_scales is not None):
+        raise ValueError(f"{name}: out_codes and out_scales need quant")
+    gate_rows = gate_cols = 0
+    if gate is not None:
+        if gate.dim() == 1:
+            gate = gate.unsqueeze(0)
+        if gate.dim() != 2 or gate.shape[0] not in (1, t) or gate.shape[1] not in (1, h):
+            raise ValueError(f"{name}: gate must be [{h}], [{t}, 1] or [{t}, {h}]")
+        if gate.shape[1] == h and h > 1:
+            gate = _rows_of(gate, 16)
+            gate_cols = 1
+        gate_rows = gate.stride(0) if gate.shape[0] == t and t > 1 else 0
+    sf_shape = (t, _blocks(h)) if quant == "block128" else (t,)
+    if out_codes is not None and (out_codes.dtype != _E4M3 or tuple(out_codes.shape) != (t, h) or not out_codes.is_contiguous() or out_codes.data_ptr() % 8 != 0):
+        raise ValueError(f"{name}: out_codes must be a contiguous e4m3 [{t}, {h}], 8-byte aligned")
+    if out_scales is not None and (out_scales.dtype != torch.float32 or tuple(out_scales.shape) != sf_shape or not out_scales.is_contiguous()):
+        raise ValueError(f"{name}: out_scales must be a contiguous float32 {list(sf_shape)}")
+    residual_out = residual if y is None else torch.empty((t, h), dtype=residual.dtype, device=device)
+    normed = codes = scales = None
+    if pre_weight is not None:
+        if out_normed:
+            normed = torch.empty((t, h), dtype=torch.float32 if residual.dtype == torch.float16 else torch.bfloat16, device=device)
+        if quant is not None:
+            codes = torch.empty((t, h), dtype=_E4M3, device=device) if out_codes is None else out_codes
+            scales = torch.empty(sf_shape, dtype=torch.float32, device=device) if out_scales is None else out_scales
+    if t and (y is not None or normed is not None or codes is not None):
+        r = _rows_of(residual, 16)
+        yy = None if y is None else _rows_of(y, 16)
+        post = None if post_weight is None else _vector(post_weight)
+        pre = None if pre_weight is None or (normed is None and codes is None) else _vector(pre_weight)
+
+        def ptr(v):
+            return None if v is None else v.data_ptr()
+
+        def kind(v):
+            return 0 if v is None else _TYPES[v.dtype]
+        _call(device, _lib.lib().mm_norm_gate_residual, ptr(yy), kind(yy), h if yy is None else max(yy.stride(0), h), r.data_ptr(), kind(r),
+              max(r.stride(0), h), ptr(post), kind(post), ptr(gate), kind(gate), gate_rows, gate_cols, ptr(pre), kind(pre),
+              None if y is None else residual_out.data_ptr(), ptr(normed), kind(normed), ptr(codes), ptr(scales),
+              {None: 0, "block128": 1, "channelwise": 2}[quant], t, h, residual_scale, eps, weight_offset)
+    return NormOutputs(residual_out, normed, codes, scales)
+
+
+def _vector(w: torch.Tensor) -> torch.Tensor:
+    w = w.contiguous()
+    return w if w.data_ptr() % 16 == 0 else w.clone()

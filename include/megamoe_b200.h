@@ -137,6 +137,40 @@ int mm_tile_order(int num_mblocks, int wave_mblocks, int gemm1_blocks, int gemm2
  * released it.  max_tiles = 0 switches the trace off.  Not for production: the stamps cost a few stores per tile. */
 int mm_set_tile_trace(void* device_words, int max_tiles, int cta);
 
+/* ---- Operators in e4m3 with one fp32 scale for each block of 128 values (activations: 1 x 128 along a row, weights: 128 x 128).
+ * Checkpoints quantised that way cannot be served by the channelwise layer above.  No counterpart in the reference's W8A8 path.
+ * type: 0 = bf16, 1 = fp16, 2 = fp32.  Row strides are in elements.  All calls are asynchronous on `stream`, allocate nothing and
+ * may be captured into a CUDA graph. */
+
+/* Activations [rows, k] (k and row_stride multiples of 8): top = max(amax of 128 values, 1e-4), sf[rows][ceil(k/128)] = top / 448,
+ * q = e4m3(448 x / top).  A block that holds an infinity or a NaN gets NaN codes and a scale that is not finite. */
+int mm_cast_block128(const void* x, int type, int64_t rows, int k, int64_t row_stride, void* q, float* sf, void* stream);
+
+/* Weights [experts, rows, k], contiguous: the same with 128 x 128 blocks, sf[experts][ceil(rows/128)][ceil(k/128)]. */
+int mm_cast_weight_block128(const void* w, int type, int experts, int rows, int k, void* q, float* sf, void* stream);
+
+/* out[m, n] = sum over blocks kb of k of (a[m, kb] . b[e][n, kb]) * sa[m][kb] * sb[e][n/128][kb]; bf16 or fp32 output, fp32 sums.
+ * Dense: experts = 1, m_indices null.  Grouped: m is a multiple of 128, the rows of 128-row block i belong to expert
+ * m_indices[128 i] and rows with m_indices -1 are left as they were.  weights_tiled: b as [expert][ceil(n/256)][k/128][256][128]
+ * bytes (n, k multiples of 128), else [expert][n][k] with k a multiple of 16. */
+int mm_fp8_gemm_block128(const void* a, int64_t a_stride, const float* sa, int64_t sa_stride, const void* b, const float* sb, int experts,
+                         int weights_tiled, const int* m_indices, void* out, int64_t out_stride, int out_fp32, int64_t m, int n, int k,
+                         void* stream);
+
+/* Norms around a block, its gate and the scaled residual, in one pass over [tokens, hidden] (hidden a multiple of 8, at most 16384):
+ *   r_out = alpha r + gate * (y * rsqrt(mean y^2 + eps) * (post + offset)),  x = r_out * rsqrt(mean r_out^2 + eps) * (pre + offset).
+ * y, post, gate, pre and the outputs that depend on them may be null; without y the residual is only normed and r_out is null.
+ * gate: element (t, h) at gate[t * gate_row_stride + h * gate_col_stride], gate_col_stride 0 or 1.  quant: 0 = no codes, 1 = codes of
+ * x with sf[tokens][ceil(hidden/128)], 2 = with sf[tokens] (the channelwise layer's inputs).  r_out has the type of r. */
+int mm_norm_gate_residual(const void* y, int y_type, int64_t y_stride, const void* r, int r_type, int64_t r_stride, const void* post,
+                          int post_type, const void* gate, int gate_type, int64_t gate_row_stride, int gate_col_stride, const void* pre,
+                          int pre_type, void* r_out, void* x_out, int x_type, void* q, float* sf, int quant, int tokens, int hidden,
+                          float alpha, float eps, float offset, void* stream);
+
+/* First failure on the current device that these operators have met since the last call, as {code, phase, block, expected, observed},
+ * and clears it; code 0 = none.  Synchronises the stream. */
+int mm_block128_read_status(void* stream, int32_t* out5);
+
 /* JSON description of the build.  Replaces get_mega_moe_hip_build_config, csrc/apis/mega_dcu.hpp:28-39. */
 int mm_build_config(char* json, int capacity);
 
