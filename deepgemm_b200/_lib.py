@@ -61,6 +61,9 @@ _SIGNATURES = {
                                      c_int64, c_int, c_int, c_void_p]),
     "mm_norm_gate_residual": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_void_p, c_int, c_void_p, c_int, c_int64, c_int, c_void_p,
                                       c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_float, c_float, c_void_p]),
+    "mm_moe_few_tokens_workspace": (c_int, [c_int] * 5 + [POINTER(c_int64)]),
+    "mm_moe_few_tokens": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                  c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_int64, c_void_p, c_void_p]),
     "mm_block128_read_status": (c_int, [c_void_p, POINTER(c_int32)]),
     "mm_set_stage_timing": (c_int, [c_int]),
     "mm_get_stage_times": (c_int, [POINTER(c_float), c_int]),

@@ -11,6 +11,7 @@
 #include "../../include/megamoe_b200.h"
 #include "block128.cuh"
 #include "block128_gemm.cuh"
+#include "block128_moe.cuh"
 #include "layout.h"
 
 // abi.cu: error message, launch counter and wait limit of the library
@@ -79,6 +80,7 @@ int device_of(Device** out) {
         B_CUDA(cudaFuncSetAttribute(mm::block128_gemm_kernel<256, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, mm::B128Shape<256>::kSmemBytes));
         B_CUDA(cudaFuncSetAttribute(mm::block128_gemm_kernel<128, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, mm::B128Shape<128>::kSmemBytes));
         B_CUDA(cudaFuncSetAttribute(mm::block128_gemm_kernel<128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, mm::B128Shape<128>::kSmemBytes));
+        B_CUDA(cudaFuncSetAttribute(mm::moe_experts_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, mm::kMoeSmemBytes));
         d.ready = true;
     }
     *out = &d;
@@ -112,6 +114,46 @@ int byte_map(const void* ptr, uint64_t inner, uint64_t rows, uint64_t row_stride
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     B_REQUIRE(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+    return 0;
+}
+
+// Work memory of mm_moe_few_tokens, in bytes from its start
+struct MoeWork {
+    int64_t counters, route_expert, route_w, xq, xsf, act_q, act_sf, rows_out, parts, total;
+    int num_counters, ctr_done1, ctr_done2, ctr_tile1, ctr_tile2, part_rows;
+};
+
+MoeWork moe_work(int T, int E, int K, int H, int I, bool cast, int ctas) {
+    MoeWork w;
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) { const int64_t o = at; at = (at + bytes + 255) / 256 * 256; return o; };
+    const int64_t routes = (int64_t)T * K;
+    const int64_t blocks = (routes < E ? routes : E) + routes / 128;
+    const int64_t nt1 = I / 128, nt2 = (H + 255) / 256;
+    w.ctr_done1 = 32;
+    w.ctr_done2 = w.ctr_done1 + (int)blocks;
+    w.ctr_tile1 = w.ctr_done2 + (int)nt2;
+    w.ctr_tile2 = w.ctr_tile1 + (int)(blocks * nt1);
+    w.num_counters = w.ctr_tile2 + (int)(blocks * nt2);
+    w.part_rows = (int)(routes < 128 ? routes : 128);
+    w.counters = take((int64_t)w.num_counters * 4);
+    w.route_expert = take(routes * 4);
+    w.route_w = take(routes * 4);
+    w.xq = take(cast ? (int64_t)T * H : 0);
+    w.xsf = take(cast ? (int64_t)T * (H / 128) * 4 : 0);
+    w.act_q = take(routes * I);
+    w.act_sf = take(routes * (I / 128) * 4);
+    w.rows_out = take(routes * H * 4);
+    w.parts = take((int64_t)2 * ctas * 2 * w.part_rows * 256 * 4);
+    w.total = at;
+    return w;
+}
+
+int moe_check_shape(int T, int E, int K, int H, int I) {
+    B_REQUIRE(T >= 0 && E > 0 && E <= MM_MAX_EXPERTS && K > 0 && K <= MM_MAX_TOPK && K <= E, "mm_moe_few_tokens: need 0 < topk <= min(experts, %d), experts <= %d",
+              MM_MAX_TOPK, MM_MAX_EXPERTS);
+    B_REQUIRE(H > 0 && I > 0 && H % 128 == 0 && I % 128 == 0 && H <= 32768 && I <= 32768, "mm_moe_few_tokens: hidden sizes must be multiples of 128, at most 32768");
+    B_REQUIRE((int64_t)T * K <= mm::kMoeMaxRoutes, "mm_moe_few_tokens: at most %d routes (tokens x topk)", mm::kMoeMaxRoutes);
     return 0;
 }
 
@@ -258,6 +300,86 @@ int mm_fp8_gemm_block128(const void* a, int64_t a_stride, const float* sa, int64
         if (bn == 256) mm::block128_gemm_kernel<256, false><<<grid, mm::kB128Threads, mm::B128Shape<256>::kSmemBytes, st>>>(tm_a, tm_b, p);
         else mm::block128_gemm_kernel<128, false><<<grid, mm::kB128Threads, mm::B128Shape<128>::kSmemBytes, st>>>(tm_a, tm_b, p);
     }
+    B_LAUNCHED();
+    return 0;
+}
+
+int mm_moe_few_tokens_workspace(int T, int E, int K, int H, int I, int64_t* bytes) {
+    B_REQUIRE(bytes, "mm_moe_few_tokens_workspace: null pointer");
+    if (int rc = moe_check_shape(T, E, K, H, I)) return rc;
+    Device* d;
+    if (int rc = device_of(&d)) return rc;
+    *bytes = moe_work(T, E, K, H, I, true, d->sms).total;
+    return 0;
+}
+
+int mm_moe_few_tokens(const void* x, int x_is_fp8, int64_t x_stride, const float* x_sf, const float* logits, int64_t logits_stride, const void* topk_idx,
+                      int idx_i64, const float* topk_w, const void* w1, const float* s1, const void* w2, const float* s2, int tiled, int T, int E, int K,
+                      int H, int I, float clamp, void* work, int64_t work_bytes, void* y, void* stream_) {
+    if (int rc = moe_check_shape(T, E, K, H, I)) return rc;
+    B_REQUIRE(!isnan(clamp) && clamp > 0.0f, "mm_moe_few_tokens: the clamp must be positive (+inf for none)");
+    if (T == 0) return 0;
+    B_REQUIRE(x && w1 && s1 && w2 && s2 && work && y && (!x_is_fp8 || x_sf), "mm_moe_few_tokens: null pointer");
+    B_REQUIRE((logits != nullptr) != (topk_idx != nullptr) && (!topk_idx || topk_w), "mm_moe_few_tokens: either logits or topk_idx with topk_w");
+    B_REQUIRE(aligned(x, 16) && aligned(w1, 16) && aligned(w2, 16) && aligned(work, 256) && aligned(y, 16) && x_stride % 16 == 0 && x_stride >= H,
+              "mm_moe_few_tokens: x, weights and y must be 16-byte, the work memory 256-byte aligned");
+    B_REQUIRE(!x_is_fp8 || x_stride == H, "mm_moe_few_tokens: codes must be contiguous");
+    B_REQUIRE(!logits || logits_stride >= E, "mm_moe_few_tokens: bad logits stride");
+    Device* d;
+    if (int rc = device_of(&d)) return rc;
+    const MoeWork w = moe_work(T, E, K, H, I, true, d->sms);
+    B_REQUIRE(work_bytes >= w.total, "mm_moe_few_tokens: needs %lld bytes of work memory, has %lld", (long long)w.total, (long long)work_bytes);
+    uint8_t* base = static_cast<uint8_t*>(work);
+    mm::MoeParams p;
+    memset(&p, 0, sizeof(p));
+    p.tokens = T; p.experts = E; p.topk = K; p.hidden = H; p.inter = I;
+    p.logits = logits; p.logits_stride = logits_stride;
+    p.topk_idx = topk_idx; p.idx_i64 = idx_i64; p.topk_w = topk_w;
+    if (x_is_fp8) {
+        p.xq = static_cast<const uint8_t*>(x);
+        p.xsf = x_sf;
+    } else {
+        p.x = x; p.x_stride = x_stride;
+        p.xq_out = base + w.xq; p.xsf_out = reinterpret_cast<float*>(base + w.xsf);
+        p.xq = p.xq_out; p.xsf = p.xsf_out;
+    }
+    p.route_expert = reinterpret_cast<int*>(base + w.route_expert);
+    p.route_w = reinterpret_cast<float*>(base + w.route_w);
+    p.counters = reinterpret_cast<int*>(base + w.counters);
+    p.num_counters = w.num_counters;
+    p.ctr_done1 = w.ctr_done1; p.ctr_done2 = w.ctr_done2; p.ctr_tile1 = w.ctr_tile1; p.ctr_tile2 = w.ctr_tile2;
+    p.s1 = s1; p.s2 = s2; p.tiled = tiled ? 1 : 0;
+    p.act_q = base + w.act_q; p.act_sf = reinterpret_cast<float*>(base + w.act_sf);
+    p.rows_out = reinterpret_cast<float*>(base + w.rows_out);
+    p.parts = reinterpret_cast<float*>(base + w.parts); p.part_rows = w.part_rows;
+    p.y = static_cast<__nv_bfloat16*>(y);
+    p.clamp = clamp;
+    p.status = d->status;
+    p.timeout_ns = mm_detail_pipe_timeout_ns();
+    CUtensorMap tm1, tm2;
+    if (tiled) {
+        if (int rc = byte_map(w1, 128, (uint64_t)E * (I / 128) * (H / 128) * 256, 128, 0, 0, 256, &tm1)) return rc;
+        if (int rc = byte_map(w2, 128, (uint64_t)E * ((H + 255) / 256) * (I / 128) * 256, 128, 0, 0, 256, &tm2)) return rc;
+    } else {
+        if (int rc = byte_map(w1, (uint64_t)H, (uint64_t)E * 2 * I, (uint64_t)H, 0, 0, 128, &tm1)) return rc;
+        if (int rc = byte_map(w2, (uint64_t)I, (uint64_t)E * H, (uint64_t)I, 0, 0, 128, &tm2)) return rc;
+    }
+    cudaStream_t st = static_cast<cudaStream_t>(stream_);
+    mm::moe_route_kernel<<<T, 256, 0, st>>>(p);
+    B_LAUNCHED();
+    // the second launch starts while the first one runs (its barriers, TMEM and tensor maps need nothing of it) and waits on the device
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((unsigned)d->sms);
+    cfg.blockDim = dim3(mm::kB128Threads);
+    cfg.dynamicSmemBytes = mm::kMoeSmemBytes;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    B_CUDA(cudaLaunchKernelEx(&cfg, mm::moe_experts_kernel, tm1, tm2, p));
     B_LAUNCHED();
     return 0;
 }

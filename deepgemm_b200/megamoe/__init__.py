@@ -739,8 +739,8 @@ def swiglu_quant_channelwise_out(x: torch.Tensor, topk_weights: Optional[torch.T
 
 
 from .block128 import (  # noqa: E402  (the modules share this package's library, not each other's names)
-    NormOutputs, cast_to_fp8_block128, cast_weight_to_fp8_block128, check_block128_status, fp8_gemm_nt_block128,
-    m_grouped_fp8_gemm_nt_contiguous_block128, norm_gate_residual,
+    NormOutputs, cast_to_fp8_block128, cast_weight_to_fp8_block128, check_block128_status, fp8_gemm_nt_block128, fp8_moe_few_tokens,
+    m_grouped_fp8_gemm_nt_contiguous_block128, norm_gate_residual, transform_fp8_weights_for_few_tokens,
 )
 
 __all__ = [
@@ -766,6 +766,8 @@ __all__ = [
     "cast_weight_to_fp8_block128",
     "check_block128_status",
     "fp8_gemm_nt_block128",
+    "fp8_moe_few_tokens",
     "m_grouped_fp8_gemm_nt_contiguous_block128",
     "norm_gate_residual",
+    "transform_fp8_weights_for_few_tokens",
 ]

@@ -7,6 +7,7 @@ checkpoint quantised by blocks cannot be converted to that without a second roun
   cast_to_fp8_block128, cast_weight_to_fp8_block128      bf16 / fp16 / fp32 -> codes and scales
   fp8_gemm_nt_block128                                   dense product
   m_grouped_fp8_gemm_nt_contiguous_block128              product of rows grouped by expert
+  fp8_moe_few_tokens                                     a whole mixture-of-experts layer for a few tokens, on one GPU
   norm_gate_residual                                     norms around a block with its gate, scaled residual and either cast
 
 Calls are asynchronous on the current stream of the tensors' device, keep nothing between calls and may be captured into a CUDA
@@ -15,6 +16,7 @@ graph.  `check_block128_status()` reports what a kernel could not (a bounded wai
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -190,6 +192,121 @@ def m_grouped_fp8_gemm_nt_contiguous_block128(a: Tuple[torch.Tensor, torch.Tenso
     if check:
         check_block128_status(device)
     return d
+
+
+def transform_fp8_weights_for_few_tokens(l1_weights: torch.Tensor, l2_weights: torch.Tensor, layout: str = "tiled"):
+    """bf16, fp16 or fp32 [E, 2I, H] (gate rows, then up rows) and [E, H, I] -> ((w1, s1 [E, 2I/128, H/128]), (w2, s2 [E, H/128, I/128])).
+    layout="tiled" packs the codes in the order the kernel streams them (`pack_weights_tiled`), "native" keeps [E, rows, K]."""
+    if layout not in ("tiled", "native"):
+        raise ValueError("layout must be 'tiled' or 'native'")
+    if l1_weights.dim() != 3 or l2_weights.dim() != 3:
+        raise ValueError("MoE weights must be 3D tensors")
+    (w1, s1), (w2, s2) = cast_weight_to_fp8_block128(l1_weights), cast_weight_to_fp8_block128(l2_weights)
+    if layout == "tiled":
+        from . import pack_weights_tiled
+        w1, w2 = pack_weights_tiled(w1, "l1"), pack_weights_tiled(w2, "l2")
+    return (w1, s1), (w2, s2)
+
+
+@lru_cache(maxsize=256)
+def _moe_work_bytes(device: int, t: int, e: int, k: int, h: int, i: int) -> int:
+    out = ctypes.c_int64()
+    with torch.cuda.device(device):
+        _lib.check(_lib.lib().mm_moe_few_tokens_workspace(t, e, k, h, i, ctypes.byref(out)))
+    return out.value
+
+
+def fp8_moe_few_tokens(x, l1_weights: Tuple[torch.Tensor, torch.Tensor], l2_weights: Tuple[torch.Tensor, torch.Tensor], *,
+                       router_logits: Optional[torch.Tensor] = None, num_topk: Optional[int] = None, topk_idx: Optional[torch.Tensor] = None,
+                       topk_weights: Optional[torch.Tensor] = None, activation_clamp: Optional[float] = None,
+                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A whole mixture-of-experts layer for a few tokens (T * topk <= 4096 routes), in two launches on one GPU:
+
+        y[t] = sum over slots of weight * W2[e] . cast(silu(g) * u),    (g, u) = W1[e] . cast(x[t])
+
+    x: bf16 [T, H], or (codes [T, H], scales [T, H/128]) as the casts of this module give them.  Routing: router_logits fp32 [T, E] with
+    num_topk -- the largest logits, ties to the lower index, softmax over the chosen ones, as `fill_inputs_from_router`; NaN and -inf
+    (closed experts) are never chosen -- or topk_idx (int32 or int64) and topk_weights fp32, both [T, topk]; an index outside 0 .. E-1 or a
+    weight of 0 is no route.  A token without any route gets zeros.  Weights: `transform_fp8_weights_for_few_tokens`, tiled or native.
+    activation_clamp bounds gate and up to +-clamp, as in `fp8_mega_moe`.
+
+    Sums, SwiGLU and the combine are fp32; the output bf16 [T, H] is rounded once.  Each call takes its work memory from torch's
+    allocator.  For many tokens per expert use the grouped product, for channelwise weights or several GPUs `fp8_mega_moe`."""
+    name = "fp8_moe_few_tokens"
+    x_sf = None
+    if isinstance(x, (tuple, list)):
+        x, x_sf = x
+    (w1, s1), (w2, s2) = l1_weights, l2_weights
+    device = _require_cuda(name, x, x_sf, w1, s1, w2, s2, router_logits, topk_idx, topk_weights, out)
+    if x.dim() != 2 or x.dtype != (torch.bfloat16 if x_sf is None else _E4M3):
+        raise RuntimeError(f"{name} expects x as bfloat16 [T, H] or as e4m3 codes with their scales")
+    if w1.dtype != _E4M3 or w2.dtype != _E4M3 or s1.dtype != torch.float32 or s2.dtype != torch.float32:
+        raise RuntimeError(f"{name} expects e4m3 weights with fp32 scales")
+    t, h = x.shape
+    if s1.dim() != 3 or s2.dim() != 3 or s1.shape[1] % 2 != 0:
+        raise RuntimeError(f"{name} expects weight scales [E, 2I/128, H/128] and [E, H/128, I/128]")
+    e, i = s1.shape[0], s1.shape[1] * 64
+    if h == 0 or i == 0 or h % 128 != 0 or tuple(s1.shape) != (e, i // 64, h // 128) or tuple(s2.shape) != (e, h // 128, i // 128):
+        raise RuntimeError(f"{name}: weight scales {tuple(s1.shape)} and {tuple(s2.shape)} do not match H = {h}")
+    tiled = w1.dim() == 5
+    if tiled:
+        ok = tuple(w1.shape) == (e, i // 128, h // 128, 256, 128) and tuple(w2.shape) == (e, (h + 255) // 256, i // 128, 256, 128)
+    else:
+        ok = tuple(w1.shape) == (e, 2 * i, h) and tuple(w2.shape) == (e, h, i)
+    if not ok:
+        raise RuntimeError(f"{name}: weights {tuple(w1.shape)} and {tuple(w2.shape)} do not match their scales (both native or both tiled)")
+    for v in (w1, w2):
+        if not v.is_contiguous() or v.data_ptr() % 16 != 0:
+            raise RuntimeError(f"{name}: weights must be contiguous and 16-byte aligned")
+    if (router_logits is None) == (topk_idx is None):
+        raise ValueError(f"{name}: pass either router_logits with num_topk, or topk_idx with topk_weights")
+    if router_logits is not None:
+        if num_topk is None or topk_weights is not None:
+            raise ValueError(f"{name}: router_logits need num_topk and no topk_weights")
+        if router_logits.dtype != torch.float32 or tuple(router_logits.shape) != (t, e):
+            raise RuntimeError(f"{name}: router_logits must be fp32 [{t}, {e}]")
+        k = int(num_topk)
+        router_logits = _scale_rows(router_logits)
+    else:
+        if topk_weights is None or topk_idx.dim() != 2 or topk_idx.shape[0] != t or topk_idx.shape != topk_weights.shape:
+            raise RuntimeError(f"{name}: topk_idx and topk_weights must both be [{t}, topk]")
+        if topk_idx.dtype not in (torch.int32, torch.int64) or topk_weights.dtype != torch.float32:
+            raise RuntimeError(f"{name}: topk_idx must be int32 or int64, topk_weights fp32")
+        k = topk_idx.shape[1]
+        if num_topk is not None and num_topk != k:
+            raise ValueError(f"{name}: num_topk does not match topk_idx")
+        topk_idx, topk_weights = topk_idx.contiguous(), topk_weights.contiguous()
+    if not 0 < k <= min(e, 32):
+        raise ValueError(f"{name}: topk must be in 1..{min(e, 32)}")
+    if t * k > 4096:
+        raise ValueError(f"{name}: {t} tokens x {k} experts are more than 4096 routes; use the grouped product")
+    if x_sf is not None and (x_sf.dtype != torch.float32 or tuple(x_sf.shape) != (t, h // 128)):
+        raise RuntimeError(f"{name}: scales of x must be fp32 [{t}, {h // 128}]")
+    clamp = float("inf") if activation_clamp is None else float(activation_clamp)
+    if not clamp > 0:
+        raise ValueError(f"{name}: activation_clamp must be positive")
+    if out is None:
+        out = torch.empty((t, h), dtype=torch.bfloat16, device=device)
+    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (t, h) or not out.is_contiguous() or out.data_ptr() % 16 != 0:
+        raise RuntimeError(f"{name}: out must be a contiguous bfloat16 [{t}, {h}], 16-byte aligned")
+    if t == 0:
+        return out
+    if x_sf is None:
+        x = _rows_of(x, 32)              # 16 values
+        stride = max(x.stride(0), h)
+    else:
+        x, x_sf, stride = x.contiguous(), x_sf.contiguous(), h
+        if x.data_ptr() % 16 != 0:
+            x = x.clone()
+    s1, s2 = s1.contiguous(), s2.contiguous()
+    nbytes = _moe_work_bytes(device.index, t, e, k, h, i)
+    work = torch.empty((nbytes,), dtype=torch.uint8, device=device)
+    logits = router_logits
+    _call(device, _lib.lib().mm_moe_few_tokens, x.data_ptr(), x_sf is not None, stride, None if x_sf is None else x_sf.data_ptr(),
+          None if logits is None else logits.data_ptr(), 0 if logits is None else max(logits.stride(0), e), None if topk_idx is None else topk_idx.data_ptr(),
+          topk_idx is not None and topk_idx.dtype == torch.int64, None if topk_weights is None else topk_weights.data_ptr(), w1.data_ptr(), s1.data_ptr(),
+          w2.data_ptr(), s2.data_ptr(), tiled, t, e, k, h, i, clamp, work.data_ptr(), nbytes, out.data_ptr())
+    return out
 
 
 def check_block128_status(device: Optional[torch.device] = None) -> None:

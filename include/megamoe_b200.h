@@ -167,6 +167,22 @@ int mm_norm_gate_residual(const void* y, int y_type, int64_t y_stride, const voi
                           int pre_type, void* r_out, void* x_out, int x_type, void* q, float* sf, int quant, int tokens, int hidden,
                           float alpha, float eps, float offset, void* stream);
 
+/* A whole mixture-of-experts layer for a few tokens (T * K <= 4096 routes) in two launches, on one GPU, without a symmetric buffer:
+ *   y[t] = sum over s of w[t][s] * W2[e] cast(silu(g) u),  (g, u) = W1[e] cast(x[t]),  e = topk[t][s]
+ * with e4m3 weights scaled by 128 x 128 blocks and casts of 128 values; fp32 sums, one rounding to bf16 at the end.
+ * x: bf16 [T][x_stride] (cast here), or (x_is_fp8) codes [T][H] with x_sf [T][H/128].  Routing: logits f32 [T][logits_stride] -- the K
+ * largest (ties to the lower index; NaN and -inf are never chosen) weighted with a softmax over them -- or topk_idx [T][K] (int32, or
+ * int64 if idx_i64) with topk_w [T][K]; an index outside 0 .. E-1 or a weight of 0 is no route, and a token without routes gets zeros.
+ * w1 [E][2I][H] (rows 0 .. I-1 gate), s1 [E][2I/128][H/128]; w2 [E][H][I], s2 [E][H/128][I/128]; tiled: w1 and w2 packed as for
+ * mm_fp8_w8a8_mega_moe.  clamp: of gate and up to +-clamp, +inf for none.  work: at least mm_moe_few_tokens_workspace bytes, 256-byte
+ * aligned, its contents are not read from one call to the next; calls that may run at the same time need work memory of their own.
+ * Stands in for the layer above where weights are scaled by blocks and no other rank takes part; the reference has no such path. */
+int mm_moe_few_tokens_workspace(int T, int E, int K, int H, int I, int64_t* bytes);
+int mm_moe_few_tokens(const void* x, int x_is_fp8, int64_t x_stride, const float* x_sf, const float* logits, int64_t logits_stride,
+                      const void* topk_idx, int idx_i64, const float* topk_w, const void* w1, const float* s1, const void* w2,
+                      const float* s2, int tiled, int T, int E, int K, int H, int I, float clamp, void* work, int64_t work_bytes,
+                      void* y, void* stream);
+
 /* First failure on the current device that these operators have met since the last call, as {code, phase, block, expected, observed},
  * and clears it; code 0 = none.  Synchronises the stream. */
 int mm_block128_read_status(void* stream, int32_t* out5);
