@@ -120,7 +120,7 @@ int byte_map(const void* ptr, uint64_t inner, uint64_t rows, uint64_t row_stride
 // Work memory of mm_moe_few_tokens, in bytes from its start
 struct MoeWork {
     int64_t counters, route_expert, route_w, xq, xsf, act_q, act_sf, rows_out, parts, total;
-    int num_counters, ctr_done1, ctr_done2, ctr_tile1, ctr_tile2, part_rows;
+    int num_counters, ctr_done1, ctr_done2, ctr_tile1, ctr_tile2, part_rows, act_sf_pitch;
 };
 
 MoeWork moe_work(int T, int E, int K, int H, int I, bool cast, int ctas) {
@@ -142,9 +142,10 @@ MoeWork moe_work(int T, int E, int K, int H, int I, bool cast, int ctas) {
     w.xq = take(cast ? (int64_t)T * H : 0);
     w.xsf = take(cast ? (int64_t)T * (H / 128) * 4 : 0);
     w.act_q = take(routes * I);
-    w.act_sf = take(routes * (I / 128) * 4);
+    w.act_sf_pitch = (I / 128 + 31) / 32 * 32;
+    w.act_sf = take(routes * w.act_sf_pitch * 4);
     w.rows_out = take(routes * H * 4);
-    w.parts = take((int64_t)2 * ctas * 2 * w.part_rows * 256 * 4);
+    w.parts = take((int64_t)5 * ctas * w.part_rows * 256 * 4);
     w.total = at;
     return w;
 }
@@ -349,7 +350,7 @@ int mm_moe_few_tokens(const void* x, int x_is_fp8, int64_t x_stride, const float
     p.num_counters = w.num_counters;
     p.ctr_done1 = w.ctr_done1; p.ctr_done2 = w.ctr_done2; p.ctr_tile1 = w.ctr_tile1; p.ctr_tile2 = w.ctr_tile2;
     p.s1 = s1; p.s2 = s2; p.tiled = tiled ? 1 : 0;
-    p.act_q = base + w.act_q; p.act_sf = reinterpret_cast<float*>(base + w.act_sf);
+    p.act_q = base + w.act_q; p.act_sf = reinterpret_cast<float*>(base + w.act_sf); p.act_sf_pitch = w.act_sf_pitch;
     p.rows_out = reinterpret_cast<float*>(base + w.rows_out);
     p.parts = reinterpret_cast<float*>(base + w.parts); p.part_rows = w.part_rows;
     p.y = static_cast<__nv_bfloat16*>(y);

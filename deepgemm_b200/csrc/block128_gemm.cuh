@@ -5,9 +5,11 @@
 // The tensor core sums one block of 128 k exactly as it would any product; the scales change from block to block, so each
 // block's accumulator is read back from TMEM, multiplied and added to fp32 sums in registers, while the tensor core works on
 // the next block in another TMEM buffer.  For a 128 x 256 tile that is 32768 values for each 512 cycles of MMA at the e4m3
-// rate: 8 epilogue warps hold 128 sums per thread and take two of them with each fma.rn.f32x2.
+// rate: 8 epilogue warps hold 128 sums per thread.
 //
-// One CTA per SM, 384 threads: warp 0 = TMA, warp 1 = MMA, warp 2 owns TMEM, warps 4-11 = epilogue (registers moved to them).
+// One CTA per SM, 384 threads: warp 0 = TMA, warp 1 = MMA, warps 2-3 = scales, warps 4-11 = epilogue (registers moved to them).  The
+// scales of a k block travel with its operands, copied to a ring of their own in shared memory: read from global memory by the epilogue
+// they cost it an L2 latency now and then, and every cycle of the epilogue counts.
 // kSplit > 1: the CTAs of a cluster share one tile and divide its k blocks; the fp32 parts meet in distributed shared memory
 // and are added in rank order, so the result does not depend on timing.
 #pragma once
@@ -45,17 +47,36 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap
         ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
         : "memory");
 }
+// Bounded wait like mbar_wait, for hand-overs that follow one another every few hundred cycles: the clock is not read before the wait
+// has failed a thousand times, because reading it costs more than such a hand-over.
+__device__ __forceinline__ bool mbar_wait_often(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t timeout_ns) {
+    uint64_t t0 = 0;
+    for (uint32_t it = 1;; ++it) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((it & 1023u) != 0u) continue;
+        if (*abort_flag != 0) return false;
+        const uint64_t t = global_timer_ns();
+        if (t0 == 0) t0 = t;
+        else if (t - t0 > timeout_ns) { *abort_flag = 1; return false; }
+    }
+}
 template <int kRegs> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 template <int kRegs> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 
 // Two fp32 sums at a time.
-__device__ __forceinline__ uint64_t pack_f32x2(uint32_t lo, uint32_t hi) {
+__device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi) {
     uint64_t v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
     return v;
 }
-__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& lo, float& hi) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+__device__ __forceinline__ float2 unpack_f32x2(uint64_t v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+__device__ __forceinline__ float4 unpack_f32x4(uint64_t a, uint64_t b) {
+    const float2 x = unpack_f32x2(a), y = unpack_f32x2(b);
+    return make_float4(x.x, x.y, y.x, y.y);
 }
 __device__ __forceinline__ void fma_f32x2(uint64_t& acc, uint64_t a, uint64_t b) {
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
@@ -76,9 +97,14 @@ template <int kBN> struct B128Shape {
     static constexpr int kABytes = 128 * 128;
     static constexpr int kBBytes = kBN * 128;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kStagingBytes = 8 * 32 * 33 * 4;            // a 32 x 32 fp32 piece for each epilogue warp
+    // Scales of a k block: 128 rows, then two of the weights.  A stage is filled when the MMA that read it last is done; the epilogue
+    // may be as many blocks behind that as there are accumulators, and one more.
+    static constexpr int kScaleSlots = 16;
+    static_assert(kScaleSlots >= kStages + kAccs + 1, "scale ring");
+    static constexpr int kScaleBytes = 544;
+    static constexpr int kStagingBytes = 8 * 32 * 17 * 4;            // a 32 x 16 fp32 piece for each epilogue warp
     static constexpr int kBarBytes = 256;
-    static constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + kBarBytes;
+    static constexpr int kSmemBytes = kStages * kStageBytes + kScaleSlots * kScaleBytes + kStagingBytes + kBarBytes;
     static_assert(kSmemBytes <= 232448, "exceeds the 227 KiB of shared memory a CTA can have");
     static_assert(128 * (kBN + 4) * 4 <= kStages * kStageBytes, "the fp32 part of a split tile fits in the operand ring");
 };
@@ -93,25 +119,38 @@ __device__ __forceinline__ void b128_tile(const B128GemmParams& p, int tile, int
     mt = g * 8 + r - nt * gm;
 }
 
-// Adds one k block's accumulator (kCols columns of this warp's 32 lanes at `taddr`) times `s` to the sums.
-template <int kCols>
-__device__ __forceinline__ void b128_promote(uint64_t (&acc)[kCols / 2], uint32_t taddr, float s, uint32_t free_bar, int lane) {
-    const uint64_t s2 = pack_f32x2(__float_as_uint(s), __float_as_uint(s));
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+
+// Adds kCols columns of one k block's accumulator (this warp's 32 lanes, from `taddr` on) times `s` to the sums; kLast: they are the
+// warp's last ones, the tensor core may have the buffer back.  Two sums with each fma: plain fma is as fast by itself, but takes twice the
+// issue slots, and the thread that issues the MMAs sits on one of the same four schedulers: beside plain fma four MMAs took 955 cycles,
+// beside fma.rn.f32x2 512, their own rate.  64 columns a step: 336 cycles for a k block, 394 with 32.
+template <int kCols, bool kLast, int kStep = 64>
+__device__ __forceinline__ void b128_promote(uint64_t* sum, uint32_t taddr, float s, uint32_t free_bar, int lane) {
+    const uint64_t s2 = pack_f32x2(s, s);
 #pragma unroll
-    for (int c = 0; c < kCols; c += 64) {
-        uint32_t v0[32], v1[32];
-        tmem_ld_32x32(taddr + c, v0);
-        tmem_ld_32x32(taddr + c + 32, v1);
+    for (int c = 0; c < kCols; c += kStep) {
+        uint32_t v[kStep / 32][32];
+#pragma unroll
+        for (int i = 0; i < kStep / 32; ++i) tmem_ld_32x32(taddr + c + 32 * i, v[i]);
         tmem_ld_wait();
-        if (c + 64 >= kCols) {                       // all of it is in registers: the tensor core may have the buffer back
+        if (kLast && c + kStep >= kCols) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(free_bar);
         }
 #pragma unroll
-        for (int j = 0; j < 16; ++j) fma_f32x2(acc[c / 2 + j], pack_f32x2(v0[2 * j], v0[2 * j + 1]), s2);
+        for (int i = 0; i < kStep / 32; ++i)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) fma_f32x2(acc[c / 2 + 16 + j], pack_f32x2(v1[2 * j], v1[2 * j + 1]), s2);
+            for (int j = 0; j < 16; ++j)
+                fma_f32x2(sum[c / 2 + 16 * i + j], pack_f32x2(__uint_as_float(v[i][2 * j]), __uint_as_float(v[i][2 * j + 1])), s2);
     }
 }
 
@@ -123,8 +162,9 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     constexpr int kCols = kBN / 2;                               // columns of a tile that one epilogue thread sums
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t smem_base = smem_u32(smem);
-    uint8_t* staging = smem + kStages * S::kStageBytes;
-    const uint32_t bars = smem_base + kStages * S::kStageBytes + S::kStagingBytes;
+    uint8_t* scales = smem + kStages * S::kStageBytes;
+    uint8_t* staging = scales + S::kScaleSlots * S::kScaleBytes;
+    const uint32_t bars = smem_u32(staging) + S::kStagingBytes;
     auto full_bar = [&](int s) { return bars + 8u * s; };
     auto empty_bar = [&](int s) { return bars + 8u * (kStages + s); };
     auto tfull_bar = [&](int a) { return bars + 8u * (2 * kStages + a); };
@@ -147,7 +187,7 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     const int kb1 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (part + 1) / split);
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+        for (int s = 0; s < kStages; ++s) { mbar_init(full_bar(s), 3); mbar_init(empty_bar(s), 1); }
         for (int a = 0; a < kAccs; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), 8); }
         *abort_flag = 0;
         fence_barrier_init();
@@ -171,7 +211,7 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     };
 
     if (warp < 4) {
-        regs_dec<88>();
+        regs_dec<56>();
         if (warp == 0 && lane == 0) {
             // ------------------------------------------------------------------ TMA
             int stage = 0; uint32_t phase = 0;
@@ -184,7 +224,7 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                 if (e < 0) continue;
                 const int64_t tiled0 = (static_cast<int64_t>(e) * p.tiled_n_blocks + (nt * kBN) / 256) * p.k_blocks;
                 for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
+                    if (!mbar_wait_often(empty_bar(stage), phase ^ 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
                     const uint32_t a_dst = smem_base + stage * S::kStageBytes;
                     mbar_arrive_expect_tx(full_bar(stage), bytes);
                     if (p.tiled) tma_load_2d(a_dst + S::kABytes, &tm_b, 0, static_cast<int32_t>((tiled0 + kb) * 256 + (nt * kBN) % 256), full_bar(stage));
@@ -204,29 +244,67 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                 b128_tile(p, tile, mt, nt);
                 if (tile_expert(mt) < 0) continue;
                 for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
-                    if (!mbar_wait(full_bar(stage), phase, abort_flag, p.timeout_ns)) { alive = false; break; }
+                    if (!mbar_wait_often(tempty_bar(acc), acc_phase ^ 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
+                    if (!mbar_wait_often(full_bar(stage), phase, abort_flag, p.timeout_ns)) { alive = false; break; }
                     tc_fence_after();
                     const uint64_t da = umma_desc_k_sw128(smem_base + stage * S::kStageBytes);
                     const uint64_t db = umma_desc_k_sw128(smem_base + stage * S::kStageBytes + S::kABytes);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) umma_f8(tmem_base + acc * kBN, da + 2u * k, db + 2u * k, idesc, k != 0 ? 1u : 0u);
+                    umma_commit(tfull_bar(acc));             // first: the epilogue is what the loop waits for
                     umma_commit(empty_bar(stage));
-                    umma_commit(tfull_bar(acc));
                     if (++stage == kStages) { stage = 0; phase ^= 1u; }
                     if (++acc == kAccs) { acc = 0; acc_phase ^= 1u; }
                 }
             }
+        } else if (warp >= 2) {
+            // ------------------------------------------------------------------ scales, two rows a lane
+            constexpr int kAhead = 2;                        // copies in flight before the oldest is handed over
+            int stage = 0; uint32_t phase = 0;
+            int slot = 0, hand = 0, pending = 0;
+            bool alive = true;
+            const int l64 = threadIdx.x - 64;
+            auto hand_over = [&]() {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full_bar(hand));
+                if (++hand == kStages) hand = 0;
+                --pending;
+            };
+            for (int tile = first_tile; tile < num_tiles && alive; tile += tile_step) {
+                int mt, nt;
+                b128_tile(p, tile, mt, nt);
+                const int e = tile_expert(mt);
+                if (e < 0) continue;
+                const float* sa0 = p.sa + static_cast<int64_t>(min(mt * 128 + l64, p.m - 1)) * p.sa_stride;
+                const float* sa1 = p.sa + static_cast<int64_t>(min(mt * 128 + 64 + l64, p.m - 1)) * p.sa_stride;
+                const float* sb = p.sb + (static_cast<int64_t>(e) * p.n_sf + min(nt * (kBN / 128) + (l64 & 1), p.n_sf - 1)) * p.k_blocks;
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (!mbar_wait_often(empty_bar(stage), phase ^ 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
+                    const uint32_t dst = smem_u32(scales) + slot * S::kScaleBytes + l64 * 4;
+                    cp_async_4(dst, sa0 + kb);
+                    cp_async_4(dst + 256, sa1 + kb);
+                    if (l64 < 2) cp_async_4(dst + 512, sb + kb);
+                    cp_async_commit();
+                    ++pending;
+                    if (++stage == kStages) { stage = 0; phase ^= 1u; }
+                    if (++slot == S::kScaleSlots) slot = 0;
+                    if (pending > kAhead) { cp_async_wait<kAhead>(); hand_over(); }
+                }
+            }
+            cp_async_wait<0>();
+            while (pending > 0) hand_over();
         }
         __syncwarp();
     } else {
         // ---------------------------------------------------------------------- epilogue
-        regs_inc<208>();
+        regs_inc<224>();
         const int q = warp & 3;                              // TMEM lane quarter of this warp
         const int half = (warp - 4) >> 2;                    // which half of the columns
         const int et = q * 32 + lane;                        // row of the tile
-        float* my_staging = reinterpret_cast<float*>(staging) + (warp - 4) * 32 * 33;
+        float* my_staging = reinterpret_cast<float*>(staging) + (warp - 4) * 32 * 17;
+        const float* my_scales = reinterpret_cast<const float*>(scales);
         int acc = 0; uint32_t acc_phase = 0;
+        int slot = 0;
         bool alive = true;
         for (int tile = first_tile; tile < num_tiles && alive; tile += tile_step) {
             int mt, nt;
@@ -244,20 +322,18 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
             const int row = mt * 128 + et;
             bool row_ok = row < p.m;
             if (row_ok && p.m_indices != nullptr) row_ok = p.m_indices[row] == e;
-            const float* sa = p.sa + static_cast<int64_t>(row < p.m ? row : 0) * p.sa_stride;
-            const int n_block = min(nt * (kBN / 128) + (kBN == 256 ? half : 0), p.n_sf - 1);
-            const float* sb = p.sb + (static_cast<int64_t>(e) * p.n_sf + n_block) * p.k_blocks;
             uint64_t sum[kCols / 2];
 #pragma unroll
             for (int j = 0; j < kCols / 2; ++j) sum[j] = 0ull;
-            float s_next = sa[kb0] * sb[kb0];
+#pragma unroll 1
             for (int kb = kb0; kb < kb1; ++kb) {
-                const float s = s_next;
-                if (kb + 1 < kb1) s_next = sa[kb + 1] * sb[kb + 1];
-                if (!mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.timeout_ns)) { alive = false; break; }
+                if (!mbar_wait_often(tfull_bar(acc), acc_phase, abort_flag, p.timeout_ns)) { alive = false; break; }
                 tc_fence_after();
-                b128_promote<kCols>(sum, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * kBN + half * kCols, s, tempty_bar(acc), lane);
+                const float* sc = my_scales + slot * (S::kScaleBytes / 4);
+                const float s = sc[et] * sc[128 + (kBN == 256 ? half : 0)];
+                b128_promote<kCols, true>(sum, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * kBN + half * kCols, s, tempty_bar(acc), lane);
                 if (++acc == kAccs) { acc = 0; acc_phase ^= 1u; }
+                if (++slot == S::kScaleSlots) slot = 0;
             }
             if (!alive) break;
             if (kSplit) {
@@ -265,12 +341,7 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                 // was complete, so every copy and every MMA of this CTA is done)
                 float* mine = reinterpret_cast<float*>(smem) + et * (kBN + 4) + half * kCols;
 #pragma unroll
-                for (int j = 0; j < kCols / 2; j += 2) {
-                    float4 f;
-                    unpack_f32x2(sum[j], f.x, f.y);
-                    unpack_f32x2(sum[j + 1], f.z, f.w);
-                    *reinterpret_cast<float4*>(mine + 2 * j) = f;
-                }
+                for (int j = 0; j < kCols; j += 4) *reinterpret_cast<float4*>(mine + j) = unpack_f32x4(sum[j / 2], sum[j / 2 + 1]);
                 continue;
             }
             const int col0 = nt * kBN + half * kCols;
@@ -279,38 +350,38 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                     if (p.out_fp32) {
                         float* o = static_cast<float*>(p.out) + row * p.out_stride + col0;
 #pragma unroll
-                        for (int j = 0; j < kCols / 2; j += 4) {
+                        for (int j = 0; j < kCols; j += 8) {
                             uint32_t v[8];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) { float a, b; unpack_f32x2(sum[j + i], a, b); v[2 * i] = __float_as_uint(a); v[2 * i + 1] = __float_as_uint(b); }
-                            st_global_32b(o + 2 * j, v);
+                            for (int i = 0; i < 4; ++i) { const float2 f = unpack_f32x2(sum[j / 2 + i]); v[2 * i] = __float_as_uint(f.x); v[2 * i + 1] = __float_as_uint(f.y); }
+                            st_global_32b(o + j, v);
                         }
                     } else {
                         __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + row * p.out_stride + col0;
 #pragma unroll
-                        for (int j = 0; j < kCols / 2; j += 8) {
+                        for (int j = 0; j < kCols; j += 16) {
                             uint32_t v[8];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) { float a, b; unpack_f32x2(sum[j + i], a, b); v[i] = pack_bf16x2(a, b); }
-                            st_global_32b(o + 2 * j, v);
+                            for (int i = 0; i < 8; ++i) { const float2 f = unpack_f32x2(sum[j / 2 + i]); v[i] = pack_bf16x2(f.x, f.y); }
+                            st_global_32b(o + j, v);
                         }
                     }
                 }
             } else {
-                // any number of columns and any alignment: 32 columns at a time through shared memory, so that a warp writes
+                // any number of columns and any alignment: 16 columns at a time through shared memory, so that half a warp writes
                 // neighbouring columns of one row
+                const unsigned rows_ok = __ballot_sync(0xffffffffu, row_ok);
 #pragma unroll
-                for (int c = 0; c < kCols; c += 32) {
+                for (int c = 0; c < kCols; c += 16) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) unpack_f32x2(sum[c / 2 + j], my_staging[lane * 33 + 2 * j], my_staging[lane * 33 + 2 * j + 1]);
+                    for (int j = 0; j < 8; ++j) { const float2 f = unpack_f32x2(sum[c / 2 + j]); my_staging[lane * 17 + 2 * j] = f.x; my_staging[lane * 17 + 2 * j + 1] = f.y; }
                     __syncwarp();
-                    const unsigned rows_ok = __ballot_sync(0xffffffffu, row_ok);
-                    const int col = col0 + c + lane;
-                    for (int r = 0; r < 32; ++r) {
+                    const int col = col0 + c + (lane & 15);
+                    for (int r = lane >> 4; r < 32; r += 2) {
                         if (!((rows_ok >> r) & 1u) || col >= p.n) continue;
                         const int64_t at = (mt * 128 + q * 32 + r) * p.out_stride + col;
-                        if (p.out_fp32) static_cast<float*>(p.out)[at] = my_staging[r * 33 + lane];
-                        else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16(my_staging[r * 33 + lane]);
+                        if (p.out_fp32) static_cast<float*>(p.out)[at] = my_staging[r * 17 + (lane & 15)];
+                        else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16(my_staging[r * 17 + (lane & 15)]);
                     }
                     __syncwarp();
                 }

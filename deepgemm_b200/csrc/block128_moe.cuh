@@ -29,13 +29,21 @@ namespace mm {
 
 constexpr int kMoeMaxRoutes = 4096;
 constexpr int kMoeMaxBlocks = MM_MAX_EXPERTS + kMoeMaxRoutes / 128;      // of up to 128 routes of one expert
-constexpr int kMoeStages = 4;
-constexpr int kMoeABytes = 128 * 128;
-constexpr int kMoeStageBytes = kMoeABytes + 256 * 128;
-constexpr int kMoePlanBytes = kMoeMaxRoutes * 4 + kMoeMaxBlocks * 8;
-constexpr int kMoeSmemBytes = kMoeStages * kMoeStageBytes + kMoePlanBytes + 1024 /* row maxima */ + 512 /* barriers */;
+constexpr int kMoeBBytes = 256 * 128;
+// The operand ring: four stages with room for 128 token rows, or five with room for 48 where no expert has more.  (An MMA reads 128 rows
+// either way; those behind the last route are whatever the ring holds there, and their sums are not looked at.)
+constexpr int kMoeMaxStages = 5, kMoeFewRows = 48;
+constexpr int kMoeRingBytes = 4 * (128 * 128 + kMoeBBytes);
+static_assert(kMoeMaxStages * (kMoeFewRows * 128 + kMoeBBytes) <= kMoeRingBytes, "the ring of few rows");
+constexpr int kMoePlanBytes = kMoeMaxRoutes * 2 + kMoeMaxBlocks * 8 + kMoeMaxRoutes / 8;
+constexpr int kMoeTurnRows = 8, kMoeTurnPitch = 260;    // fp32 rows that change hands between the epilogue warps
+// Scales of a unit: 128 rows, then two of the weights.  As in block128_gemm.cuh: stages + accumulators + 1 units may be on their way.
+constexpr int kMoeScaleSlots = 8, kMoeScaleBytes = 544;
+static_assert(kMoeScaleSlots >= kMoeMaxStages + 2 + 1, "scale ring");
+constexpr int kMoeSmemBytes = kMoeRingBytes + kMoePlanBytes + kMoeTurnRows * kMoeTurnPitch * 4 + kMoeScaleSlots * kMoeScaleBytes + 512 /* barriers */;
 static_assert(kMoeSmemBytes <= 232448, "exceeds the 227 KiB of shared memory a CTA can have");
 constexpr int kMoeClaims = 4;
+constexpr int kMoeCtrTiles1 = 16;
 constexpr int kMoeStreamTiles = 16;        // tiles per SM below which chunks are equal shares
 
 struct MoeParams {
@@ -49,14 +57,16 @@ struct MoeParams {
     uint8_t* xq_out; float* xsf_out;
     int* route_expert; float* route_w;       // [tokens * topk], -1 = none
     int* counters; int num_counters;
-    // counters: [0] claims, [32 ..) finished tiles of the first product by block of routes, then of the second by output tile, then
-    // k blocks that have arrived for each tile that was cut, of either product
+    // counters: [0] claims, [kMoeCtrTiles1] finished tiles of the first product, [32 ..) of them by block of routes, then
+    // of the second by output tile, then k blocks that have arrived for each tile that was cut, of either product
     int ctr_done1, ctr_done2, ctr_tile1, ctr_tile2;
     const float* s1; const float* s2;
     int tiled;
-    uint8_t* act_q; float* act_sf;           // [routes][inter], [routes][inter / 128], by place in the sorted list
+    // [routes][inter] and [routes][inter / 128], by place in the sorted list.  A row of scales has 128-byte lines of its own: they are
+    // read through L1, which must not hold a line that another expert's tiles are still writing to
+    uint8_t* act_q; float* act_sf; int act_sf_pitch;
     float* rows_out;                         // [routes][hidden]: weighted rows of the second product, by route
-    float* parts; int part_rows;             // [2 products][chunks][2][part_rows][256]
+    float* parts; int part_rows;             // [2 products][chunks][2][part_rows][256], then [CTAs][part_rows][256] for tiles that are whole
     __nv_bfloat16* y;
     float clamp;
     int* status;
@@ -141,12 +151,11 @@ __global__ void __launch_bounds__(256) moe_route_kernel(const MoeParams p) {
 // The list of weight blocks of one product: tiles * kb units, cut into chunks.
 struct MoeList {
     int tiles, kb, chunks;
-    bool shares;                                                     // chunks are equal shares, else tiles
-    __device__ __forceinline__ int start(int c) const {
-        return shares ? static_cast<int>(static_cast<int64_t>(tiles) * kb * c / chunks) : c * kb;
-    }
+    int shares;                                                     // chunks are equal shares, else tiles
+    // shares: tiles < 16 CTAs and kb <= 256 keep the products below 2^31
+    __device__ __forceinline__ int start(int c) const { return shares ? static_cast<int>(static_cast<uint32_t>(tiles * kb) * c / chunks) : c * kb; }
     __device__ __forceinline__ int chunk_of(int unit) const {        // the chunk c with start(c) <= unit < start(c + 1)
-        return shares ? static_cast<int>(((static_cast<int64_t>(unit) + 1) * chunks - 1) / (static_cast<int64_t>(tiles) * kb)) : unit / kb;
+        return shares ? static_cast<int>((static_cast<uint32_t>(unit + 1) * chunks - 1) / static_cast<uint32_t>(tiles * kb)) : unit / kb;
     }
 };
 __device__ __forceinline__ MoeList moe_list(int tiles, int kb, int ctas) {
@@ -157,80 +166,235 @@ __device__ __forceinline__ MoeList moe_list(int tiles, int kb, int ctas) {
     return l;
 }
 
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kLeft> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
-
-// 64 columns of one accumulator
-template <bool kLast>
-__device__ __forceinline__ void moe_promote64(uint64_t* acc, uint32_t taddr, float s, uint32_t free_bar, int lane) {
-    const uint64_t s2 = pack_f32x2(__float_as_uint(s), __float_as_uint(s));
-    uint32_t v0[32], v1[32];
-    tmem_ld_32x32(taddr, v0);
-    tmem_ld_32x32(taddr + 32, v1);
-    tmem_ld_wait();
-    if (kLast) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(free_bar);
+// Shared memory behind the operand ring
+struct MoeWords {
+    int abort;
+    uint32_t tmem;
+    int claim[kMoeClaims];
+    volatile int last;                                   // the boss's answer to the other epilogue warps
+    int blocks, most;                                    // blocks of routes, routes of the most popular expert
+    int ready;                                           // blocks of routes whose activations this CTA knows to be finished
+    MoeList list[2];                                     // of either product
+};
+struct MoeSmem {
+    float* turn;                                         // [kMoeTurnRows][kMoeTurnPitch]
+    uint2* block;                                        // blocks of routes: expert | rows << 16, first place
+    uint32_t* valid;                                     // a bit for each route
+    uint16_t* route;                                     // routes sorted by expert
+    float* scale;                                        // [slots][128 rows, 2 of the weights, 6 unused]
+    uint32_t bars;
+    MoeWords* words;
+    static constexpr int kBars = 2 * kMoeMaxStages + 5 + 2 * kMoeClaims;
+    static_assert(8 * kBars + sizeof(MoeWords) <= 512, "barriers");
+    __device__ __forceinline__ explicit MoeSmem(uint8_t* smem) {
+        turn = reinterpret_cast<float*>(smem + kMoeRingBytes);
+        block = reinterpret_cast<uint2*>(turn + kMoeTurnRows * kMoeTurnPitch);
+        valid = reinterpret_cast<uint32_t*>(block + kMoeMaxBlocks);
+        route = reinterpret_cast<uint16_t*>(valid + kMoeMaxRoutes / 32);
+        scale = reinterpret_cast<float*>(route + kMoeMaxRoutes);
+        uint8_t* tail = reinterpret_cast<uint8_t*>(scale) + kMoeScaleSlots * kMoeScaleBytes;
+        bars = smem_u32(tail);
+        words = reinterpret_cast<MoeWords*>(tail + 8 * kBars);
     }
-#pragma unroll
-    for (int j = 0; j < 16; ++j) fma_f32x2(acc[j], pack_f32x2(v0[2 * j], v0[2 * j + 1]), s2);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) fma_f32x2(acc[16 + j], pack_f32x2(v1[2 * j], v1[2 * j + 1]), s2);
+    __device__ __forceinline__ uint32_t esync_bar() const { return bars + 8u * (kBars - 1); }
+};
+
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int32_t c0, int32_t c1) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1) : "memory");
 }
 
-// Bounded wait until *p (written by other CTAs, released) has reached `want`.
+// silu(gate) * up of one row's block of 128, four columns a lane, and its cast
+__device__ __forceinline__ void moe_finish_row(const MoeParams& p, float4 g4, float4 u4, bool do_clamp, int64_t place, int nt, int lane) {
+    const float g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
+    float v[4];
+    uint32_t top_bits = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float a = g[i], b = u[i];
+        if (do_clamp) {                                              // NaN stays NaN
+            a = a < -p.clamp ? -p.clamp : (a > p.clamp ? p.clamp : a);
+            b = b < -p.clamp ? -p.clamp : (b > p.clamp ? p.clamp : b);
+        }
+        v[i] = silu_f(a) * b;
+        top_bits = max(top_bits, abs_bits(v[i]));
+    }
+    const float top = group_top(__reduce_max_sync(0xffffffffu, top_bits));
+    const GroupQuotient quot(top);
+    *reinterpret_cast<uint32_t*>(p.act_q + place * p.inter + nt * 128 + lane * 4) = pack4_e4m3(quot(v[0]), quot(v[1]), quot(v[2]), quot(v[3]));
+    if (lane == 0) p.act_sf[place * p.act_sf_pitch + nt] = __fdiv_rn(top, 448.0f);
+}
+__device__ __forceinline__ void add4(float4& a, const float4& b) { a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w; }
+
+// Bounded wait until *p (written by other CTAs, released) has reached `want`.  One thread of a CTA asks, and not without pause: with every
+// warp of every CTA asking (1480 pollers), the counts themselves got through so slowly that a single token took 80 to 150 us.
 __device__ __forceinline__ bool moe_wait_count(const int* p, int want, volatile int* abort_flag, uint64_t timeout_ns) {
-    if (ld_acquire_gpu(p) >= want) return true;
     const uint64_t t0 = global_timer_ns();
     while (ld_acquire_gpu(p) < want) {
         if (*abort_flag != 0) return false;
         if (global_timer_ns() - t0 > timeout_ns) { *abort_flag = 1; return false; }
+        __nanosleep(100);
     }
     return true;
 }
+__device__ __forceinline__ void st_release_cta(uint32_t addr, int v) { asm volatile("st.release.cta.shared::cta.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+__device__ __forceinline__ int ld_acquire_cta(uint32_t addr) {
+    int v;
+    asm volatile("ld.acquire.cta.shared::cta.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+// Bounded wait, a warp at a time, until this CTA knows that the activations of block of routes `rb` are finished; returns how many are, or 0.
+__device__ __forceinline__ int moe_wait_ready(uint32_t ready, int rb, int lane, volatile int* abort_flag, uint64_t timeout_ns) {
+    int n = 0;
+    if (lane == 0) {
+        const uint64_t t0 = global_timer_ns();
+        while ((n = ld_acquire_cta(ready)) <= rb) {
+            n = 0;
+            if (*abort_flag != 0) break;
+            if (global_timer_ns() - t0 > timeout_ns) { *abort_flag = 1; break; }
+        }
+    }
+    n = __shfl_sync(0xffffffffu, n, 0);
+    __syncwarp();
+    return n;
+}
+__device__ __forceinline__ int atomic_add_acq_rel(int* p, int v) {
+    int old;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
+    return old;
+}
+
+// Work memory for the sums of a tile, [part_rows][256]: of a part, by the chunk that brought it (a chunk holds two at most, one that its
+// beginning cuts off and one its end), or of a whole tile, one for each CTA.
+__device__ __forceinline__ float* moe_part(const MoeParams& p, const MoeList& l, int kind, int ch, int tile, bool whole) {
+    const int64_t at = whole ? static_cast<int64_t>(gridDim.x) * 4 + blockIdx.x
+                             : (static_cast<int64_t>(kind) * gridDim.x + ch) * 2 + (l.start(ch) > tile * l.kb ? 0 : 1);
+    return p.parts + at * p.part_rows * 256;
+}
+
+// What the eight epilogue warps do with a tile, or a part of one, once its sums have been written down.  Returns the phase of their barrier,
+// or -1 if a wait has run out.  A function of its own, so that none of its values is kept in registers beside the 128 sums.
+__device__ __noinline__ int moe_finish_tile(const MoeParams& p, uint8_t* smem, int kind, int tile, int rb, int nt, int c, int units, int phase) {
+    const MoeSmem sm(smem);
+    const MoeList& l = sm.words->list[kind];
+    const int ew = (threadIdx.x >> 5) - 4, lane = threadIdx.x & 31;
+    const bool boss = threadIdx.x == 128;
+    const bool whole = units == l.kb;
+    const uint2 blk = sm.block[rb];
+    const int rows = blk.x >> 16;
+    const bool turn = whole && rows <= kMoeTurnRows;
+    // Barrier of the eight warps, bounded like every other wait: a warp that has given up does not hold the others.  What the warps
+    // wrote before it is released to the GPU by the boss's count behind it, and what that count acquired they may read behind the
+    // next one (from L2: another SM has written it).
+    auto sync = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sm.esync_bar());
+        const bool ok = mbar_wait_often(sm.esync_bar(), static_cast<uint32_t>(phase), &sm.words->abort, p.timeout_ns);
+        phase ^= 1;
+        return ok;
+    };
+    if (!sync()) return -1;
+    int c0 = c, c1 = c;
+    if (!whole) {
+        // the parts are added up by whoever brings the last one, in the order of the chunks
+        if (boss) sm.words->last = atomic_add_acq_rel(p.counters + (kind ? p.ctr_tile2 : p.ctr_tile1) + tile, units) + units == l.kb;
+        if (!sync()) return -1;
+        if (sm.words->last == 0) return phase;
+        c0 = l.chunk_of(tile * l.kb);
+        c1 = l.chunk_of(tile * l.kb + l.kb - 1);
+    }
+    // four columns from `col` on of a row: up to four parts' loads in flight, added in order
+    auto join = [&](int row, int col) {
+        if (turn) return *reinterpret_cast<const float4*>(sm.turn + row * kMoeTurnPitch + col);
+        float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int ch = c0; ch <= c1; ch += 4) {
+            float4 f[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (ch + i <= c1) f[i] = __ldcg(reinterpret_cast<const float4*>(moe_part(p, l, kind, ch + i, tile, whole) + row * 256 + col));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (ch + i <= c1) add4(t, f[i]);
+        }
+        return t;
+    };
+    if (kind == 0) {
+        // a row at a time for each warp: with one thread to a row, as the sums were held, a tile of few rows would keep eight warps
+        // waiting for the few threads that have any
+        const bool do_clamp = p.clamp < 3.0e38f;
+        for (int r = ew; r < rows; r += 8) moe_finish_row(p, join(r, lane * 4), join(r, 128 + lane * 4), do_clamp, static_cast<int64_t>(blk.y) + r, nt, lane);
+        if (!sync()) return -1;
+        if (boss) {
+            red_release_gpu_add(p.counters + p.ctr_done1 + rb, 1);
+            red_release_gpu_add(p.counters + kMoeCtrTiles1, 1);
+        }
+        return phase;
+    }
+    const int cols = min(256, p.hidden - nt * 256);
+    if (!whole) {
+        for (int r = ew; r < rows; r += 8) {
+            const uint32_t rr = sm.route[blk.y + r];
+            const float w = p.route_w[rr];
+            for (int col = lane * 4; col < cols; col += 128) {
+                const float4 t = join(r, col);
+                *reinterpret_cast<float4*>(p.rows_out + static_cast<int64_t>(rr) * p.hidden + nt * 256 + col) = make_float4(t.x * w, t.y * w, t.z * w, t.w * w);
+            }
+        }
+        if (!sync()) return -1;
+    }
+    if (boss) sm.words->last = atomic_add_acq_rel(p.counters + p.ctr_done2 + nt, 1) == sm.words->blocks - 1;
+    if (!sync()) return -1;
+    if (sm.words->last != 0) {
+        // every expert's rows of these outputs are there: add each token's up, in the order of its slots
+        const int cols4 = cols / 4;
+        for (int i = threadIdx.x - 128; i < p.tokens * cols4; i += kB128EpiThreads) {
+            const int t = i / cols4, col = nt * 256 + (i - t * cols4) * 4;
+            const int r0 = t * p.topk;
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int s = 0; s < p.topk; s += 8) {
+                float4 f[8];
+                bool ok[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int r = r0 + s + j;
+                    ok[j] = s + j < p.topk && ((sm.valid[r >> 5] >> (r & 31)) & 1u);
+                    if (ok[j]) f[j] = __ldcg(reinterpret_cast<const float4*>(p.rows_out + static_cast<int64_t>(r) * p.hidden + col));
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) if (ok[j]) add4(a, f[j]);
+            }
+            *reinterpret_cast<uint2*>(p.y + static_cast<int64_t>(t) * p.hidden + col) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
+        }
+    }
+    return phase;
+}
 
 __global__ void __launch_bounds__(kB128Threads, 1)
-moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_constant__ CUtensorMap tm_w2, const MoeParams p) {
+moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_constant__ CUtensorMap tm_w2, const __grid_constant__ MoeParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t smem_base = smem_u32(smem);
-    uint8_t* plan_gen = smem + kMoeStages * kMoeStageBytes;
-    uint32_t* s_route = reinterpret_cast<uint32_t*>(plan_gen);                       // sorted by expert: token << 16 | route
-    uint2* s_block = reinterpret_cast<uint2*>(plan_gen + kMoeMaxRoutes * 4);         // blocks of routes: expert | rows << 16, first place
-    float* s_max = reinterpret_cast<float*>(plan_gen + kMoePlanBytes);               // [2 halves][128 rows]
-    uint8_t* tail = plan_gen + kMoePlanBytes + 1024;
-    const uint32_t bars = smem_u32(tail);
-    auto full_bar = [&](int s) { return bars + 8u * s; };
-    auto empty_bar = [&](int s) { return bars + 8u * (kMoeStages + s); };
-    auto tfull_bar = [&](int a) { return bars + 8u * (2 * kMoeStages + a); };
-    auto tempty_bar = [&](int a) { return bars + 8u * (2 * kMoeStages + 2 + a); };
-    auto cfull_bar = [&](int c) { return bars + 8u * (2 * kMoeStages + 4 + c); };
-    auto cempty_bar = [&](int c) { return bars + 8u * (2 * kMoeStages + 4 + kMoeClaims + c); };
-    const uint32_t esync_bar = bars + 8u * (2 * kMoeStages + 4 + 2 * kMoeClaims);
-    constexpr int kTail = 8 * (2 * kMoeStages + 5 + 2 * kMoeClaims);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + kTail);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + kTail + 8);
-    volatile int* s_claim = reinterpret_cast<volatile int*>(tail + kTail + 16);      // [kMoeClaims]
-    volatile int* s_last = s_claim + kMoeClaims;
-    int* s_blocks = reinterpret_cast<int*>(tail + kTail + 16) + kMoeClaims + 1;
-    static_assert(kTail + 16 + 4 * (kMoeClaims + 2) <= 512, "barriers");
+    const MoeSmem sm(smem);
+    auto full_bar = [&](int s) { return sm.bars + 8u * s; };
+    auto empty_bar = [&](int s) { return sm.bars + 8u * (kMoeMaxStages + s); };
+    auto tfull_bar = [&](int a) { return sm.bars + 8u * (2 * kMoeMaxStages + a); };
+    auto tempty_bar = [&](int a) { return sm.bars + 8u * (2 * kMoeMaxStages + 2 + a); };
+    auto cfull_bar = [&](int c) { return sm.bars + 8u * (2 * kMoeMaxStages + 4 + c); };
+    auto cempty_bar = [&](int c) { return sm.bars + 8u * (2 * kMoeMaxStages + 4 + kMoeClaims + c); };
+    volatile int* abort_flag = &sm.words->abort;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kMoeStages; ++s) { mbar_init(full_bar(s), 3); mbar_init(empty_bar(s), 1); }
+        for (int s = 0; s < kMoeMaxStages; ++s) { mbar_init(full_bar(s), 3); mbar_init(empty_bar(s), 1); }
         for (int a = 0; a < 2; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), 8); }
         for (int c = 0; c < kMoeClaims; ++c) { mbar_init(cfull_bar(c), 1); mbar_init(cempty_bar(c), 11); }
-        mbar_init(esync_bar, 8);
+        mbar_init(sm.esync_bar(), 8);
         *abort_flag = 0;
+        st_release_cta(smem_u32(&sm.words->ready), 0);
         fence_barrier_init();
         prefetch_tensormap(&tm_w1);
         prefetch_tensormap(&tm_w2);
     }
     if (warp == 1) {
-        tmem_alloc(smem_u32(tmem_slot), 512);
+        tmem_alloc(smem_u32(&sm.words->tmem), 512);
         tmem_relinquish();
     }
     pdl_wait();                                          // routes, cast x and zeroed counters of the first launch
@@ -249,7 +413,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
         }
         __syncthreads();
         if (warp == 0) {
-            int off = 0, blocks = 0;
+            int off = 0, blocks = 0, most = 0;
             for (int e0 = 0; e0 < p.experts; e0 += 32) {             // counts -> first places, and the blocks of each expert
                 const int e = e0 + lane;
                 const int n = e < p.experts ? s_off[e] : 0;
@@ -261,22 +425,28 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                     if (lane >= o) { n_scan += a; b_scan += c; }
                 }
                 const int first = off + n_scan - n;
+                most = max(most, n);
                 for (int i = 0; i < b; ++i)
-                    s_block[blocks + b_scan - b + i] = make_uint2(static_cast<uint32_t>(e) | static_cast<uint32_t>(min(128, n - 128 * i)) << 16, first + 128 * i);
+                    sm.block[blocks + b_scan - b + i] = make_uint2(static_cast<uint32_t>(e) | static_cast<uint32_t>(min(128, n - 128 * i)) << 16, first + 128 * i);
                 if (e < p.experts) s_off[e] = first;
                 off += __shfl_sync(0xffffffffu, n_scan, 31);
                 blocks += __shfl_sync(0xffffffffu, b_scan, 31);
             }
-            if (lane == 0) *s_blocks = blocks;
+            most = __reduce_max_sync(0xffffffffu, most);
+            if (lane == 0) {
+                sm.words->blocks = blocks;
+                sm.words->most = most;
+                sm.words->list[0] = moe_list(blocks * (p.inter / 128), p.hidden / 128, gridDim.x);
+                sm.words->list[1] = moe_list(blocks * ((p.hidden + 255) / 256), p.inter / 128, gridDim.x);
+            }
             __syncwarp();
             for (int r0 = 0; r0 < routes; r0 += 32) {                // place every route, 32 at a time
                 const int r = r0 + lane;
                 const uint32_t e = r < routes ? s_id[r] : 0xffffu;
                 const uint32_t same = __match_any_sync(0xffffffffu, e);
-                if (e != 0xffffu) {
-                    const int at = s_off[e] + __popc(same & ((1u << lane) - 1u));
-                    s_route[at] = static_cast<uint32_t>(r / p.topk) << 16 | static_cast<uint32_t>(r);
-                }
+                if (e != 0xffffu) sm.route[s_off[e] + __popc(same & ((1u << lane) - 1u))] = static_cast<uint16_t>(r);
+                const uint32_t valid = __ballot_sync(0xffffffffu, e != 0xffffu);
+                if (lane == 0) sm.valid[r0 / 32] = valid;
                 __syncwarp();
                 if (e != 0xffffu && (same >> lane) == 1u) s_off[e] += __popc(same);      // the group's last lane
                 __syncwarp();
@@ -287,33 +457,38 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t tmem_base = sm.words->tmem;
 
-    const int n_blocks = *s_blocks;                                  // blocks of routes
+    const int n_blocks = sm.words->blocks;                                  // blocks of routes
+    const bool few_rows = sm.words->most <= kMoeFewRows;
+    const int stages = few_rows ? kMoeMaxStages : 4;
+    const uint32_t a_bytes = few_rows ? kMoeFewRows * 128 : 128 * 128, stage_bytes = a_bytes + kMoeBBytes;
+    const uint32_t topk_magic = 0xffffffffu / static_cast<uint32_t>(p.topk) + 1u;        // r / topk, exact for r < 2^16; topk 1 apart
+    auto token_of = [&](uint32_t r) { return p.topk == 1 ? r : __umulhi(r, topk_magic); };
     const int kb1 = p.hidden / 128, kb2 = p.inter / 128;
     const int nt1 = p.inter / 128, nt2 = (p.hidden + 255) / 256;
-    const MoeList list1 = moe_list(n_blocks * nt1, kb1, gridDim.x), list2 = moe_list(n_blocks * nt2, kb2, gridDim.x);
-    const int chunks1 = list1.chunks, chunks = n_blocks == 0 ? 0 : chunks1 + list2.chunks;
+    const int chunks1 = sm.words->list[0].chunks, chunks = n_blocks == 0 ? 0 : chunks1 + sm.words->list[1].chunks;
 
     // The chunk of claim number i of this CTA, as its consumers read it (a warp at a time; -1 = no more)
     struct Claims { int slot = 0; uint32_t phase = 0; };
     auto next_claim = [&](Claims& c, bool one_thread) {
         int id = -1;
-        if (!mbar_wait(cfull_bar(c.slot), c.phase, abort_flag, p.timeout_ns)) return -1;
-        id = s_claim[c.slot];
+        if (!mbar_wait_often(cfull_bar(c.slot), c.phase, abort_flag, p.timeout_ns)) return -1;
+        id = sm.words->claim[c.slot];
         if (!one_thread) __syncwarp();
         if (one_thread || lane == 0) mbar_arrive(cempty_bar(c.slot));
         if (++c.slot == kMoeClaims) { c.slot = 0; c.phase ^= 1u; }
         return id;
     };
-    // tile number -> (block of routes, output tile): the first product block by block, the second output tile by output tile
+    // tile number -> (block of routes, output tile), block by block: the second product then begins with what was finished first
     auto split_tile = [&](int kind, int tile, int& rb, int& nt) {
-        if (kind == 0) { rb = tile / nt1; nt = tile - rb * nt1; }
-        else { nt = tile / n_blocks; rb = tile - nt * n_blocks; }
+        const int n = kind ? nt2 : nt1;
+        rb = tile / n;
+        nt = tile - rb * n;
     };
 
     if (warp < 4) {
-        regs_dec<88>();
+        regs_dec<56>();
         if (warp == 0) {
             // ------------------------------------------------------------------ claims and weights
             if (lane == 0) {
@@ -322,30 +497,40 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                 int id = chunks > 0 ? atomicAdd(p.counters, 1) : 0;
                 bool alive = true;
                 while (alive) {
-                    if (!mbar_wait(cempty_bar(slot), cphase ^ 1u, abort_flag, p.timeout_ns)) break;
+                    if (!mbar_wait_often(cempty_bar(slot), cphase ^ 1u, abort_flag, p.timeout_ns)) break;
                     const int chunk = id < chunks ? id : -1;
-                    s_claim[slot] = chunk;
+                    sm.words->claim[slot] = chunk;
                     mbar_arrive(cfull_bar(slot));
                     if (++slot == kMoeClaims) { slot = 0; cphase ^= 1u; }
                     if (chunk < 0) break;
-                    id = atomicAdd(p.counters, 1);                   // the next one, wanted only after this one's copies
                     const int kind = chunk >= chunks1 ? 1 : 0;
-                    const MoeList& l = kind ? list2 : list1;
+                    const MoeList& l = sm.words->list[kind];
                     const int c = chunk - (kind ? chunks1 : 0);
                     const CUtensorMap* map = kind ? &tm_w2 : &tm_w1;
                     int u = l.start(c);
                     const int end = l.start(c + 1);
+                    if (kind && p.tiled && l.shares) {
+                        // HBM has nothing to do until the activations of the first product are finished: what of this share the ring
+                        // does not hold goes to L2 meanwhile
+                        for (int v = u + stages; v < min(end, u + stages + 8); ++v) {
+                            const int tile = v / l.kb;
+                            int rb, nt;
+                            split_tile(kind, tile, rb, nt);
+                            const int64_t at = (static_cast<int64_t>(sm.block[rb].x & 0xffff) * nt2 + nt) * l.kb + v - tile * l.kb;
+                            tma_prefetch_2d(map, 0, static_cast<int32_t>(at * 256));
+                        }
+                    }
                     while (u < end && alive) {
                         const int tile = u / l.kb, k0 = u - tile * l.kb, k1 = min(l.kb, k0 + end - u);
                         int rb, nt;
                         split_tile(kind, tile, rb, nt);
-                        const int e = s_block[rb].x & 0xffff;
+                        const int e = sm.block[rb].x & 0xffff;
                         const int64_t tiled0 = (static_cast<int64_t>(e) * (kind ? nt2 : nt1) + nt) * l.kb;
                         const int row_a = kind ? e * p.hidden + nt * 256 : e * 2 * p.inter + nt * 128;
                         const int row_b = kind ? row_a + 128 : row_a + p.inter;
                         for (int k = k0; k < k1; ++k) {
-                            if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
-                            const uint32_t dst = smem_base + stage * kMoeStageBytes + kMoeABytes;
+                            if (!mbar_wait_often(empty_bar(stage), phase ^ 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
+                            const uint32_t dst = smem_base + stage * stage_bytes + a_bytes;
                             mbar_arrive_expect_tx(full_bar(stage), 256 * 128);
                             if (p.tiled) {
                                 tma_load_2d(dst, map, 0, static_cast<int32_t>((tiled0 + k) * 256), full_bar(stage));
@@ -353,10 +538,13 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                                 tma_load_2d(dst, map, k * 128, row_a, full_bar(stage));
                                 tma_load_2d(dst + 128 * 128, map, k * 128, row_b, full_bar(stage));
                             }
-                            if (++stage == kMoeStages) { stage = 0; phase ^= 1u; }
+                            if (++stage == stages) { stage = 0; phase ^= 1u; }
                         }
                         u += k1 - k0;
                     }
+                    // Not before the copies are under way: whoever claims ahead takes a second share while others have none.  The ring
+                    // holds more work than the claim takes.
+                    if (alive) id = atomicAdd(p.counters, 1);
                 }
             }
         } else if (warp == 1) {
@@ -370,18 +558,19 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                 while (alive) {
                     const int chunk = next_claim(claims, true);
                     if (chunk < 0) break;
-                    const int units = chunk >= chunks1 ? list2.start(chunk - chunks1 + 1) - list2.start(chunk - chunks1) : list1.start(chunk + 1) - list1.start(chunk);
+                    const MoeList& l = sm.words->list[chunk >= chunks1 ? 1 : 0];
+                    const int c = chunk - (chunk >= chunks1 ? chunks1 : 0), units = l.start(c + 1) - l.start(c);
                     for (int u = 0; u < units; ++u) {
-                        if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
-                        if (!mbar_wait(full_bar(stage), phase, abort_flag, p.timeout_ns)) { alive = false; break; }
+                        if (!mbar_wait_often(tempty_bar(acc), acc_phase ^ 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
+                        if (!mbar_wait_often(full_bar(stage), phase, abort_flag, p.timeout_ns)) { alive = false; break; }
                         tc_fence_after();
-                        const uint64_t da = umma_desc_k_sw128(smem_base + stage * kMoeStageBytes);
-                        const uint64_t db = umma_desc_k_sw128(smem_base + stage * kMoeStageBytes + kMoeABytes);
+                        const uint64_t da = umma_desc_k_sw128(smem_base + stage * stage_bytes);
+                        const uint64_t db = umma_desc_k_sw128(smem_base + stage * stage_bytes + a_bytes);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) umma_f8(tmem_base + acc * 256, da + 2u * k, db + 2u * k, idesc, k != 0 ? 1u : 0u);
-                        umma_commit(empty_bar(stage));
                         umma_commit(tfull_bar(acc));
-                        if (++stage == kMoeStages) { stage = 0; phase ^= 1u; }
+                        umma_commit(empty_bar(stage));
+                        if (++stage == stages) { stage = 0; phase ^= 1u; }
                         if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
                     }
                 }
@@ -390,16 +579,18 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
             // ------------------------------------------------------------------ token operand: rows gathered by route, 16 bytes a lane
             constexpr int kAhead = 2;                                // copies in flight before the oldest is handed over
             int stage = 0; uint32_t phase = 0;                       // next stage to fill
+            int slot = 0;                                            // next place in the ring of scales
             int hand = 0, pending = 0;                               // next stage to hand over, stages filled but not handed over
             const int l64 = threadIdx.x - 64;
             const int piece = l64 & 7;
+            int ready_blocks = 0;                                    // this CTA's chunks of the second product go up in blocks of routes
             Claims claims;
             bool alive = true;
             auto hand_over = [&]() {
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(full_bar(hand));
-                if (++hand == kMoeStages) hand = 0;
+                if (++hand == stages) hand = 0;
                 --pending;
             };
             auto drain = [&]() {
@@ -407,46 +598,68 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                 while (pending > 0) hand_over();
             };
             while (alive) {
-                if (!mbar_try_wait(cfull_bar(claims.slot), claims.phase)) drain();       // no chunk to go on with yet
+                if (!__all_sync(0xffffffffu, mbar_try_wait(cfull_bar(claims.slot), claims.phase))) drain();       // no chunk to go on with yet
                 const int chunk = next_claim(claims, false);
                 if (chunk < 0) break;
                 const int kind = chunk >= chunks1 ? 1 : 0;
-                const MoeList& l = kind ? list2 : list1;
+                const MoeList& l = sm.words->list[kind];
                 const int c = chunk - (kind ? chunks1 : 0);
                 const int pitch = kind ? p.inter : p.hidden;
                 const uint8_t* src = kind ? p.act_q : p.xq;
+                const float* src_sf = kind ? p.act_sf : p.xsf;
+                const int sf_pitch = kind ? p.act_sf_pitch : kb1;
                 int u = l.start(c);
                 const int end = l.start(c + 1);
                 while (u < end && alive) {
                     const int tile = u / l.kb, k0 = u - tile * l.kb, k1 = min(l.kb, k0 + end - u);
                     int rb, nt;
                     split_tile(kind, tile, rb, nt);
-                    const uint2 blk = s_block[rb];
-                    const int rows = blk.x >> 16, first = blk.y;
-                    if (kind) {
-                        // the rows this product reads: everything filled so far is handed over first, because the tiles that finish
-                        // them may be this CTA's own
-                        bool ready = false;
-                        if (lane == 0) ready = ld_acquire_gpu(p.counters + p.ctr_done1 + rb) >= nt1;
-                        ready = __shfl_sync(0xffffffffu, ready, 0);
-                        if (!ready) {
-                            drain();
-                            if (lane == 0) ready = moe_wait_count(p.counters + p.ctr_done1 + rb, nt1, abort_flag, p.timeout_ns);
-                            ready = __shfl_sync(0xffffffffu, ready, 0);
-                            if (!ready) { alive = false; break; }
+                    const uint2 blk = sm.block[rb];
+                    const int e = blk.x & 0xffff, rows = blk.x >> 16, first = blk.y;
+                    // the last two lanes bring the weights' scales: gate and up, or two blocks of outputs (the last tile may have one)
+                    const int n_block = kind ? min(2 * nt + (l64 & 1), kb1 - 1) : nt + (l64 & 1) * nt1;
+                    const float* sb = kind ? p.s2 + (static_cast<int64_t>(e) * kb1 + n_block) * kb2 : p.s1 + (static_cast<int64_t>(e) * 2 * nt1 + n_block) * kb1;
+                    if (kind && rb >= ready_blocks) {
+                        // The rows this product reads.  One warp asks for both, and if it has to wait, everything filled so far is handed
+                        // over first, because the tiles that finish those rows may be this CTA's own.
+                        if (warp == 2) {
+                            auto look = [&]() {                      // lane 0: all tiles of the first product, or at least this block's
+                                const int all = ld_acquire_gpu(p.counters + kMoeCtrTiles1), own = ld_acquire_gpu(p.counters + p.ctr_done1 + rb);
+                                return all >= n_blocks * nt1 ? n_blocks : own >= nt1 ? rb + 1 : 0;
+                            };
+                            ready_blocks = __shfl_sync(0xffffffffu, lane == 0 ? look() : 0, 0);
+                            if (ready_blocks == 0) {
+                                drain();
+                                int n = 0;
+                                if (lane == 0 && moe_wait_count(p.counters + p.ctr_done1 + rb, nt1, abort_flag, p.timeout_ns)) n = max(look(), rb + 1);
+                                ready_blocks = __shfl_sync(0xffffffffu, n, 0);
+                            }
+                            if (ready_blocks == 0) { alive = false; break; }
+                            if (lane == 0) st_release_cta(smem_u32(&sm.words->ready), ready_blocks);
+                            __syncwarp();                            // what lane 0 has acquired, the others may read
+                        } else {
+                            if (ld_acquire_cta(smem_u32(&sm.words->ready)) <= rb) drain();
+                            ready_blocks = moe_wait_ready(smem_u32(&sm.words->ready), rb, lane, abort_flag, p.timeout_ns);
+                            if (ready_blocks == 0) { alive = false; break; }
                         }
-                        __syncwarp();                                // what lane 0 has acquired, the others may read
                     }
                     for (int k = k0; k < k1; ++k) {
-                        if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
-                        const uint32_t dst = smem_base + stage * kMoeStageBytes;
+                        if (!mbar_wait_often(empty_bar(stage), phase ^ 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
+                        const uint32_t sdst = smem_u32(sm.scale) + slot * kMoeScaleBytes;
+                        for (int r = l64; r < rows; r += 64) {
+                            const uint32_t row = kind ? first + r : token_of(sm.route[first + r]);
+                            cp_async_4(sdst + r * 4, src_sf + static_cast<int64_t>(row) * sf_pitch + k);
+                        }
+                        if (l64 >= 62) cp_async_4(sdst + 512 + (l64 - 62) * 4, sb + k);
+                        if (++slot == kMoeScaleSlots) slot = 0;
+                        const uint32_t dst = smem_base + stage * stage_bytes;
                         for (int r = l64 >> 3; r < rows; r += 8) {
-                            const int row = kind ? first + r : static_cast<int>(s_route[first + r] >> 16);
+                            const uint32_t row = kind ? first + r : token_of(sm.route[first + r]);
                             cp_async_16(dst + r * 128 + ((piece ^ (r & 7)) << 4), src + static_cast<int64_t>(row) * pitch + k * 128 + piece * 16);
                         }
                         cp_async_commit();
                         ++pending;
-                        if (++stage == kMoeStages) { stage = 0; phase ^= 1u; }
+                        if (++stage == stages) { stage = 0; phase ^= 1u; }
                         if (pending > kAhead) {
                             cp_async_wait<kAhead>();
                             hand_over();
@@ -460,23 +673,14 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
         __syncwarp();
     } else {
         // ---------------------------------------------------------------------- epilogue
-        regs_inc<208>();
+        regs_inc<224>();
         const int q = warp & 3, half = (warp - 4) >> 2;
         const int et = q * 32 + lane;
-        const bool boss = threadIdx.x == 128;
-        const bool do_clamp = p.clamp < 3.0e38f;
         int acc = 0; uint32_t acc_phase = 0;
-        uint32_t sync_phase = 0;
+        int sync_phase = 0;
+        int slot = 0;                                                // place of the next unit in the ring of scales
         Claims claims;
         bool alive = true;
-        // barrier of the eight epilogue warps, bounded like every other wait: a warp that has given up does not hold the others
-        auto epi_sync = [&]() {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(esync_bar);
-            if (!mbar_wait(esync_bar, sync_phase, abort_flag, p.timeout_ns)) alive = false;
-            sync_phase ^= 1u;
-            return alive;
-        };
         if (n_blocks == 0) {                                         // no route at all: the sum is empty
             for (int64_t i = static_cast<int64_t>(blockIdx.x) * kB128EpiThreads + threadIdx.x - 128; i < static_cast<int64_t>(p.tokens) * p.hidden / 8;
                  i += static_cast<int64_t>(gridDim.x) * kB128EpiThreads)
@@ -486,7 +690,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
             const int chunk = next_claim(claims, false);
             if (chunk < 0) break;
             const int kind = chunk >= chunks1 ? 1 : 0;
-            const MoeList& l = kind ? list2 : list1;
+            const MoeList& l = sm.words->list[kind];
             const int c = chunk - (kind ? chunks1 : 0);
             int u = l.start(c);
             const int end = l.start(c + 1);
@@ -495,175 +699,57 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                 u += k1 - k0;
                 int rb, nt;
                 split_tile(kind, tile, rb, nt);
-                const uint2 blk = s_block[rb];
-                const int e = blk.x & 0xffff, rows = blk.x >> 16, place = static_cast<int>(blk.y) + et;
+                const uint2 blk = sm.block[rb];
+                const int rows = blk.x >> 16, place = static_cast<int>(blk.y) + et;
                 const bool row_ok = et < rows, warp_ok = q * 32 < rows;
-                const uint32_t route = row_ok ? s_route[place] : 0u;
-                if (kind && warp_ok) {                               // scales of the activations: written by other CTAs
-                    bool ready = true;
-                    if (lane == 0) ready = moe_wait_count(p.counters + p.ctr_done1 + rb, nt1, abort_flag, p.timeout_ns);
-                    if (!__shfl_sync(0xffffffffu, ready, 0)) { alive = false; break; }
-                    __syncwarp();
-                }
-                const float* sa = kind ? p.act_sf + static_cast<int64_t>(row_ok ? place : 0) * kb2 : p.xsf + static_cast<int64_t>(route >> 16) * kb1;
+                const uint32_t route = row_ok ? sm.route[place] : 0u;
                 // column parts A and B of this thread: gate and up, or two neighbouring runs of 64 outputs
                 const int col_a = kind ? half * 128 : half * 64, col_b = kind ? col_a + 64 : col_a + 128;
-                const float* sb_a;
-                const float* sb_b;
-                if (kind) {
-                    sb_a = p.s2 + (static_cast<int64_t>(e) * (p.hidden / 128) + min(2 * nt + half, p.hidden / 128 - 1)) * kb2;
-                    sb_b = sb_a;
-                } else {
-                    sb_a = p.s1 + (static_cast<int64_t>(e) * 2 * nt1 + nt) * kb1;
-                    sb_b = sb_a + static_cast<int64_t>(nt1) * kb1;
-                }
-                uint64_t sum[64];
+                uint64_t sum[64];                                    // pairs: 64 columns of part A, 64 of part B
 #pragma unroll
                 for (int j = 0; j < 64; ++j) sum[j] = 0ull;
-                float lane_a = 0.0f, lane_b = 0.0f, s_next = 0.0f;       // weight scales of 32 k blocks, one a lane
-                if (warp_ok) s_next = kind ? __ldcg(sa + k0) : sa[k0];
+#pragma unroll 1
                 for (int k = k0; k < k1; ++k) {
-                    const int i = (k - k0) & 31;
-                    if (i == 0 && warp_ok && k + lane < k1) { lane_a = sb_a[k + lane]; lane_b = sb_b[k + lane]; }
-                    const float s_row = s_next;
-                    if (warp_ok && k + 1 < k1) s_next = kind ? __ldcg(sa + k + 1) : sa[k + 1];
-                    const float w_a = __shfl_sync(0xffffffffu, lane_a, i), w_b = __shfl_sync(0xffffffffu, lane_b, i);
-                    if (!mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.timeout_ns)) { alive = false; break; }
+                    if (!mbar_wait_often(tfull_bar(acc), acc_phase, abort_flag, p.timeout_ns)) { alive = false; break; }
                     tc_fence_after();
                     if (warp_ok) {
+                        const float* sc = sm.scale + slot * (kMoeScaleBytes / 4);
+                        const float s_row = sc[et];
                         const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * 256;
-                        moe_promote64<false>(sum, t_addr + col_a, s_row * w_a, 0, lane);
-                        moe_promote64<true>(sum + 32, t_addr + col_b, s_row * w_b, tempty_bar(acc), lane);
-                    } else {
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(tempty_bar(acc));
+                        b128_promote<64, false, 32>(sum, t_addr + col_a, s_row * sc[kind ? 128 + half : 128], 0, lane);
+                        b128_promote<64, true, 32>(sum + 32, t_addr + col_b, s_row * sc[kind ? 128 + half : 129], tempty_bar(acc), lane);
+                    } else if (lane == 0) {
+                        mbar_arrive(tempty_bar(acc));
                     }
+                    if (++slot == kMoeScaleSlots) slot = 0;
                     if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
                 }
                 if (!alive) break;
-                if (k1 - k0 < l.kb) {
-                    // a part of the tile: written down, and added up by whoever brings the last one, in the order of the chunks
-                    const int64_t part_size = static_cast<int64_t>(p.part_rows) * 256;
-                    auto part_of = [&](int ch) {      // a chunk holds two parts at most: one that its beginning cuts off, one its end
-                        const int which = l.start(ch) > tile * l.kb ? 0 : 1;
-                        return p.parts + ((static_cast<int64_t>(kind) * gridDim.x + ch) * 2 + which) * part_size + static_cast<int64_t>(et) * 256 + half * 128;
-                    };
-                    if (row_ok) {
-                        float* o = part_of(c);
+                const bool whole = k1 - k0 == l.kb;
+                // Where the sums go next: rows of activations that are finished here to shared memory if they fit; else, and parts of a
+                // tile, to work memory; whole rows of outputs straight to their place.
+                const bool turn = whole && rows <= kMoeTurnRows;
+                if (row_ok) {
+                    if (kind && whole) {
+                        if (half * 128 < p.hidden - nt * 256) {
+                            const float w = p.route_w[route];
+                            float* o = p.rows_out + static_cast<int64_t>(route) * p.hidden + nt * 256 + half * 128;
 #pragma unroll
-                        for (int j = 0; j < 64; j += 4) {
-                            uint32_t v[8];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) { float a, b; unpack_f32x2(sum[j + i], a, b); v[2 * i] = __float_as_uint(a); v[2 * i + 1] = __float_as_uint(b); }
-                            st_global_32b(o + 2 * j, v);
-                        }
-                    }
-                    __threadfence();
-                    if (!epi_sync()) break;
-                    if (boss) *s_last = atomicAdd(p.counters + (kind ? p.ctr_tile2 : p.ctr_tile1) + tile, k1 - k0) + (k1 - k0) == l.kb;
-                    if (!epi_sync()) break;
-                    if (*s_last == 0) continue;
-                    __threadfence();
-                    if (row_ok) {
-                        const int c0 = l.chunk_of(tile * l.kb), c1 = l.chunk_of(tile * l.kb + l.kb - 1);
-#pragma unroll
-                        for (int j0 = 0; j0 < 64; j0 += 16) {
-                            float t[32];
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) t[j] = 0.0f;
-                            for (int ch = c0; ch <= c1; ++ch) {
-                                const float4* in = reinterpret_cast<const float4*>(part_of(ch) + 2 * j0);
-#pragma unroll
-                                for (int j = 0; j < 8; ++j) {
-                                    const float4 f = __ldcg(in + j);
-                                    t[4 * j] += f.x; t[4 * j + 1] += f.y; t[4 * j + 2] += f.z; t[4 * j + 3] += f.w;
-                                }
+                            for (int j = 0; j < 128; j += 4) {
+                                const float4 f = unpack_f32x4(sum[j / 2], sum[j / 2 + 1]);
+                                *reinterpret_cast<float4*>(o + j) = make_float4(f.x * w, f.y * w, f.z * w, f.w * w);
                             }
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) sum[j0 + j] = pack_f32x2(__float_as_uint(t[2 * j]), __float_as_uint(t[2 * j + 1]));
                         }
+                    } else {
+                        float* o = turn ? sm.turn + et * kMoeTurnPitch : moe_part(p, l, kind, c, tile, whole) + et * 256;
+#pragma unroll
+                        for (int j = 0; j < 128; j += 4)
+                            *reinterpret_cast<float4*>(o + (j < 64 ? col_a + j : col_b + j - 64)) = unpack_f32x4(sum[j / 2], sum[j / 2 + 1]);
                     }
                 }
-                if (kind == 0) {
-                    // silu(gate) * up, and the cast: this thread has half of the block of 128, its partner in the other half the rest
-                    uint32_t top_bits = 0;
-                    if (row_ok) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            float g[2], v[2];
-                            unpack_f32x2(sum[j], g[0], g[1]);
-                            unpack_f32x2(sum[32 + j], v[0], v[1]);
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                if (do_clamp) {                      // NaN stays NaN
-                                    g[i] = g[i] < -p.clamp ? -p.clamp : (g[i] > p.clamp ? p.clamp : g[i]);
-                                    v[i] = v[i] < -p.clamp ? -p.clamp : (v[i] > p.clamp ? p.clamp : v[i]);
-                                }
-                                v[i] *= silu_f(g[i]);
-                                top_bits = max(top_bits, abs_bits(v[i]));
-                            }
-                            sum[j] = pack_f32x2(__float_as_uint(v[0]), __float_as_uint(v[1]));
-                        }
-                        s_max[half * 128 + et] = __uint_as_float(top_bits);
-                    }
-                    if (!epi_sync()) break;
-                    if (row_ok) {
-                        top_bits = max(top_bits, __float_as_uint(s_max[(half ^ 1) * 128 + et]));
-                        const float top = group_top(top_bits);
-                        const GroupQuotient quot(top);
-                        uint4* o = reinterpret_cast<uint4*>(p.act_q + static_cast<int64_t>(place) * p.inter + nt * 128 + half * 64);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            uint32_t w[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                float a, b, d, f;
-                                unpack_f32x2(sum[j * 8 + 2 * i], a, b);
-                                unpack_f32x2(sum[j * 8 + 2 * i + 1], d, f);
-                                w[i] = pack4_e4m3(quot(a), quot(b), quot(d), quot(f));
-                            }
-                            o[j] = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
-                        if (half == 0) p.act_sf[static_cast<int64_t>(place) * kb2 + nt] = __fdiv_rn(top, 448.0f);
-                    }
-                    __threadfence();
-                    if (!epi_sync()) break;
-                    if (boss) red_release_gpu_add(p.counters + p.ctr_done1 + rb, 1);
-                } else {
-                    const int col0 = nt * 256 + half * 128;
-                    if (row_ok && col0 < p.hidden) {
-                        const int r = static_cast<int>(route & 0xffffu);
-                        const float w = p.route_w[r];
-                        float* o = p.rows_out + static_cast<int64_t>(r) * p.hidden + col0;
-#pragma unroll
-                        for (int j = 0; j < 64; j += 4) {
-                            uint32_t v[8];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) { float a, b; unpack_f32x2(sum[j + i], a, b); v[2 * i] = __float_as_uint(a * w); v[2 * i + 1] = __float_as_uint(b * w); }
-                            st_global_32b(o + 2 * j, v);
-                        }
-                    }
-                    __threadfence();
-                    if (!epi_sync()) break;
-                    if (boss) *s_last = atomicAdd(p.counters + p.ctr_done2 + nt, 1) == n_blocks - 1;
-                    if (!epi_sync()) break;
-                    if (*s_last != 0) {
-                        // every expert's rows of these 256 outputs are there: add each token's up, in the order of its slots
-                        __threadfence();
-                        const int cols4 = min(256, p.hidden - nt * 256) / 4;
-                        for (int i = threadIdx.x - 128; i < p.tokens * cols4; i += kB128EpiThreads) {
-                            const int t = i / cols4, col = nt * 256 + (i - t * cols4) * 4;
-                            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-                            for (int s = 0; s < p.topk; ++s) {
-                                const int r = t * p.topk + s;
-                                if (p.route_expert[r] < 0) continue;
-                                const float4 f = __ldcg(reinterpret_cast<const float4*>(p.rows_out + static_cast<int64_t>(r) * p.hidden + col));
-                                a.x += f.x; a.y += f.y; a.z += f.z; a.w += f.w;
-                            }
-                            *reinterpret_cast<uint2*>(p.y + static_cast<int64_t>(t) * p.hidden + col) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
-                        }
-                    }
-                }
+                const int ph = moe_finish_tile(p, smem, kind, tile, rb, nt, c, k1 - k0, sync_phase);
+                if (ph < 0) { alive = false; break; }
+                sync_phase = ph;
             }
         }
     }
