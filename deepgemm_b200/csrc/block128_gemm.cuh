@@ -60,6 +60,9 @@ __device__ __forceinline__ bool mbar_wait_often(uint32_t bar, uint32_t parity, v
         else if (t - t0 > timeout_ns) { *abort_flag = 1; return false; }
     }
 }
+__device__ __forceinline__ void mbar_arrive_n(uint32_t bar, uint32_t n) {
+    asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar), "r"(n) : "memory");
+}
 template <int kRegs> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 template <int kRegs> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 
@@ -129,11 +132,11 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int kLeft> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
 
 // Adds kCols columns of one k block's accumulator (this warp's 32 lanes, from `taddr` on) times `s` to the sums; kLast: they are the
-// warp's last ones, the tensor core may have the buffer back.  Two sums with each fma: plain fma is as fast by itself, but takes twice the
+// warp's last ones, the tensor core may have the buffer back (`arrivals` of the eight that its barrier counts).  Two sums with each fma: plain fma is as fast by itself, but takes twice the
 // issue slots, and the thread that issues the MMAs sits on one of the same four schedulers: beside plain fma four MMAs took 955 cycles,
 // beside fma.rn.f32x2 512, their own rate.  64 columns a step: 336 cycles for a k block, 394 with 32.
 template <int kCols, bool kLast, int kStep = 64>
-__device__ __forceinline__ void b128_promote(uint64_t* sum, uint32_t taddr, float s, uint32_t free_bar, int lane) {
+__device__ __forceinline__ void b128_promote(uint64_t* sum, uint32_t taddr, float s, uint32_t free_bar, uint32_t arrivals, int lane) {
     const uint64_t s2 = pack_f32x2(s, s);
 #pragma unroll
     for (int c = 0; c < kCols; c += kStep) {
@@ -144,7 +147,7 @@ __device__ __forceinline__ void b128_promote(uint64_t* sum, uint32_t taddr, floa
         if (kLast && c + kStep >= kCols) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(free_bar);
+            if (lane == 0) mbar_arrive_n(free_bar, arrivals);
         }
 #pragma unroll
         for (int i = 0; i < kStep / 32; ++i)
@@ -331,7 +334,7 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                 tc_fence_after();
                 const float* sc = my_scales + slot * (S::kScaleBytes / 4);
                 const float s = sc[et] * sc[128 + (kBN == 256 ? half : 0)];
-                b128_promote<kCols, true>(sum, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * kBN + half * kCols, s, tempty_bar(acc), lane);
+                b128_promote<kCols, true>(sum, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * kBN + half * kCols, s, tempty_bar(acc), 1u, lane);
                 if (++acc == kAccs) { acc = 0; acc_phase ^= 1u; }
                 if (++slot == S::kScaleSlots) slot = 0;
             }

@@ -37,13 +37,14 @@ constexpr int kMoeRingBytes = 4 * (128 * 128 + kMoeBBytes);
 static_assert(kMoeMaxStages * (kMoeFewRows * 128 + kMoeBBytes) <= kMoeRingBytes, "the ring of few rows");
 constexpr int kMoePlanBytes = kMoeMaxRoutes * 2 + kMoeMaxBlocks * 8 + kMoeMaxRoutes / 8;
 constexpr int kMoeTurnRows = 8, kMoeTurnPitch = 260;    // fp32 rows that change hands between the epilogue warps
+constexpr int kMoeSegments = 8;
+constexpr int kMoeCtrTiles1 = 16;
+constexpr int kMoeTailBytes = 768;        // barriers and MoeWords
 // Scales of a unit: 128 rows, then two of the weights.  As in block128_gemm.cuh: stages + accumulators + 1 units may be on their way.
 constexpr int kMoeScaleSlots = 8, kMoeScaleBytes = 544;
 static_assert(kMoeScaleSlots >= kMoeMaxStages + 2 + 1, "scale ring");
-constexpr int kMoeSmemBytes = kMoeRingBytes + kMoePlanBytes + kMoeTurnRows * kMoeTurnPitch * 4 + kMoeScaleSlots * kMoeScaleBytes + 512 /* barriers */;
+constexpr int kMoeSmemBytes = kMoeRingBytes + kMoePlanBytes + kMoeTurnRows * kMoeTurnPitch * 4 + kMoeScaleSlots * kMoeScaleBytes + kMoeTailBytes;
 static_assert(kMoeSmemBytes <= 232448, "exceeds the 227 KiB of shared memory a CTA can have");
-constexpr int kMoeClaims = 4;
-constexpr int kMoeCtrTiles1 = 16;
 constexpr int kMoeStreamTiles = 16;        // tiles per SM below which chunks are equal shares
 
 struct MoeParams {
@@ -166,15 +167,25 @@ __device__ __forceinline__ MoeList moe_list(int tiles, int kb, int ctas) {
     return l;
 }
 
+// A run of k blocks of one tile, as the TMA thread walks through its chunks and the other warps follow it.  They read it from shared memory
+// whenever they want something of it: held in registers beside the epilogue's 128 sums it made them spill in the innermost loop.
+struct MoeSegment {
+    int kind;                                            // 0, 1: first or second product; -1: no more
+    int chunk, tile, block, out;                         // chunk and tile of its product; block of routes and output tile
+    int k0, k1;
+    int rows, first;                                     // of the block of routes
+    int expert;
+};
+
 // Shared memory behind the operand ring
 struct MoeWords {
-    int abort;
+    volatile int abort;
     uint32_t tmem;
-    int claim[kMoeClaims];
     volatile int last;                                   // the boss's answer to the other epilogue warps
     int blocks, most;                                    // blocks of routes, routes of the most popular expert
     int ready;                                           // blocks of routes whose activations this CTA knows to be finished
     MoeList list[2];                                     // of either product
+    MoeSegment segment[kMoeSegments];
 };
 struct MoeSmem {
     float* turn;                                         // [kMoeTurnRows][kMoeTurnPitch]
@@ -184,8 +195,8 @@ struct MoeSmem {
     float* scale;                                        // [slots][128 rows, 2 of the weights, 6 unused]
     uint32_t bars;
     MoeWords* words;
-    static constexpr int kBars = 2 * kMoeMaxStages + 5 + 2 * kMoeClaims;
-    static_assert(8 * kBars + sizeof(MoeWords) <= 512, "barriers");
+    static constexpr int kBars = 2 * kMoeMaxStages + 5 + 2 * kMoeSegments;
+    static_assert(8 * kBars + sizeof(MoeWords) <= kMoeTailBytes, "barriers");
     __device__ __forceinline__ explicit MoeSmem(uint8_t* smem) {
         turn = reinterpret_cast<float*>(smem + kMoeRingBytes);
         block = reinterpret_cast<uint2*>(turn + kMoeTurnRows * kMoeTurnPitch);
@@ -273,14 +284,15 @@ __device__ __forceinline__ float* moe_part(const MoeParams& p, const MoeList& l,
 
 // What the eight epilogue warps do with a tile, or a part of one, once its sums have been written down.  Returns the phase of their barrier,
 // or -1 if a wait has run out.  A function of its own, so that none of its values is kept in registers beside the 128 sums.
-__device__ __noinline__ int moe_finish_tile(const MoeParams& p, uint8_t* smem, int kind, int tile, int rb, int nt, int c, int units, int phase) {
+__device__ __noinline__ int moe_finish_tile(const MoeParams& p, uint8_t* smem, int slot, int phase, bool idle) {
     const MoeSmem sm(smem);
+    const MoeSegment& g = sm.words->segment[slot];
+    const int kind = g.kind, tile = g.tile, rb = g.block, nt = g.out, units = g.k1 - g.k0;
     const MoeList& l = sm.words->list[kind];
     const int ew = (threadIdx.x >> 5) - 4, lane = threadIdx.x & 31;
     const bool boss = threadIdx.x == 128;
     const bool whole = units == l.kb;
-    const uint2 blk = sm.block[rb];
-    const int rows = blk.x >> 16;
+    const int rows = g.rows;
     const bool turn = whole && rows <= kMoeTurnRows;
     // Barrier of the eight warps, bounded like every other wait: a warp that has given up does not hold the others.  What the warps
     // wrote before it is released to the GPU by the boss's count behind it, and what that count acquired they may read behind the
@@ -292,8 +304,20 @@ __device__ __noinline__ int moe_finish_tile(const MoeParams& p, uint8_t* smem, i
         phase ^= 1;
         return ok;
     };
-    if (!sync()) return -1;
-    int c0 = c, c1 = c;
+    if (idle) {                                          // a whole tile's time to wait
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sm.esync_bar());
+        const uint64_t t0 = global_timer_ns();
+        while (!mbar_try_wait(sm.esync_bar(), static_cast<uint32_t>(phase))) {
+            __nanosleep(64);
+            if (sm.words->abort != 0) return -1;
+            if (global_timer_ns() - t0 > p.timeout_ns) { sm.words->abort = 1; return -1; }
+        }
+        phase ^= 1;
+    } else if (!sync()) {
+        return -1;
+    }
+    int c0 = g.chunk, c1 = g.chunk;
     if (!whole) {
         // the parts are added up by whoever brings the last one, in the order of the chunks
         if (boss) sm.words->last = atomic_add_acq_rel(p.counters + (kind ? p.ctr_tile2 : p.ctr_tile1) + tile, units) + units == l.kb;
@@ -321,7 +345,7 @@ __device__ __noinline__ int moe_finish_tile(const MoeParams& p, uint8_t* smem, i
         // a row at a time for each warp: with one thread to a row, as the sums were held, a tile of few rows would keep eight warps
         // waiting for the few threads that have any
         const bool do_clamp = p.clamp < 3.0e38f;
-        for (int r = ew; r < rows; r += 8) moe_finish_row(p, join(r, lane * 4), join(r, 128 + lane * 4), do_clamp, static_cast<int64_t>(blk.y) + r, nt, lane);
+        for (int r = ew; r < rows; r += 8) moe_finish_row(p, join(r, lane * 4), join(r, 128 + lane * 4), do_clamp, static_cast<int64_t>(g.first) + r, nt, lane);
         if (!sync()) return -1;
         if (boss) {
             red_release_gpu_add(p.counters + p.ctr_done1 + rb, 1);
@@ -332,7 +356,7 @@ __device__ __noinline__ int moe_finish_tile(const MoeParams& p, uint8_t* smem, i
     const int cols = min(256, p.hidden - nt * 256);
     if (!whole) {
         for (int r = ew; r < rows; r += 8) {
-            const uint32_t rr = sm.route[blk.y + r];
+            const uint32_t rr = sm.route[g.first + r];
             const float w = p.route_w[rr];
             for (int col = lane * 4; col < cols; col += 128) {
                 const float4 t = join(r, col);
@@ -346,21 +370,23 @@ __device__ __noinline__ int moe_finish_tile(const MoeParams& p, uint8_t* smem, i
     if (sm.words->last != 0) {
         // every expert's rows of these outputs are there: add each token's up, in the order of its slots
         const int cols4 = cols / 4;
+#pragma unroll 1
         for (int i = threadIdx.x - 128; i < p.tokens * cols4; i += kB128EpiThreads) {
             const int t = i / cols4, col = nt * 256 + (i - t * cols4) * 4;
             const int r0 = t * p.topk;
             float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int s = 0; s < p.topk; s += 8) {
-                float4 f[8];
-                bool ok[8];
+#pragma unroll 1
+            for (int s = 0; s < p.topk; s += 4) {
+                float4 f[4];
+                bool ok[4];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
+                for (int j = 0; j < 4; ++j) {
                     const int r = r0 + s + j;
                     ok[j] = s + j < p.topk && ((sm.valid[r >> 5] >> (r & 31)) & 1u);
                     if (ok[j]) f[j] = __ldcg(reinterpret_cast<const float4*>(p.rows_out + static_cast<int64_t>(r) * p.hidden + col));
                 }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) if (ok[j]) add4(a, f[j]);
+                for (int j = 0; j < 4; ++j) if (ok[j]) add4(a, f[j]);
             }
             *reinterpret_cast<uint2*>(p.y + static_cast<int64_t>(t) * p.hidden + col) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
         }
@@ -377,15 +403,15 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
     auto empty_bar = [&](int s) { return sm.bars + 8u * (kMoeMaxStages + s); };
     auto tfull_bar = [&](int a) { return sm.bars + 8u * (2 * kMoeMaxStages + a); };
     auto tempty_bar = [&](int a) { return sm.bars + 8u * (2 * kMoeMaxStages + 2 + a); };
-    auto cfull_bar = [&](int c) { return sm.bars + 8u * (2 * kMoeMaxStages + 4 + c); };
-    auto cempty_bar = [&](int c) { return sm.bars + 8u * (2 * kMoeMaxStages + 4 + kMoeClaims + c); };
+    auto sfull_bar = [&](int c) { return sm.bars + 8u * (2 * kMoeMaxStages + 4 + c); };
+    auto sempty_bar = [&](int c) { return sm.bars + 8u * (2 * kMoeMaxStages + 4 + kMoeSegments + c); };
     volatile int* abort_flag = &sm.words->abort;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kMoeMaxStages; ++s) { mbar_init(full_bar(s), 3); mbar_init(empty_bar(s), 1); }
         for (int a = 0; a < 2; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), 8); }
-        for (int c = 0; c < kMoeClaims; ++c) { mbar_init(cfull_bar(c), 1); mbar_init(cempty_bar(c), 11); }
+        for (int c = 0; c < kMoeSegments; ++c) { mbar_init(sfull_bar(c), 1); mbar_init(sempty_bar(c), 11); }
         mbar_init(sm.esync_bar(), 8);
         *abort_flag = 0;
         st_release_cta(smem_u32(&sm.words->ready), 0);
@@ -469,66 +495,66 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
     const int nt1 = p.inter / 128, nt2 = (p.hidden + 255) / 256;
     const int chunks1 = sm.words->list[0].chunks, chunks = n_blocks == 0 ? 0 : chunks1 + sm.words->list[1].chunks;
 
-    // The chunk of claim number i of this CTA, as its consumers read it (a warp at a time; -1 = no more)
-    struct Claims { int slot = 0; uint32_t phase = 0; };
-    auto next_claim = [&](Claims& c, bool one_thread) {
-        int id = -1;
-        if (!mbar_wait_often(cfull_bar(c.slot), c.phase, abort_flag, p.timeout_ns)) return -1;
-        id = sm.words->claim[c.slot];
-        if (!one_thread) __syncwarp();
-        if (one_thread || lane == 0) mbar_arrive(cempty_bar(c.slot));
-        if (++c.slot == kMoeClaims) { c.slot = 0; c.phase ^= 1u; }
-        return id;
+    struct Place { int slot = 0; uint32_t phase = 0; };              // in the ring of segments
+    auto segment_at = [&](const Place& at) -> const MoeSegment* {
+        return mbar_wait_often(sfull_bar(at.slot), at.phase, abort_flag, p.timeout_ns) ? &sm.words->segment[at.slot] : nullptr;
     };
-    // tile number -> (block of routes, output tile), block by block: the second product then begins with what was finished first
-    auto split_tile = [&](int kind, int tile, int& rb, int& nt) {
-        const int n = kind ? nt2 : nt1;
-        rb = tile / n;
-        nt = tile - rb * n;
+    auto segment_done = [&](Place& at) {                             // one thread of a warp, or the MMA thread
+        mbar_arrive(sempty_bar(at.slot));
     };
-
+    auto step = [&](Place& at) { if (++at.slot == kMoeSegments) { at.slot = 0; at.phase ^= 1u; } };
     if (warp < 4) {
         regs_dec<56>();
         if (warp == 0) {
             // ------------------------------------------------------------------ claims and weights
             if (lane == 0) {
                 int stage = 0; uint32_t phase = 0;
-                int slot = 0; uint32_t cphase = 0;
-                int id = chunks > 0 ? atomicAdd(p.counters, 1) : 0;
+                Place at;
                 bool alive = true;
+                auto publish = [&](const MoeSegment& g) {
+                    if (!mbar_wait_often(sempty_bar(at.slot), at.phase ^ 1u, abort_flag, p.timeout_ns)) return false;
+                    sm.words->segment[at.slot] = g;
+                    mbar_arrive(sfull_bar(at.slot));
+                    step(at);
+                    return true;
+                };
                 while (alive) {
-                    if (!mbar_wait_often(cempty_bar(slot), cphase ^ 1u, abort_flag, p.timeout_ns)) break;
-                    const int chunk = id < chunks ? id : -1;
-                    sm.words->claim[slot] = chunk;
-                    mbar_arrive(cfull_bar(slot));
-                    if (++slot == kMoeClaims) { slot = 0; cphase ^= 1u; }
-                    if (chunk < 0) break;
-                    const int kind = chunk >= chunks1 ? 1 : 0;
-                    const MoeList& l = sm.words->list[kind];
-                    const int c = chunk - (kind ? chunks1 : 0);
-                    const CUtensorMap* map = kind ? &tm_w2 : &tm_w1;
-                    int u = l.start(c);
-                    const int end = l.start(c + 1);
-                    if (kind && p.tiled && l.shares) {
+                    // Not before the copies of the last chunk are under way: whoever claims ahead takes a second share while others have
+                    // none.  The ring holds more work than the claim takes.
+                    const int id = chunks > 0 ? atomicAdd(p.counters, 1) : 0;
+                    if (id >= chunks) break;
+                    MoeSegment g;
+                    g.kind = id >= chunks1 ? 1 : 0;
+                    g.chunk = id - (g.kind ? chunks1 : 0);
+                    const MoeList l = sm.words->list[g.kind];
+                    const CUtensorMap* map = g.kind ? &tm_w2 : &tm_w1;
+                    const int per_block = g.kind ? nt2 : nt1;        // tiles go block by block: the second product begins with what was finished first
+                    int u = l.start(g.chunk);
+                    const int end = l.start(g.chunk + 1);
+                    if (g.kind && p.tiled && l.shares) {
                         // HBM has nothing to do until the activations of the first product are finished: what of this share the ring
                         // does not hold goes to L2 meanwhile
                         for (int v = u + stages; v < min(end, u + stages + 8); ++v) {
-                            const int tile = v / l.kb;
-                            int rb, nt;
-                            split_tile(kind, tile, rb, nt);
-                            const int64_t at = (static_cast<int64_t>(sm.block[rb].x & 0xffff) * nt2 + nt) * l.kb + v - tile * l.kb;
-                            tma_prefetch_2d(map, 0, static_cast<int32_t>(at * 256));
+                            const int tile = v / l.kb, rb = tile / nt2;
+                            const int64_t to = (static_cast<int64_t>(sm.block[rb].x & 0xffff) * nt2 + tile - rb * nt2) * l.kb + v - tile * l.kb;
+                            tma_prefetch_2d(map, 0, static_cast<int32_t>(to * 256));
                         }
                     }
                     while (u < end && alive) {
-                        const int tile = u / l.kb, k0 = u - tile * l.kb, k1 = min(l.kb, k0 + end - u);
-                        int rb, nt;
-                        split_tile(kind, tile, rb, nt);
-                        const int e = sm.block[rb].x & 0xffff;
-                        const int64_t tiled0 = (static_cast<int64_t>(e) * (kind ? nt2 : nt1) + nt) * l.kb;
-                        const int row_a = kind ? e * p.hidden + nt * 256 : e * 2 * p.inter + nt * 128;
-                        const int row_b = kind ? row_a + 128 : row_a + p.inter;
-                        for (int k = k0; k < k1; ++k) {
+                        g.tile = u / l.kb;
+                        g.k0 = u - g.tile * l.kb;
+                        g.k1 = min(l.kb, g.k0 + end - u);
+                        g.block = g.tile / per_block;
+                        g.out = g.tile - g.block * per_block;
+                        const uint2 blk = sm.block[g.block];
+                        g.expert = blk.x & 0xffff;
+                        g.rows = blk.x >> 16;
+                        g.first = blk.y;
+                        if (!publish(g)) { alive = false; break; }
+                        const int64_t tiled0 = (static_cast<int64_t>(g.expert) * per_block + g.out) * l.kb;
+                        const int row_a = g.kind ? g.expert * p.hidden + g.out * 256 : g.expert * 2 * p.inter + g.out * 128;
+                        const int row_b = g.kind ? row_a + 128 : row_a + p.inter;
+                        for (int k = g.k0; k < g.k1; ++k) {
                             if (!mbar_wait_often(empty_bar(stage), phase ^ 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
                             const uint32_t dst = smem_base + stage * stage_bytes + a_bytes;
                             mbar_arrive_expect_tx(full_bar(stage), 256 * 128);
@@ -540,12 +566,12 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                             }
                             if (++stage == stages) { stage = 0; phase ^= 1u; }
                         }
-                        u += k1 - k0;
+                        u += g.k1 - g.k0;
                     }
-                    // Not before the copies are under way: whoever claims ahead takes a second share while others have none.  The ring
-                    // holds more work than the claim takes.
-                    if (alive) id = atomicAdd(p.counters, 1);
                 }
+                MoeSegment none;
+                none.kind = -1;
+                if (alive) publish(none);
             }
         } else if (warp == 1) {
             // ------------------------------------------------------------------ MMA
@@ -553,13 +579,14 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                 constexpr uint32_t idesc = umma_idesc_f8(128, 256);
                 int stage = 0; uint32_t phase = 0;
                 int acc = 0; uint32_t acc_phase = 0;
-                Claims claims;
+                Place at;
                 bool alive = true;
                 while (alive) {
-                    const int chunk = next_claim(claims, true);
-                    if (chunk < 0) break;
-                    const MoeList& l = sm.words->list[chunk >= chunks1 ? 1 : 0];
-                    const int c = chunk - (chunk >= chunks1 ? chunks1 : 0), units = l.start(c + 1) - l.start(c);
+                    const MoeSegment* g = segment_at(at);
+                    if (g == nullptr || g->kind < 0) break;
+                    const int units = g->k1 - g->k0;
+                    segment_done(at);
+                    step(at);
                     for (int u = 0; u < units; ++u) {
                         if (!mbar_wait_often(tempty_bar(acc), acc_phase ^ 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
                         if (!mbar_wait_often(full_bar(stage), phase, abort_flag, p.timeout_ns)) { alive = false; break; }
@@ -584,7 +611,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
             const int l64 = threadIdx.x - 64;
             const int piece = l64 & 7;
             int ready_blocks = 0;                                    // this CTA's chunks of the second product go up in blocks of routes
-            Claims claims;
+            Place at;
             bool alive = true;
             auto hand_over = [&]() {
                 fence_proxy_async_smem();
@@ -598,27 +625,23 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                 while (pending > 0) hand_over();
             };
             while (alive) {
-                if (!__all_sync(0xffffffffu, mbar_try_wait(cfull_bar(claims.slot), claims.phase))) drain();       // no chunk to go on with yet
-                const int chunk = next_claim(claims, false);
-                if (chunk < 0) break;
-                const int kind = chunk >= chunks1 ? 1 : 0;
-                const MoeList& l = sm.words->list[kind];
-                const int c = chunk - (kind ? chunks1 : 0);
+                if (!__all_sync(0xffffffffu, mbar_try_wait(sfull_bar(at.slot), at.phase))) drain();      // nothing to go on with yet
+                const MoeSegment* seg = segment_at(at);
+                if (seg == nullptr || seg->kind < 0) break;
+                const MoeSegment g = *seg;
+                __syncwarp();
+                if (lane == 0) segment_done(at);
+                step(at);
+                const int kind = g.kind, rb = g.block, rows = g.rows, first = g.first;
                 const int pitch = kind ? p.inter : p.hidden;
                 const uint8_t* src = kind ? p.act_q : p.xq;
                 const float* src_sf = kind ? p.act_sf : p.xsf;
                 const int sf_pitch = kind ? p.act_sf_pitch : kb1;
-                int u = l.start(c);
-                const int end = l.start(c + 1);
-                while (u < end && alive) {
-                    const int tile = u / l.kb, k0 = u - tile * l.kb, k1 = min(l.kb, k0 + end - u);
-                    int rb, nt;
-                    split_tile(kind, tile, rb, nt);
-                    const uint2 blk = sm.block[rb];
-                    const int e = blk.x & 0xffff, rows = blk.x >> 16, first = blk.y;
+                {
                     // the last two lanes bring the weights' scales: gate and up, or two blocks of outputs (the last tile may have one)
-                    const int n_block = kind ? min(2 * nt + (l64 & 1), kb1 - 1) : nt + (l64 & 1) * nt1;
-                    const float* sb = kind ? p.s2 + (static_cast<int64_t>(e) * kb1 + n_block) * kb2 : p.s1 + (static_cast<int64_t>(e) * 2 * nt1 + n_block) * kb1;
+                    const int n_block = kind ? min(2 * g.out + (l64 & 1), kb1 - 1) : g.out + (l64 & 1) * nt1;
+                    const float* sb = kind ? p.s2 + (static_cast<int64_t>(g.expert) * kb1 + n_block) * kb2
+                                           : p.s1 + (static_cast<int64_t>(g.expert) * 2 * nt1 + n_block) * kb1;
                     if (kind && rb >= ready_blocks) {
                         // The rows this product reads.  One warp asks for both, and if it has to wait, everything filled so far is handed
                         // over first, because the tiles that finish those rows may be this CTA's own.
@@ -643,7 +666,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                             if (ready_blocks == 0) { alive = false; break; }
                         }
                     }
-                    for (int k = k0; k < k1; ++k) {
+                    for (int k = g.k0; k < g.k1; ++k) {
                         if (!mbar_wait_often(empty_bar(stage), phase ^ 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
                         const uint32_t sdst = smem_u32(sm.scale) + slot * kMoeScaleBytes;
                         for (int r = l64; r < rows; r += 64) {
@@ -665,7 +688,6 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                             hand_over();
                         }
                     }
-                    u += k1 - k0;
                 }
             }
             drain();
@@ -679,7 +701,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
         int acc = 0; uint32_t acc_phase = 0;
         int sync_phase = 0;
         int slot = 0;                                                // place of the next unit in the ring of scales
-        Claims claims;
+        Place at;
         bool alive = true;
         if (n_blocks == 0) {                                         // no route at all: the sum is empty
             for (int64_t i = static_cast<int64_t>(blockIdx.x) * kB128EpiThreads + threadIdx.x - 128; i < static_cast<int64_t>(p.tokens) * p.hidden / 8;
@@ -687,53 +709,42 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                 reinterpret_cast<uint4*>(p.y)[i] = make_uint4(0, 0, 0, 0);
         }
         while (alive) {
-            const int chunk = next_claim(claims, false);
-            if (chunk < 0) break;
-            const int kind = chunk >= chunks1 ? 1 : 0;
-            const MoeList& l = sm.words->list[kind];
-            const int c = chunk - (kind ? chunks1 : 0);
-            int u = l.start(c);
-            const int end = l.start(c + 1);
-            while (u < end && alive) {
-                const int tile = u / l.kb, k0 = u - tile * l.kb, k1 = min(l.kb, k0 + end - u);
-                u += k1 - k0;
-                int rb, nt;
-                split_tile(kind, tile, rb, nt);
-                const uint2 blk = sm.block[rb];
-                const int rows = blk.x >> 16, place = static_cast<int>(blk.y) + et;
-                const bool row_ok = et < rows, warp_ok = q * 32 < rows;
-                const uint32_t route = row_ok ? sm.route[place] : 0u;
+            const MoeSegment* g = segment_at(at);
+            if (g == nullptr || g->kind < 0) break;
+            const int units = g->k1 - g->k0;
+            if (q * 32 < g->rows) {
                 // column parts A and B of this thread: gate and up, or two neighbouring runs of 64 outputs
-                const int col_a = kind ? half * 128 : half * 64, col_b = kind ? col_a + 64 : col_a + 128;
+                const int col_a = g->kind ? half * 128 : half * 64, col_b = g->kind ? col_a + 64 : col_a + 128;
+                const int sb_a = g->kind ? 128 + half : 128, sb_b = g->kind ? 128 + half : 129;
+                // Warps without a row of the tile take no part in this: waiting beside the others they slow them down.  The barrier
+                // that gives the accumulator back counts all eight, so the warps of the first rows arrive for the idle ones.
+                const uint32_t arrivals = q == 0 ? 5u - static_cast<uint32_t>((g->rows + 31) >> 5) : 1u;
                 uint64_t sum[64];                                    // pairs: 64 columns of part A, 64 of part B
 #pragma unroll
                 for (int j = 0; j < 64; ++j) sum[j] = 0ull;
 #pragma unroll 1
-                for (int k = k0; k < k1; ++k) {
+                for (int u = 0; u < units; ++u) {
                     if (!mbar_wait_often(tfull_bar(acc), acc_phase, abort_flag, p.timeout_ns)) { alive = false; break; }
                     tc_fence_after();
-                    if (warp_ok) {
-                        const float* sc = sm.scale + slot * (kMoeScaleBytes / 4);
-                        const float s_row = sc[et];
-                        const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * 256;
-                        b128_promote<64, false, 32>(sum, t_addr + col_a, s_row * sc[kind ? 128 + half : 128], 0, lane);
-                        b128_promote<64, true, 32>(sum + 32, t_addr + col_b, s_row * sc[kind ? 128 + half : 129], tempty_bar(acc), lane);
-                    } else if (lane == 0) {
-                        mbar_arrive(tempty_bar(acc));
-                    }
+                    const float* sc = sm.scale + slot * (kMoeScaleBytes / 4);
+                    const float s_row = sc[et];
+                    const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * 256;
+                    b128_promote<64, false>(sum, t_addr + col_a, s_row * sc[sb_a], 0, 0, lane);
+                    b128_promote<64, true>(sum + 32, t_addr + col_b, s_row * sc[sb_b], tempty_bar(acc), arrivals, lane);
                     if (++slot == kMoeScaleSlots) slot = 0;
                     if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
                 }
                 if (!alive) break;
-                const bool whole = k1 - k0 == l.kb;
                 // Where the sums go next: rows of activations that are finished here to shared memory if they fit; else, and parts of a
                 // tile, to work memory; whole rows of outputs straight to their place.
-                const bool turn = whole && rows <= kMoeTurnRows;
-                if (row_ok) {
-                    if (kind && whole) {
-                        if (half * 128 < p.hidden - nt * 256) {
+                if (et < g->rows) {
+                    const MoeList& l = sm.words->list[g->kind];
+                    const bool whole = g->k1 - g->k0 == l.kb;
+                    if (g->kind && whole) {
+                        if (half * 128 < p.hidden - g->out * 256) {
+                            const uint32_t route = sm.route[g->first + et];
                             const float w = p.route_w[route];
-                            float* o = p.rows_out + static_cast<int64_t>(route) * p.hidden + nt * 256 + half * 128;
+                            float* o = p.rows_out + static_cast<int64_t>(route) * p.hidden + g->out * 256 + half * 128;
 #pragma unroll
                             for (int j = 0; j < 128; j += 4) {
                                 const float4 f = unpack_f32x4(sum[j / 2], sum[j / 2 + 1]);
@@ -741,16 +752,24 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                             }
                         }
                     } else {
-                        float* o = turn ? sm.turn + et * kMoeTurnPitch : moe_part(p, l, kind, c, tile, whole) + et * 256;
+                        const bool turn = whole && g->rows <= kMoeTurnRows;
+                        float* o = turn ? sm.turn + et * kMoeTurnPitch : moe_part(p, l, g->kind, g->chunk, g->tile, whole) + et * 256;
 #pragma unroll
                         for (int j = 0; j < 128; j += 4)
                             *reinterpret_cast<float4*>(o + (j < 64 ? col_a + j : col_b + j - 64)) = unpack_f32x4(sum[j / 2], sum[j / 2 + 1]);
                     }
                 }
-                const int ph = moe_finish_tile(p, smem, kind, tile, rb, nt, c, k1 - k0, sync_phase);
-                if (ph < 0) { alive = false; break; }
-                sync_phase = ph;
+            } else {
+                slot = (slot + units) % kMoeScaleSlots;
+                acc += units;
+                acc_phase ^= static_cast<uint32_t>(acc >> 1) & 1u;
+                acc &= 1;
             }
+            sync_phase = moe_finish_tile(p, smem, at.slot, sync_phase, q * 32 >= g->rows);
+            if (sync_phase < 0) break;
+            __syncwarp();
+            if (lane == 0) segment_done(at);
+            step(at);
         }
     }
 
