@@ -120,7 +120,7 @@ int byte_map(const void* ptr, uint64_t inner, uint64_t rows, uint64_t row_stride
 // Work memory of mm_moe_few_tokens, in bytes from its start
 struct MoeWork {
     int64_t counters, route_expert, route_w, xq, xsf, act_q, act_sf, rows_out, parts, total;
-    int num_counters, ctr_done1, ctr_done2, ctr_tile1, ctr_tile2, part_rows, act_sf_pitch;
+    int num_counters, ctr_done1, ctr_tile1, ctr_tile2, part_rows, act_sf_pitch;
 };
 
 MoeWork moe_work(int T, int E, int K, int H, int I, bool cast, int ctas) {
@@ -131,8 +131,7 @@ MoeWork moe_work(int T, int E, int K, int H, int I, bool cast, int ctas) {
     const int64_t blocks = (routes < E ? routes : E) + routes / 128;
     const int64_t nt1 = I / 128, nt2 = (H + 255) / 256;
     w.ctr_done1 = 32;
-    w.ctr_done2 = w.ctr_done1 + (int)blocks;
-    w.ctr_tile1 = w.ctr_done2 + (int)nt2;
+    w.ctr_tile1 = w.ctr_done1 + (int)blocks;
     w.ctr_tile2 = w.ctr_tile1 + (int)(blocks * nt1);
     w.num_counters = w.ctr_tile2 + (int)(blocks * nt2);
     w.part_rows = (int)(routes < 128 ? routes : 128);
@@ -145,7 +144,7 @@ MoeWork moe_work(int T, int E, int K, int H, int I, bool cast, int ctas) {
     w.act_sf_pitch = (I / 128 + 31) / 32 * 32;
     w.act_sf = take(routes * w.act_sf_pitch * 4);
     w.rows_out = take(routes * H * 4);
-    w.parts = take((int64_t)5 * ctas * w.part_rows * 256 * 4);
+    w.parts = take((int64_t)6 * ctas * w.part_rows * 256 * 4);
     w.total = at;
     return w;
 }
@@ -348,7 +347,7 @@ int mm_moe_few_tokens(const void* x, int x_is_fp8, int64_t x_stride, const float
     p.route_w = reinterpret_cast<float*>(base + w.route_w);
     p.counters = reinterpret_cast<int*>(base + w.counters);
     p.num_counters = w.num_counters;
-    p.ctr_done1 = w.ctr_done1; p.ctr_done2 = w.ctr_done2; p.ctr_tile1 = w.ctr_tile1; p.ctr_tile2 = w.ctr_tile2;
+    p.ctr_done1 = w.ctr_done1; p.ctr_tile1 = w.ctr_tile1; p.ctr_tile2 = w.ctr_tile2;
     p.s1 = s1; p.s2 = s2; p.tiled = tiled ? 1 : 0;
     p.act_q = base + w.act_q; p.act_sf = reinterpret_cast<float*>(base + w.act_sf); p.act_sf_pitch = w.act_sf_pitch;
     p.rows_out = reinterpret_cast<float*>(base + w.rows_out);
@@ -372,7 +371,7 @@ int mm_moe_few_tokens(const void* x, int x_is_fp8, int64_t x_stride, const float
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3((unsigned)d->sms);
-    cfg.blockDim = dim3(mm::kB128Threads);
+    cfg.blockDim = dim3(mm::kMoeThreads);
     cfg.dynamicSmemBytes = mm::kMoeSmemBytes;
     cfg.stream = st;
     cudaLaunchAttribute attr;

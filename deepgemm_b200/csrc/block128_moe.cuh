@@ -19,8 +19,9 @@
 // for is always being worked on, however many of the CTAs are resident, and two such launches may share a GPU.
 //
 // Tile = up to 128 routes of one expert x 256 weight rows (first product: 128 gate rows and their 128 up rows, so that a tile holds
-// one whole block of the activations' cast).  Warp 0 = TMA (weights), 1 = MMA, 2-3 = token operand (cp.async: rows are gathered by
-// route), 4-11 = epilogue, with the promotion by block scales of block128_gemm.cuh.
+// one whole block of the activations' cast).  Warp 0 = TMA (weights), 1 = MMA, 2-3 = token operand and scales (cp.async: rows are gathered
+// by route), 8-15 = sums: the promotion by block scales of block128_gemm.cuh, 4-7 = what becomes of the sums of a tile (joining parts,
+// SwiGLU and cast, the counts that other CTAs wait for, the combine) while the next tile is being summed.
 #pragma once
 #include "block128.cuh"
 #include "block128_gemm.cuh"
@@ -36,14 +37,15 @@ constexpr int kMoeMaxStages = 5, kMoeFewRows = 48;
 constexpr int kMoeRingBytes = 4 * (128 * 128 + kMoeBBytes);
 static_assert(kMoeMaxStages * (kMoeFewRows * 128 + kMoeBBytes) <= kMoeRingBytes, "the ring of few rows");
 constexpr int kMoePlanBytes = kMoeMaxRoutes * 2 + kMoeMaxBlocks * 8 + kMoeMaxRoutes / 8;
-constexpr int kMoeTurnRows = 8, kMoeTurnPitch = 260;    // fp32 rows that change hands between the epilogue warps
+constexpr int kMoeTurnRows = 6, kMoeTurnPitch = 260;    // fp32 rows that go from the summing to the finishing warps, in two buffers
+constexpr int kMoeThreads = 512;
 constexpr int kMoeSegments = 8;
-constexpr int kMoeCtrTiles1 = 16;
+constexpr int kMoeCtrTiles1 = 8, kMoeCtrTiles2 = 16;
 constexpr int kMoeTailBytes = 768;        // barriers and MoeWords
 // Scales of a unit: 128 rows, then two of the weights.  As in block128_gemm.cuh: stages + accumulators + 1 units may be on their way.
 constexpr int kMoeScaleSlots = 8, kMoeScaleBytes = 544;
 static_assert(kMoeScaleSlots >= kMoeMaxStages + 2 + 1, "scale ring");
-constexpr int kMoeSmemBytes = kMoeRingBytes + kMoePlanBytes + kMoeTurnRows * kMoeTurnPitch * 4 + kMoeScaleSlots * kMoeScaleBytes + kMoeTailBytes;
+constexpr int kMoeSmemBytes = kMoeRingBytes + kMoePlanBytes + 2 * kMoeTurnRows * kMoeTurnPitch * 4 + kMoeScaleSlots * kMoeScaleBytes + kMoeTailBytes;
 static_assert(kMoeSmemBytes <= 232448, "exceeds the 227 KiB of shared memory a CTA can have");
 constexpr int kMoeStreamTiles = 16;        // tiles per SM below which chunks are equal shares
 
@@ -58,16 +60,16 @@ struct MoeParams {
     uint8_t* xq_out; float* xsf_out;
     int* route_expert; float* route_w;       // [tokens * topk], -1 = none
     int* counters; int num_counters;
-    // counters: [0] claims, [kMoeCtrTiles1] finished tiles of the first product, [32 ..) of them by block of routes, then
-    // of the second by output tile, then k blocks that have arrived for each tile that was cut, of either product
-    int ctr_done1, ctr_done2, ctr_tile1, ctr_tile2;
+    // counters: [0] claims, [kMoeCtrTiles1] and [kMoeCtrTiles2] finished tiles of either product, [ctr_done1 ..) of the first one by
+    // block of routes, [ctr_tile1 ..) and [ctr_tile2 ..) k blocks that have arrived for each tile that was cut
+    int ctr_done1, ctr_tile1, ctr_tile2;
     const float* s1; const float* s2;
     int tiled;
     // [routes][inter] and [routes][inter / 128], by place in the sorted list.  A row of scales has 128-byte lines of its own: they are
     // read through L1, which must not hold a line that another expert's tiles are still writing to
     uint8_t* act_q; float* act_sf; int act_sf_pitch;
     float* rows_out;                         // [routes][hidden]: weighted rows of the second product, by route
-    float* parts; int part_rows;             // [2 products][chunks][2][part_rows][256], then [CTAs][part_rows][256] for tiles that are whole
+    float* parts; int part_rows;             // [2 products][chunks][2][part_rows][256], then [CTAs][2][part_rows][256] for tiles that are whole
     __nv_bfloat16* y;
     float clamp;
     int* status;
@@ -188,18 +190,18 @@ struct MoeWords {
     MoeSegment segment[kMoeSegments];
 };
 struct MoeSmem {
-    float* turn;                                         // [kMoeTurnRows][kMoeTurnPitch]
+    float* turn;                                         // [2][kMoeTurnRows][kMoeTurnPitch]
     uint2* block;                                        // blocks of routes: expert | rows << 16, first place
     uint32_t* valid;                                     // a bit for each route
     uint16_t* route;                                     // routes sorted by expert
     float* scale;                                        // [slots][128 rows, 2 of the weights, 6 unused]
     uint32_t bars;
     MoeWords* words;
-    static constexpr int kBars = 2 * kMoeMaxStages + 5 + 2 * kMoeSegments;
+    static constexpr int kBars = 2 * kMoeMaxStages + 9 + 2 * kMoeSegments;
     static_assert(8 * kBars + sizeof(MoeWords) <= kMoeTailBytes, "barriers");
     __device__ __forceinline__ explicit MoeSmem(uint8_t* smem) {
         turn = reinterpret_cast<float*>(smem + kMoeRingBytes);
-        block = reinterpret_cast<uint2*>(turn + kMoeTurnRows * kMoeTurnPitch);
+        block = reinterpret_cast<uint2*>(turn + 2 * kMoeTurnRows * kMoeTurnPitch);
         valid = reinterpret_cast<uint32_t*>(block + kMoeMaxBlocks);
         route = reinterpret_cast<uint16_t*>(valid + kMoeMaxRoutes / 32);
         scale = reinterpret_cast<float*>(route + kMoeMaxRoutes);
@@ -207,7 +209,9 @@ struct MoeSmem {
         bars = smem_u32(tail);
         words = reinterpret_cast<MoeWords*>(tail + 8 * kBars);
     }
-    __device__ __forceinline__ uint32_t esync_bar() const { return bars + 8u * (kBars - 1); }
+    __device__ __forceinline__ uint32_t turn_full(int b) const { return bars + 8u * (kBars - 5 + b); }
+    __device__ __forceinline__ uint32_t turn_empty(int b) const { return bars + 8u * (kBars - 3 + b); }
+    __device__ __forceinline__ uint32_t finish_bar() const { return bars + 8u * (kBars - 1); }
 };
 
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int32_t c0, int32_t c1) {
@@ -247,6 +251,28 @@ __device__ __forceinline__ bool moe_wait_count(const int* p, int want, volatile 
     }
     return true;
 }
+// Whether a phase is complete, without the pause that try_wait may make
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// Bounded wait for something that takes a tile's time
+__device__ __forceinline__ bool mbar_wait_asleep(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t timeout_ns) {
+    uint64_t t0 = 0;
+    while (!mbar_try_wait(bar, parity)) {
+        if (*abort_flag != 0) return false;
+        const uint64_t t = global_timer_ns();
+        if (t0 == 0) t0 = t;
+        else if (t - t0 > timeout_ns) { *abort_flag = 1; return false; }
+        __nanosleep(40);
+    }
+    return true;
+}
 __device__ __forceinline__ void st_release_cta(uint32_t addr, int v) { asm volatile("st.release.cta.shared::cta.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ int ld_acquire_cta(uint32_t addr) {
     int v;
@@ -275,126 +301,163 @@ __device__ __forceinline__ int atomic_add_acq_rel(int* p, int v) {
 }
 
 // Work memory for the sums of a tile, [part_rows][256]: of a part, by the chunk that brought it (a chunk holds two at most, one that its
-// beginning cuts off and one its end), or of a whole tile, one for each CTA.
-__device__ __forceinline__ float* moe_part(const MoeParams& p, const MoeList& l, int kind, int ch, int tile, bool whole) {
-    const int64_t at = whole ? static_cast<int64_t>(gridDim.x) * 4 + blockIdx.x
+// beginning cuts off and one its end), or of a whole tile, two for each CTA in turn.
+__device__ __forceinline__ float* moe_part(const MoeParams& p, const MoeList& l, int kind, int ch, int tile, bool whole, int buffer) {
+    const int64_t at = whole ? static_cast<int64_t>(gridDim.x) * 4 + blockIdx.x * 2 + buffer
                              : (static_cast<int64_t>(kind) * gridDim.x + ch) * 2 + (l.start(ch) > tile * l.kb ? 0 : 1);
     return p.parts + at * p.part_rows * 256;
 }
 
-// What the eight epilogue warps do with a tile, or a part of one, once its sums have been written down.  Returns the phase of their barrier,
-// or -1 if a wait has run out.  A function of its own, so that none of its values is kept in registers beside the 128 sums.
-__device__ __noinline__ int moe_finish_tile(const MoeParams& p, uint8_t* smem, int slot, int phase, bool idle) {
-    const MoeSmem sm(smem);
-    const MoeSegment& g = sm.words->segment[slot];
+// What the four finishing warps do with a tile, or a part of one, once its sums have been written down.  False if a wait has run out.
+__device__ __forceinline__ bool moe_finish_tile(const MoeParams& p, const MoeSmem& sm, const MoeSegment& g, int buffer, uint32_t& phase) {
     const int kind = g.kind, tile = g.tile, rb = g.block, nt = g.out, units = g.k1 - g.k0;
     const MoeList& l = sm.words->list[kind];
-    const int ew = (threadIdx.x >> 5) - 4, lane = threadIdx.x & 31;
+    const int fw = (threadIdx.x >> 5) - 4, lane = threadIdx.x & 31;
     const bool boss = threadIdx.x == 128;
     const bool whole = units == l.kb;
     const int rows = g.rows;
     const bool turn = whole && rows <= kMoeTurnRows;
-    // Barrier of the eight warps, bounded like every other wait: a warp that has given up does not hold the others.  What the warps
-    // wrote before it is released to the GPU by the boss's count behind it, and what that count acquired they may read behind the
-    // next one (from L2: another SM has written it).
+    const float* my_turn = sm.turn + buffer * kMoeTurnRows * kMoeTurnPitch;
+    // Barrier of the four warps, bounded like every other wait: a warp that has given up does not hold the others.  What the warps
+    // wrote before it (and the summing warps before the buffer was full) is released to the GPU by the boss's count behind it, and
+    // what that count acquired they may read behind the next one (from L2: another SM has written it).
     auto sync = [&]() {
         __syncwarp();
-        if (lane == 0) mbar_arrive(sm.esync_bar());
-        const bool ok = mbar_wait_often(sm.esync_bar(), static_cast<uint32_t>(phase), &sm.words->abort, p.timeout_ns);
-        phase ^= 1;
+        if (lane == 0) mbar_arrive(sm.finish_bar());
+        const bool ok = mbar_wait_often(sm.finish_bar(), phase, &sm.words->abort, p.timeout_ns);
+        phase ^= 1u;
         return ok;
     };
-    if (idle) {                                          // a whole tile's time to wait
+    auto release = [&]() {                               // the buffer's values have been read
         __syncwarp();
-        if (lane == 0) mbar_arrive(sm.esync_bar());
-        const uint64_t t0 = global_timer_ns();
-        while (!mbar_try_wait(sm.esync_bar(), static_cast<uint32_t>(phase))) {
-            __nanosleep(64);
-            if (sm.words->abort != 0) return -1;
-            if (global_timer_ns() - t0 > p.timeout_ns) { sm.words->abort = 1; return -1; }
-        }
-        phase ^= 1;
-    } else if (!sync()) {
-        return -1;
-    }
+        if (lane == 0) mbar_arrive(sm.turn_empty(buffer));
+    };
     int c0 = g.chunk, c1 = g.chunk;
     if (!whole) {
         // the parts are added up by whoever brings the last one, in the order of the chunks
+        release();                                       // parts have memory of their own
         if (boss) sm.words->last = atomic_add_acq_rel(p.counters + (kind ? p.ctr_tile2 : p.ctr_tile1) + tile, units) + units == l.kb;
-        if (!sync()) return -1;
-        if (sm.words->last == 0) return phase;
+        if (!sync()) return false;
+        if (sm.words->last == 0) return true;
         c0 = l.chunk_of(tile * l.kb);
         c1 = l.chunk_of(tile * l.kb + l.kb - 1);
     }
-    // four columns from `col` on of a row: up to four parts' loads in flight, added in order
-    auto join = [&](int row, int col) {
-        if (turn) return *reinterpret_cast<const float4*>(sm.turn + row * kMoeTurnPitch + col);
-        float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int ch = c0; ch <= c1; ch += 4) {
-            float4 f[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (ch + i <= c1) f[i] = __ldcg(reinterpret_cast<const float4*>(moe_part(p, l, kind, ch + i, tile, whole) + row * 256 + col));
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (ch + i <= c1) add4(t, f[i]);
+    // Four columns each from two places (gate and up, or two runs of outputs) of two rows, the second one four behind: eight loads in
+    // flight, two parts at a time, added in order.  v[row][place].
+    auto join = [&](int row, int col_a, int col_b, float4 (&v)[2][2]) {
+        const bool two = row + 4 < rows;
+        if (turn) {
+            const float* in = my_turn + row * kMoeTurnPitch;
+            v[0][0] = *reinterpret_cast<const float4*>(in + col_a);
+            v[0][1] = *reinterpret_cast<const float4*>(in + col_b);
+            if (two) {
+                v[1][0] = *reinterpret_cast<const float4*>(in + 4 * kMoeTurnPitch + col_a);
+                v[1][1] = *reinterpret_cast<const float4*>(in + 4 * kMoeTurnPitch + col_b);
+            }
+            return;
         }
-        return t;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i >> 1][i & 1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int ch = c0; ch <= c1; ch += 2) {
+            float4 f[2][2][2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (ch + i > c1) continue;
+                const float* in = moe_part(p, l, kind, ch + i, tile, whole, buffer) + row * 256;
+                f[i][0][0] = __ldcg(reinterpret_cast<const float4*>(in + col_a));
+                f[i][0][1] = __ldcg(reinterpret_cast<const float4*>(in + col_b));
+                if (two) {
+                    f[i][1][0] = __ldcg(reinterpret_cast<const float4*>(in + 4 * 256 + col_a));
+                    f[i][1][1] = __ldcg(reinterpret_cast<const float4*>(in + 4 * 256 + col_b));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (ch + i > c1) continue;
+                add4(v[0][0], f[i][0][0]);
+                add4(v[0][1], f[i][0][1]);
+                if (two) { add4(v[1][0], f[i][1][0]); add4(v[1][1], f[i][1][1]); }
+            }
+        }
     };
     if (kind == 0) {
         // a row at a time for each warp: with one thread to a row, as the sums were held, a tile of few rows would keep eight warps
         // waiting for the few threads that have any
         const bool do_clamp = p.clamp < 3.0e38f;
-        for (int r = ew; r < rows; r += 8) moe_finish_row(p, join(r, lane * 4), join(r, 128 + lane * 4), do_clamp, static_cast<int64_t>(g.first) + r, nt, lane);
-        if (!sync()) return -1;
-        if (boss) {
-            red_release_gpu_add(p.counters + p.ctr_done1 + rb, 1);
-            red_release_gpu_add(p.counters + kMoeCtrTiles1, 1);
+        for (int r = fw; r < rows; r += 8) {
+            float4 v[2][2];
+            join(r, lane * 4, 128 + lane * 4, v);
+            moe_finish_row(p, v[0][0], v[0][1], do_clamp, static_cast<int64_t>(g.first) + r, nt, lane);
+            if (r + 4 < rows) moe_finish_row(p, v[1][0], v[1][1], do_clamp, static_cast<int64_t>(g.first) + r + 4, nt, lane);
         }
-        return phase;
+        if (whole) release();
+        if (!sync()) return false;
+        if (boss) {
+            __threadfence();
+            atomicAdd(p.counters + p.ctr_done1 + rb, 1);
+            atomicAdd(p.counters + kMoeCtrTiles1, 1);
+        }
+        return true;
     }
     const int cols = min(256, p.hidden - nt * 256);
-    if (!whole) {
-        for (int r = ew; r < rows; r += 8) {
-            const uint32_t rr = sm.route[g.first + r];
-            const float w = p.route_w[rr];
-            for (int col = lane * 4; col < cols; col += 128) {
-                const float4 t = join(r, col);
-                *reinterpret_cast<float4*>(p.rows_out + static_cast<int64_t>(rr) * p.hidden + nt * 256 + col) = make_float4(t.x * w, t.y * w, t.z * w, t.w * w);
-            }
-        }
-        if (!sync()) return -1;
-    }
-    if (boss) sm.words->last = atomic_add_acq_rel(p.counters + p.ctr_done2 + nt, 1) == sm.words->blocks - 1;
-    if (!sync()) return -1;
-    if (sm.words->last != 0) {
-        // every expert's rows of these outputs are there: add each token's up, in the order of its slots
-        const int cols4 = cols / 4;
-#pragma unroll 1
-        for (int i = threadIdx.x - 128; i < p.tokens * cols4; i += kB128EpiThreads) {
-            const int t = i / cols4, col = nt * 256 + (i - t * cols4) * 4;
-            const int r0 = t * p.topk;
-            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-            for (int s = 0; s < p.topk; s += 4) {
-                float4 f[4];
-                bool ok[4];
+    if (whole) {
+        release();                                       // the rows are in their place already
+    } else {
+        for (int r = fw; r < rows; r += 8) {
+            float4 v[2][2];
+            join(r, lane * 4, 128 + lane * 4, v);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int r = r0 + s + j;
-                    ok[j] = s + j < p.topk && ((sm.valid[r >> 5] >> (r & 31)) & 1u);
-                    if (ok[j]) f[j] = __ldcg(reinterpret_cast<const float4*>(p.rows_out + static_cast<int64_t>(r) * p.hidden + col));
+            for (int i = 0; i < 2; ++i) {
+                if (r + 4 * i >= rows) continue;
+                const uint32_t rr = sm.route[g.first + r + 4 * i];
+                const float w = p.route_w[rr];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int col = lane * 4 + 128 * j;
+                    const float4 t = v[i][j];
+                    if (col < cols) *reinterpret_cast<float4*>(p.rows_out + static_cast<int64_t>(rr) * p.hidden + nt * 256 + col) = make_float4(t.x * w, t.y * w, t.z * w, t.w * w);
                 }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) if (ok[j]) add4(a, f[j]);
             }
-            *reinterpret_cast<uint2*>(p.y + static_cast<int64_t>(t) * p.hidden + col) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
         }
     }
-    return phase;
+    if (!sync()) return false;
+    if (boss) {
+        __threadfence();
+        atomicAdd(p.counters + kMoeCtrTiles2, 1);
+    }
+    return true;
 }
 
-__global__ void __launch_bounds__(kB128Threads, 1)
+// The combine, by the finishing warps of every CTA once all tiles of the second product are finished: each token's rows, in the order of its
+// slots, four columns a thread.  `tiles`: how many there are.
+__device__ __forceinline__ void moe_combine(const MoeParams& p, const MoeSmem& sm, int tiles, uint32_t phase) {
+    const int lane = threadIdx.x & 31;
+    if (threadIdx.x == 128 && !moe_wait_count(p.counters + kMoeCtrTiles2, tiles, &sm.words->abort, p.timeout_ns)) return;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(sm.finish_bar());
+    if (!mbar_wait_often(sm.finish_bar(), phase, &sm.words->abort, p.timeout_ns)) return;
+    const int cols4 = p.hidden / 4;
+    for (int i = blockIdx.x * 128 + threadIdx.x - 128; i < p.tokens * cols4; i += gridDim.x * 128) {
+        const int t = i / cols4, col = (i - t * cols4) * 4;
+        const int r0 = t * p.topk;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < p.topk; s += 8) {
+            float4 f[8];
+            bool ok[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int r = r0 + s + j;
+                ok[j] = s + j < p.topk && ((sm.valid[r >> 5] >> (r & 31)) & 1u);
+                if (ok[j]) f[j] = __ldcg(reinterpret_cast<const float4*>(p.rows_out + static_cast<int64_t>(r) * p.hidden + col));
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) if (ok[j]) add4(a, f[j]);
+        }
+        *reinterpret_cast<uint2*>(p.y + static_cast<int64_t>(t) * p.hidden + col) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
+    }
+}
+
+__global__ void __launch_bounds__(kMoeThreads, 1)
 moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_constant__ CUtensorMap tm_w2, const __grid_constant__ MoeParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t smem_base = smem_u32(smem);
@@ -411,8 +474,9 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
     if (threadIdx.x == 0) {
         for (int s = 0; s < kMoeMaxStages; ++s) { mbar_init(full_bar(s), 3); mbar_init(empty_bar(s), 1); }
         for (int a = 0; a < 2; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), 8); }
-        for (int c = 0; c < kMoeSegments; ++c) { mbar_init(sfull_bar(c), 1); mbar_init(sempty_bar(c), 11); }
-        mbar_init(sm.esync_bar(), 8);
+        for (int c = 0; c < kMoeSegments; ++c) { mbar_init(sfull_bar(c), 1); mbar_init(sempty_bar(c), 15); }
+        for (int b = 0; b < 2; ++b) { mbar_init(sm.turn_full(b), 8); mbar_init(sm.turn_empty(b), 4); }
+        mbar_init(sm.finish_bar(), 4);
         *abort_flag = 0;
         st_release_cta(smem_u32(&sm.words->ready), 0);
         fence_barrier_init();
@@ -625,7 +689,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                 while (pending > 0) hand_over();
             };
             while (alive) {
-                if (!__all_sync(0xffffffffu, mbar_try_wait(sfull_bar(at.slot), at.phase))) drain();      // nothing to go on with yet
+                if (!__all_sync(0xffffffffu, mbar_test(sfull_bar(at.slot), at.phase))) drain();          // nothing to go on with yet
                 const MoeSegment* seg = segment_at(at);
                 if (seg == nullptr || seg->kind < 0) break;
                 const MoeSegment g = *seg;
@@ -693,21 +757,41 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
             drain();
         }
         __syncwarp();
-    } else {
-        // ---------------------------------------------------------------------- epilogue
-        regs_inc<224>();
-        const int q = warp & 3, half = (warp - 4) >> 2;
-        const int et = q * 32 + lane;
-        int acc = 0; uint32_t acc_phase = 0;
-        int sync_phase = 0;
-        int slot = 0;                                                // place of the next unit in the ring of scales
-        Place at;
-        bool alive = true;
+    } else if (warp < 8) {
+        // ---------------------------------------------------------------------- finishing
+        regs_dec<104>();
         if (n_blocks == 0) {                                         // no route at all: the sum is empty
-            for (int64_t i = static_cast<int64_t>(blockIdx.x) * kB128EpiThreads + threadIdx.x - 128; i < static_cast<int64_t>(p.tokens) * p.hidden / 8;
-                 i += static_cast<int64_t>(gridDim.x) * kB128EpiThreads)
+            for (int64_t i = static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x - 128; i < static_cast<int64_t>(p.tokens) * p.hidden / 8;
+                 i += static_cast<int64_t>(gridDim.x) * 128)
                 reinterpret_cast<uint4*>(p.y)[i] = make_uint4(0, 0, 0, 0);
         }
+        int buffer = 0; uint32_t buffer_phase = 0, sync_phase = 0;
+        Place at;
+        while (true) {
+            const MoeSegment* g = segment_at(at);
+            if (g == nullptr) break;
+            if (g->kind < 0) {
+                if (n_blocks > 0) moe_combine(p, sm, n_blocks * nt2, sync_phase);
+                break;
+            }
+            if (!mbar_wait_asleep(sm.turn_full(buffer), buffer_phase, abort_flag, p.timeout_ns)) break;
+            if (!moe_finish_tile(p, sm, *g, buffer, sync_phase)) break;
+            __syncwarp();
+            if (lane == 0) segment_done(at);
+            step(at);
+            buffer ^= 1;
+            if (buffer == 0) buffer_phase ^= 1u;
+        }
+    } else {
+        // ---------------------------------------------------------------------- sums
+        regs_inc<176>();
+        const int q = warp & 3, half = (warp - 8) >> 2;
+        const int et = q * 32 + lane;
+        int acc = 0; uint32_t acc_phase = 0;
+        int slot = 0;                                                // place of the next unit in the ring of scales
+        int buffer = 0; uint32_t buffer_phase = 0;
+        Place at;
+        bool alive = true;
         while (alive) {
             const MoeSegment* g = segment_at(at);
             if (g == nullptr || g->kind < 0) break;
@@ -729,12 +813,12 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                     const float* sc = sm.scale + slot * (kMoeScaleBytes / 4);
                     const float s_row = sc[et];
                     const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * 256;
-                    b128_promote<64, false>(sum, t_addr + col_a, s_row * sc[sb_a], 0, 0, lane);
-                    b128_promote<64, true>(sum + 32, t_addr + col_b, s_row * sc[sb_b], tempty_bar(acc), arrivals, lane);
+                    b128_promote<64, false, 32>(sum, t_addr + col_a, s_row * sc[sb_a], 0, 0, lane);
+                    b128_promote<64, true, 32>(sum + 32, t_addr + col_b, s_row * sc[sb_b], tempty_bar(acc), arrivals, lane);
                     if (++slot == kMoeScaleSlots) slot = 0;
                     if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
                 }
-                if (!alive) break;
+                if (!alive || !mbar_wait_often(sm.turn_empty(buffer), buffer_phase ^ 1u, abort_flag, p.timeout_ns)) break;
                 // Where the sums go next: rows of activations that are finished here to shared memory if they fit; else, and parts of a
                 // tile, to work memory; whole rows of outputs straight to their place.
                 if (et < g->rows) {
@@ -753,20 +837,27 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                         }
                     } else {
                         const bool turn = whole && g->rows <= kMoeTurnRows;
-                        float* o = turn ? sm.turn + et * kMoeTurnPitch : moe_part(p, l, g->kind, g->chunk, g->tile, whole) + et * 256;
+                        float* o = turn ? sm.turn + (buffer * kMoeTurnRows + et) * kMoeTurnPitch : moe_part(p, l, g->kind, g->chunk, g->tile, whole, buffer) + et * 256;
 #pragma unroll
                         for (int j = 0; j < 128; j += 4)
                             *reinterpret_cast<float4*>(o + (j < 64 ? col_a + j : col_b + j - 64)) = unpack_f32x4(sum[j / 2], sum[j / 2 + 1]);
                     }
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(sm.turn_full(buffer));
             } else {
+                // Not ahead of the others, though: a barrier tells a phase from the one after the next by nothing.  So an idle warp is
+                // counted where the sums are handed on, and waits there, mostly asleep, until the others have come.
+                if (!mbar_wait_often(sm.turn_empty(buffer), buffer_phase ^ 1u, abort_flag, p.timeout_ns)) break;
+                if (lane == 0) mbar_arrive(sm.turn_full(buffer));
+                if (!mbar_wait_asleep(sm.turn_full(buffer), buffer_phase, abort_flag, p.timeout_ns)) break;
                 slot = (slot + units) % kMoeScaleSlots;
                 acc += units;
                 acc_phase ^= static_cast<uint32_t>(acc >> 1) & 1u;
                 acc &= 1;
             }
-            sync_phase = moe_finish_tile(p, smem, at.slot, sync_phase, q * 32 >= g->rows);
-            if (sync_phase < 0) break;
+            buffer ^= 1;
+            if (buffer == 0) buffer_phase ^= 1u;
             __syncwarp();
             if (lane == 0) segment_done(at);
             step(at);
