@@ -31,38 +31,45 @@ def _blocks(n: int) -> int:
     return (n + 127) // 128
 
 
-def _call(device: torch.device, fn, *args) -> None:
-    """Run a library call (its last argument, the stream, is added here) with `device` current."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+# The stream's handle without building a Stream object around it: 0.1 us instead of 3, and a call for one token takes about ten.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _call(index: int, fn, *args) -> None:
+    """Run a library call (its last argument, the stream, is added here) with device `index` current."""
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
     if rc != 0:
         _lib.check(rc)
 
 
-def _require_cuda(name: str, *tensors: Optional[torch.Tensor]) -> torch.device:
-    device = None
+def _device_index(name: str, *tensors: Optional[torch.Tensor]) -> int:
+    index = tensors[0].get_device()
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
+        if t is not None and t.get_device() != index:
+            index = -1
+    if index < 0:
+        if any(t is not None and not t.is_cuda for t in tensors):
             raise RuntimeError(f"{name} needs CUDA tensors (this package has no CPU path)")
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise RuntimeError(f"{name}: tensors are on different devices ({device} and {t.device})")
-    return device
+        raise RuntimeError(f"{name}: tensors are on different devices")
+    return index
 
 
 def _rows_of(t: torch.Tensor, align: int) -> torch.Tensor:
     """`t` [rows, k] as it is if its rows are dense and start on `align`-byte boundaries, else a contiguous copy."""
-    size = t.element_size()
-    if t.stride(1) == 1 and t.stride(0) >= t.size(1) and (t.stride(0) * size) % align == 0 and t.data_ptr() % align == 0:
+    pitch, step = t.stride()
+    if step == 1 and t.data_ptr() % align == 0 and (t.shape[0] <= 1 or (pitch >= t.shape[1] and (pitch * t.element_size()) % align == 0)):
         return t
     t = t.contiguous()
-    return t if t.data_ptr() % align == 0 else t.clone()
+    return t if t.data_ptr() % align == 0 and (t.shape[0] <= 1 or (t.stride(0) * t.element_size()) % align == 0) else t.clone()
+
+
+def _pitch(t: torch.Tensor) -> int:
+    """Elements from a row to the next; the stride of a single row says nothing."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def cast_to_fp8_block128(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -70,19 +77,23 @@ def cast_to_fp8_block128(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
     For each 128 values of a row: top = max(amax, 1e-4), scale = top / 448, code = e4m3(448 x / top), ties to even.  A block that
     holds an infinity or a NaN gets NaN codes and a scale that is not finite."""
-    if x.dim() < 1 or x.dtype not in _TYPES:
+    kind = _TYPES.get(x.dtype)
+    if kind is None or x.dim() < 1:
         raise TypeError("cast_to_fp8_block128 expects a bfloat16, float16 or float32 tensor with at least one dimension")
-    k = x.shape[-1]
+    shape = x.shape
+    k = shape[-1]
     if k == 0 or k % 8 != 0:
         raise ValueError("the row length must be a positive multiple of 8")
-    device = _require_cuda("cast_to_fp8_block128", x)
-    rows2d = x if x.dim() == 2 else x.reshape(-1, k)
-    rows2d = _rows_of(rows2d, 16)
-    rows = rows2d.shape[0]
-    q = torch.empty(x.shape, dtype=_E4M3, device=device)
-    sf = torch.empty((*x.shape[:-1], (k + 127) // 128), dtype=torch.float32, device=device)
+    index = _device_index("cast_to_fp8_block128", x)
+    q = x.new_empty(shape, dtype=_E4M3)
+    sf = x.new_empty((*shape[:-1], (k + 127) // 128), dtype=torch.float32)
+    rows = x.numel() // k
     if rows:
-        _call(device, _lib.lib().mm_cast_block128, rows2d.data_ptr(), _TYPES[x.dtype], rows, k, rows2d.stride(0), q.data_ptr(), sf.data_ptr())
+        stride = k
+        if not x.is_contiguous() or x.data_ptr() % 16 != 0:
+            x = _rows_of(x if x.dim() == 2 else x.reshape(-1, k), 16)
+            stride = _pitch(x)
+        _call(index, _lib.lib().mm_cast_block128, x.data_ptr(), kind, rows, k, stride, q.data_ptr(), sf.data_ptr())
     return q, sf
 
 
@@ -94,14 +105,14 @@ def cast_weight_to_fp8_block128(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Te
     n, k = w.shape[-2:]
     if k == 0 or k % 8 != 0:
         raise ValueError("the row length must be a positive multiple of 8")
-    device = _require_cuda("cast_weight_to_fp8_block128", w)
+    index = _device_index("cast_weight_to_fp8_block128", w)
     w = w.contiguous()
     if w.data_ptr() % 16 != 0:
         w = w.clone()
-    q = torch.empty(w.shape, dtype=_E4M3, device=device)
-    sf = torch.empty((*w.shape[:-2], _blocks(n), _blocks(k)), dtype=torch.float32, device=device)
+    q = w.new_empty(w.shape, dtype=_E4M3)
+    sf = w.new_empty((*w.shape[:-2], _blocks(n), _blocks(k)), dtype=torch.float32)
     if w.numel():
-        _call(device, _lib.lib().mm_cast_weight_block128, w.data_ptr(), _TYPES[w.dtype], w.shape[0] if w.dim() == 3 else 1, n, k, q.data_ptr(), sf.data_ptr())
+        _call(index, _lib.lib().mm_cast_weight_block128, w.data_ptr(), _TYPES[w.dtype], w.shape[0] if w.dim() == 3 else 1, n, k, q.data_ptr(), sf.data_ptr())
     return q, sf
 
 
@@ -112,14 +123,20 @@ def _check_operands(name, a, a_sf, b, b_sf, n, k):
         raise RuntimeError(f"{name} expects fp32 scales")
     if k == 0 or k % 16 != 0:
         raise RuntimeError(f"{name}: K must be a positive multiple of 16")
-    if a.dim() != 2 or a.shape[1] != k or tuple(a_sf.shape) != (a.shape[0], _blocks(k)):
+    kb = (k + 127) // 128
+    if a.dim() != 2 or a.shape[1] != k or a_sf.shape != (a.shape[0], kb):
         raise RuntimeError(f"{name} expects a [M, K] with scales [M, ceil(K/128)], got {tuple(a.shape)} and {tuple(a_sf.shape)}")
-    if tuple(b_sf.shape[-2:]) != (_blocks(n), _blocks(k)):
+    if b_sf.shape[-2:] != ((n + 127) // 128, kb):
         raise RuntimeError(f"{name} expects weight scales [.., ceil(N/128), ceil(K/128)], got {tuple(b_sf.shape)}")
 
 
 def _scale_rows(sf: torch.Tensor) -> torch.Tensor:
-    return sf if sf.stride(1) == 1 and sf.stride(0) >= sf.shape[1] else sf.contiguous()
+    return sf if sf.is_contiguous() or (sf.stride(1) == 1 and sf.stride(0) >= sf.shape[1]) else sf.contiguous()
+
+
+def _dense(t: torch.Tensor, align: int) -> torch.Tensor:
+    t = t.contiguous()
+    return t if t.data_ptr() % align == 0 else t.clone()
 
 
 def fp8_gemm_nt_block128(a: Tuple[torch.Tensor, torch.Tensor], b: Tuple[torch.Tensor, torch.Tensor], out: Optional[torch.Tensor] = None,
@@ -130,26 +147,26 @@ def fp8_gemm_nt_block128(a: Tuple[torch.Tensor, torch.Tensor], b: Tuple[torch.Te
     the output is bf16 or fp32 (`out`'s type, else `out_dtype`, else bf16)."""
     (a_q, a_sf), (b_q, b_sf) = a, b
     name = "fp8_gemm_nt_block128"
-    device = _require_cuda(name, a_q, a_sf, b_q, b_sf, out)
+    index = _device_index(name, a_q, a_sf, b_q, b_sf, out)
     if b_q.dim() != 2 or b_sf.dim() != 2:
         raise RuntimeError(f"{name} expects b [N, K] with 2D scales")
     n, k = b_q.shape
     _check_operands(name, a_q, a_sf, b_q, b_sf, n, k)
     m = a_q.shape[0]
     if out is None:
-        out = torch.empty((m, n), dtype=torch.bfloat16 if out_dtype is None else out_dtype, device=device)
-    elif tuple(out.shape) != (m, n) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n) or (out_dtype is not None and out.dtype != out_dtype):
-        raise RuntimeError(f"{name}: out must be [{m}, {n}] with dense rows (and of out_dtype, if that is given)")
+        out = a_q.new_empty((m, n), dtype=torch.bfloat16 if out_dtype is None else out_dtype)
+        pitch = n
+    else:
+        if tuple(out.shape) != (m, n) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n) or (out_dtype is not None and out.dtype != out_dtype):
+            raise RuntimeError(f"{name}: out must be [{m}, {n}] with dense rows (and of out_dtype, if that is given)")
+        pitch = _pitch(out)
     if out.dtype not in (torch.bfloat16, torch.float32):
         raise RuntimeError(f"{name}: the output is bfloat16 or float32")
     if m == 0 or n == 0:
         return out
-    a_q, b_q = _rows_of(a_q, 16), b_q.contiguous()
-    if b_q.data_ptr() % 16 != 0:
-        b_q = b_q.clone()
-    a_sf, b_sf = _scale_rows(a_sf), b_sf.contiguous()
-    _call(device, _lib.lib().mm_fp8_gemm_block128, a_q.data_ptr(), max(a_q.stride(0), k), a_sf.data_ptr(), max(a_sf.stride(0), _blocks(k)), b_q.data_ptr(),
-          b_sf.data_ptr(), 1, 0, None, out.data_ptr(), max(out.stride(0), n), out.dtype == torch.float32, m, n, k)
+    a_q, b_q, a_sf, b_sf = _rows_of(a_q, 16), _dense(b_q, 16), _scale_rows(a_sf), b_sf.contiguous()
+    _call(index, _lib.lib().mm_fp8_gemm_block128, a_q.data_ptr(), _pitch(a_q), a_sf.data_ptr(), _pitch(a_sf), b_q.data_ptr(),
+          b_sf.data_ptr(), 1, 0, None, out.data_ptr(), pitch, out.dtype == torch.float32, m, n, k)
     return out
 
 
@@ -162,7 +179,7 @@ def m_grouped_fp8_gemm_nt_contiguous_block128(a: Tuple[torch.Tensor, torch.Tenso
     left as they were.  check=True synchronises and raises if a 128-row block mixed experts (such rows are not written)."""
     (a_q, a_sf), (w, w_sf) = a, b
     name = "m_grouped_fp8_gemm_nt_contiguous_block128"
-    device = _require_cuda(name, a_q, a_sf, w, w_sf, d, m_indices)
+    index = _device_index(name, a_q, a_sf, w, w_sf, d, m_indices)
     if w_sf.dim() != 3 or w.dim() not in (3, 5) or w.shape[0] != w_sf.shape[0]:
         raise RuntimeError(f"{name} expects weights [E, N, K] (or tiled) with scales [E, ceil(N/128), ceil(K/128)]")
     k = a_q.shape[-1]
@@ -183,14 +200,11 @@ def m_grouped_fp8_gemm_nt_contiguous_block128(a: Tuple[torch.Tensor, torch.Tenso
     if rows and n and w.shape[0] == 0:
         raise RuntimeError(f"{name}: no experts")
     if rows and n:
-        a_q, w = _rows_of(a_q, 16), w.contiguous()
-        if w.data_ptr() % 16 != 0:
-            w = w.clone()
-        a_sf, w_sf, m_indices = _scale_rows(a_sf), w_sf.contiguous(), m_indices.contiguous()
-        _call(device, _lib.lib().mm_fp8_gemm_block128, a_q.data_ptr(), max(a_q.stride(0), k), a_sf.data_ptr(), max(a_sf.stride(0), _blocks(k)), w.data_ptr(),
+        a_q, w, a_sf, w_sf, m_indices = _rows_of(a_q, 16), _dense(w, 16), _scale_rows(a_sf), w_sf.contiguous(), m_indices.contiguous()
+        _call(index, _lib.lib().mm_fp8_gemm_block128, a_q.data_ptr(), _pitch(a_q), a_sf.data_ptr(), _pitch(a_sf), w.data_ptr(),
               w_sf.data_ptr(), w.shape[0], tiled, m_indices.data_ptr(), d.data_ptr(), n, d.dtype == torch.float32, rows, n, k)
     if check:
-        check_block128_status(device)
+        check_block128_status(index)
     return d
 
 
@@ -237,7 +251,7 @@ def fp8_moe_few_tokens(x, l1_weights: Tuple[torch.Tensor, torch.Tensor], l2_weig
     if isinstance(x, (tuple, list)):
         x, x_sf = x
     (w1, s1), (w2, s2) = l1_weights, l2_weights
-    device = _require_cuda(name, x, x_sf, w1, s1, w2, s2, router_logits, topk_idx, topk_weights, out)
+    index = _device_index(name, x, x_sf, w1, s1, w2, s2, router_logits, topk_idx, topk_weights, out)
     if x.dim() != 2 or x.dtype != (torch.bfloat16 if x_sf is None else _E4M3):
         raise RuntimeError(f"{name} expects x as bfloat16 [T, H] or as e4m3 codes with their scales")
     if w1.dtype != _E4M3 or w2.dtype != _E4M3 or s1.dtype != torch.float32 or s2.dtype != torch.float32:
@@ -286,30 +300,30 @@ def fp8_moe_few_tokens(x, l1_weights: Tuple[torch.Tensor, torch.Tensor], l2_weig
     if not clamp > 0:
         raise ValueError(f"{name}: activation_clamp must be positive")
     if out is None:
-        out = torch.empty((t, h), dtype=torch.bfloat16, device=device)
+        out = x.new_empty((t, h), dtype=torch.bfloat16)
     elif out.dtype != torch.bfloat16 or tuple(out.shape) != (t, h) or not out.is_contiguous() or out.data_ptr() % 16 != 0:
         raise RuntimeError(f"{name}: out must be a contiguous bfloat16 [{t}, {h}], 16-byte aligned")
     if t == 0:
         return out
     if x_sf is None:
         x = _rows_of(x, 32)              # 16 values
-        stride = max(x.stride(0), h)
+        stride = _pitch(x)
     else:
         x, x_sf, stride = x.contiguous(), x_sf.contiguous(), h
         if x.data_ptr() % 16 != 0:
             x = x.clone()
     s1, s2 = s1.contiguous(), s2.contiguous()
-    nbytes = _moe_work_bytes(device.index, t, e, k, h, i)
-    work = torch.empty((nbytes,), dtype=torch.uint8, device=device)
+    nbytes = _moe_work_bytes(index, t, e, k, h, i)
+    work = x.new_empty((nbytes,), dtype=torch.uint8)
     logits = router_logits
-    _call(device, _lib.lib().mm_moe_few_tokens, x.data_ptr(), x_sf is not None, stride, None if x_sf is None else x_sf.data_ptr(),
-          None if logits is None else logits.data_ptr(), 0 if logits is None else max(logits.stride(0), e), None if topk_idx is None else topk_idx.data_ptr(),
+    _call(index, _lib.lib().mm_moe_few_tokens, x.data_ptr(), x_sf is not None, stride, None if x_sf is None else x_sf.data_ptr(),
+          None if logits is None else logits.data_ptr(), 0 if logits is None else _pitch(logits), None if topk_idx is None else topk_idx.data_ptr(),
           topk_idx is not None and topk_idx.dtype == torch.int64, None if topk_weights is None else topk_weights.data_ptr(), w1.data_ptr(), s1.data_ptr(),
           w2.data_ptr(), s2.data_ptr(), tiled, t, e, k, h, i, clamp, work.data_ptr(), nbytes, out.data_ptr())
     return out
 
 
-def check_block128_status(device: Optional[torch.device] = None) -> None:
+def check_block128_status(device=None) -> None:
     """Synchronise the current stream and raise if a kernel of this module has reported a failure on `device` since the last call."""
     out = (ctypes.c_int32 * 5)()
     with torch.cuda.device(device):
@@ -346,69 +360,93 @@ def norm_gate_residual(y: Optional[torch.Tensor], residual: torch.Tensor, *, pos
     residual is fp16, never narrower than the range of the stream).  Arithmetic is fp32 throughout and each output is rounded once.  H is a
     multiple of 8, at most 16384."""
     name = "norm_gate_residual"
-    device = _require_cuda(name, y, residual, post_weight, gate, pre_weight, out_codes, out_scales)
-    for t in (y, residual, post_weight, gate, pre_weight):
-        if t is not None and t.dtype not in _TYPES:
-            raise TypeError(f"{name} expects bfloat16, float16 or float32 tensors")
+    index = _device_index(name, residual, y, post_weight, gate, pre_weight, out_codes, out_scales)
     if residual.dim() != 2:
         raise ValueError(f"{name} expects a residual [T, H]")
     t, h = residual.shape
     if h == 0 or h % 8 != 0 or h > 16384:
         raise ValueError(f"{name}: H must be a multiple of 8, at most 16384")
-    if y is None and (post_weight is not None or gate is not None or residual_scale != 1.0):
-        raise ValueError(f"{name}: post_weight, gate and residual_scale need y")
-    if y is not None and tuple(y.shape) != (t, h):
+    if y is None:
+        if post_weight is not None or gate is not None or residual_scale != 1.0:
+            raise ValueError(f"{name}: post_weight, gate and residual_scale need y")
+    elif y.shape != (t, h):
         raise ValueError(f"{name}: y must be [{t}, {h}]")
-    for w in (post_weight, pre_weight):
-        if w is not None and tuple(w.shape) != (h,):
-            raise ValueError(f"{name}: norm weights must be [{h}]")
-    if quant not in (None, "block128", "channelwise"):
+    quant_kind = _QUANT.get(quant)
+    if quant_kind is None:
         raise ValueError(f"{name}: quant must be None, 'block128' or 'channelwise'")
-    if pre_weight is None and quant is not None:
+    if quant_kind == 0:
+        if out_codes is not None or out_scales is not None:
+            raise ValueError(f"{name}: out_codes and out_scales need quant")
+    elif pre_weight is None:
         raise ValueError(f"{name}: codes need pre_weight")
-    if quant is None and (out_codes is not None or out_scales is not None):
-        raise ValueError(f"{name}: out_codes and out_scales need quant")
-    gate_rows = gate_cols = 0
-    if gate is not None:
-        if gate.dim() == 1:
-            gate = gate.unsqueeze(0)
-        if gate.dim() != 2 or gate.shape[0] not in (1, t) or gate.shape[1] not in (1, h):
-            raise ValueError(f"{name}: gate must be [{h}], [{t}, 1] or [{t}, {h}]")
-        if gate.shape[1] == h and h > 1:
-            gate = _rows_of(gate, 16)
-            gate_cols = 1
-        gate_rows = gate.stride(0) if gate.shape[0] == t and t > 1 else 0
-    sf_shape = (t, _blocks(h)) if quant == "block128" else (t,)
-    if out_codes is not None and (out_codes.dtype != _E4M3 or tuple(out_codes.shape) != (t, h) or not out_codes.is_contiguous() or out_codes.data_ptr() % 8 != 0):
-        raise ValueError(f"{name}: out_codes must be a contiguous e4m3 [{t}, {h}], 8-byte aligned")
-    if out_scales is not None and (out_scales.dtype != torch.float32 or tuple(out_scales.shape) != sf_shape or not out_scales.is_contiguous()):
-        raise ValueError(f"{name}: out_scales must be a contiguous float32 {list(sf_shape)}")
-    residual_out = residual if y is None else torch.empty((t, h), dtype=residual.dtype, device=device)
+    r_kind = _type_of(name, residual)
+    y_kind = gate_kind = post_kind = pre_kind = normed_kind = gate_rows = gate_cols = 0
+    y_ptr = post_ptr = gate_ptr = pre_ptr = normed_ptr = codes_ptr = scales_ptr = new_ptr = None
+    y_stride = h
+    r = _rows_of(residual, 16)
+    residual_out = residual
+    if y is not None:
+        y_kind = _type_of(name, y)
+        y = _rows_of(y, 16)
+        y_ptr, y_stride = y.data_ptr(), _pitch(y)
+        residual_out = residual.new_empty((t, h))
+        new_ptr = residual_out.data_ptr()
+        if post_weight is not None:
+            post_weight, post_kind = _norm_weight(name, post_weight, h)
+            post_ptr = post_weight.data_ptr()
+        if gate is not None:
+            gate_kind = _type_of(name, gate)
+            if gate.dim() == 1:
+                gate = gate.unsqueeze(0)
+            if gate.dim() != 2 or gate.shape[0] not in (1, t) or gate.shape[1] not in (1, h):
+                raise ValueError(f"{name}: gate must be [{h}], [{t}, 1] or [{t}, {h}]")
+            if gate.shape[1] == h:
+                gate = _rows_of(gate, 16)
+                gate_cols = 1
+            gate_rows = gate.stride(0) if gate.shape[0] == t and t > 1 else 0
+            gate_ptr = gate.data_ptr()
     normed = codes = scales = None
     if pre_weight is not None:
+        pre_weight, pre_kind = _norm_weight(name, pre_weight, h)
+        pre_ptr = pre_weight.data_ptr()
         if out_normed:
-            normed = torch.empty((t, h), dtype=torch.float32 if residual.dtype == torch.float16 else torch.bfloat16, device=device)
-        if quant is not None:
-            codes = torch.empty((t, h), dtype=_E4M3, device=device) if out_codes is None else out_codes
-            scales = torch.empty(sf_shape, dtype=torch.float32, device=device) if out_scales is None else out_scales
-    if t and (y is not None or normed is not None or codes is not None):
-        r = _rows_of(residual, 16)
-        yy = None if y is None else _rows_of(y, 16)
-        post = None if post_weight is None else _vector(post_weight)
-        pre = None if pre_weight is None or (normed is None and codes is None) else _vector(pre_weight)
-
-        def ptr(v):
-            return None if v is None else v.data_ptr()
-
-        def kind(v):
-            return 0 if v is None else _TYPES[v.dtype]
-        _call(device, _lib.lib().mm_norm_gate_residual, ptr(yy), kind(yy), h if yy is None else max(yy.stride(0), h), r.data_ptr(), kind(r),
-              max(r.stride(0), h), ptr(post), kind(post), ptr(gate), kind(gate), gate_rows, gate_cols, ptr(pre), kind(pre),
-              None if y is None else residual_out.data_ptr(), ptr(normed), kind(normed), ptr(codes), ptr(scales),
-              {None: 0, "block128": 1, "channelwise": 2}[quant], t, h, residual_scale, eps, weight_offset)
+            normed = residual.new_empty((t, h), dtype=torch.float32 if r_kind == 1 else torch.bfloat16)
+            normed_ptr, normed_kind = normed.data_ptr(), 2 if r_kind == 1 else 0
+        if quant_kind:
+            sf_shape = (t, (h + 127) // 128) if quant_kind == 1 else (t,)
+            if out_codes is None:
+                codes = residual.new_empty((t, h), dtype=_E4M3)
+            else:
+                codes = out_codes
+                if codes.dtype != _E4M3 or codes.shape != (t, h) or not codes.is_contiguous() or codes.data_ptr() % 8 != 0:
+                    raise ValueError(f"{name}: out_codes must be a contiguous e4m3 [{t}, {h}], 8-byte aligned")
+            if out_scales is None:
+                scales = residual.new_empty(sf_shape, dtype=torch.float32)
+            else:
+                scales = out_scales
+                if scales.dtype != torch.float32 or scales.shape != sf_shape or not scales.is_contiguous():
+                    raise ValueError(f"{name}: out_scales must be a contiguous float32 {list(sf_shape)}")
+            codes_ptr, scales_ptr = codes.data_ptr(), scales.data_ptr()
+        if normed is None and codes is None:
+            pre_ptr = None
+    if t and (y is not None or pre_ptr is not None):
+        _call(index, _lib.lib().mm_norm_gate_residual, y_ptr, y_kind, y_stride, r.data_ptr(), r_kind, _pitch(r), post_ptr, post_kind, gate_ptr,
+              gate_kind, gate_rows, gate_cols, pre_ptr, pre_kind, new_ptr, normed_ptr, normed_kind, codes_ptr, scales_ptr, quant_kind, t, h,
+              residual_scale, eps, weight_offset)
     return NormOutputs(residual_out, normed, codes, scales)
 
 
-def _vector(w: torch.Tensor) -> torch.Tensor:
-    w = w.contiguous()
-    return w if w.data_ptr() % 16 == 0 else w.clone()
+_QUANT = {None: 0, "block128": 1, "channelwise": 2}
+
+
+def _type_of(name: str, t: torch.Tensor) -> int:
+    kind = _TYPES.get(t.dtype)
+    if kind is None:
+        raise TypeError(f"{name} expects bfloat16, float16 or float32 tensors")
+    return kind
+
+
+def _norm_weight(name: str, w: torch.Tensor, h: int) -> Tuple[torch.Tensor, int]:
+    if w.shape != (h,):
+        raise ValueError(f"{name}: norm weights must be [{h}]")
+    return _dense(w, 16), _type_of(name, w)
