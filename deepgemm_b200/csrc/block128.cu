@@ -173,13 +173,19 @@ int mm_cast_block128(const void* x, int type, int64_t rows, int k, int64_t row_s
     B_REQUIRE(rows < kMaxDim && groups < kMaxDim, "mm_cast_block128: too many groups");
     Device* d;
     if (int rc = device_of(&d)) return rc;
-    int64_t blocks = (groups + 15) / 16;
-    if (blocks > (int64_t)d->sms * 16) blocks = (int64_t)d->sms * 16;
+    const int64_t blocks = (groups + 16 * mm::kCastGroups - 1) / (16 * mm::kCastGroups);
     cudaStream_t st = static_cast<cudaStream_t>(stream_);
     uint8_t* o = static_cast<uint8_t*>(q);
-    if (type == mm::B128_BF16) mm::cast_block128_kernel<mm::B128_BF16><<<(unsigned)blocks, 256, 0, st>>>(x, row_stride, (uint32_t)groups, (uint32_t)per_row, k, o, sf);
-    else if (type == mm::B128_FP16) mm::cast_block128_kernel<mm::B128_FP16><<<(unsigned)blocks, 256, 0, st>>>(x, row_stride, (uint32_t)groups, (uint32_t)per_row, k, o, sf);
-    else mm::cast_block128_kernel<mm::B128_FP32><<<(unsigned)blocks, 256, 0, st>>>(x, row_stride, (uint32_t)groups, (uint32_t)per_row, k, o, sf);
+    const bool flat = k % 128 == 0 && row_stride == k;
+#define B_CAST(T)                                                                                                                                     \
+    do {                                                                                                                                              \
+        if (flat) mm::cast_block128_kernel<T, true><<<(unsigned)blocks, 256, 0, st>>>(x, row_stride, (uint32_t)groups, (uint32_t)per_row, k, o, sf);  \
+        else mm::cast_block128_kernel<T, false><<<(unsigned)blocks, 256, 0, st>>>(x, row_stride, (uint32_t)groups, (uint32_t)per_row, k, o, sf);      \
+    } while (0)
+    if (type == mm::B128_BF16) B_CAST(mm::B128_BF16);
+    else if (type == mm::B128_FP16) B_CAST(mm::B128_FP16);
+    else B_CAST(mm::B128_FP32);
+#undef B_CAST
     B_LAUNCHED();
     return 0;
 }
@@ -227,14 +233,25 @@ int mm_norm_gate_residual(const void* y, int y_type, int64_t y_stride, const voi
     p.y_stride = y_stride; p.r_stride = r_stride; p.gate_row_stride = gate_row_stride; p.gate_col_stride = gate_col_stride;
     p.tokens = tokens; p.hidden = hidden; p.quant = quant; p.alpha = alpha; p.eps = eps; p.offset = offset;
     const int vecs = hidden / 8;
-    const int per = vecs <= 1024 ? 1 : 2;
-    const int threads = ((vecs + per - 1) / per + 31) / 32 * 32;
-    const int resident = 2048 / threads;
-    int64_t blocks = (int64_t)d->sms * (resident < 1 ? 1 : resident);
+    // One vector of 8 values per thread while a row has an SM to itself (one row of 4096: 3.9 us against 4.7) and for an fp32 residual, whose
+    // two would not fit the registers (4000 x 4096: 49 us against 61), else two (see the kernel).  64 registers a thread, so 1024 threads
+    // are resident on an SM; a block more than those waits a whole turn (74 us instead of 62).
+    const bool two = vecs > 1024 || (tokens > 2 * d->sms && r_type != mm::B128_FP32);
+    const int threads = ((two ? (vecs + 1) / 2 : vecs) + 31) / 32 * 32;
+    int64_t blocks = (int64_t)d->sms * (threads < 1024 ? 1024 / threads : 1);
     if (blocks > tokens) blocks = tokens;
     cudaStream_t st = static_cast<cudaStream_t>(stream_);
-    if (per == 1) mm::norm_gate_residual_kernel<1><<<(unsigned)blocks, threads, 0, st>>>(p);
-    else mm::norm_gate_residual_kernel<2><<<(unsigned)blocks, threads, 0, st>>>(p);
+    const bool usual = (!y || y_type == mm::B128_BF16) && (!x_out || x_type == mm::B128_BF16) && (!post || post_type == mm::B128_FP32) &&
+                       (!pre || pre_type == mm::B128_FP32) && (!gate || gate_type == mm::B128_FP32);
+#define B_NORM(V)                                                                                                                                           \
+    do {                                                                                                                                                    \
+        if (usual && r_type == mm::B128_BF16) mm::norm_gate_residual_kernel<V, mm::B128_BF16, mm::B128_BF16, mm::B128_FP32><<<(unsigned)blocks, threads, 0, st>>>(p);   \
+        else if (usual && r_type == mm::B128_FP32) mm::norm_gate_residual_kernel<V, mm::B128_BF16, mm::B128_FP32, mm::B128_FP32><<<(unsigned)blocks, threads, 0, st>>>(p); \
+        else mm::norm_gate_residual_kernel<V, mm::kAny, mm::kAny, mm::kAny><<<(unsigned)blocks, threads, 0, st>>>(p);                                     \
+    } while (0)
+    if (two) B_NORM(2);
+    else B_NORM(1);
+#undef B_NORM
     B_LAUNCHED();
     return 0;
 }

@@ -140,12 +140,12 @@ __global__ void __launch_bounds__(256) moe_route_kernel(const MoeParams p) {
         for (int g0 = (warp - 1) * 2; g0 < groups; g0 += 14) {
             const int g = g0 + (lane >> 4);
             const int col = g * 128 + (lane & 15) * 8;
-            float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (g < groups) load8(p.x, t * p.x_stride + col, B128_BF16, v);
+            F8 v = zero8();
+            if (g < groups) v = load8<B128_BF16>(p.x, t * p.x_stride + col, B128_BF16);
             const float top = group_top(half_warp_max(amax8(v)));
             if (g < groups) {
-                *reinterpret_cast<uint2*>(p.xq_out + static_cast<int64_t>(t) * p.hidden + col) = quantise8(v, GroupQuotient(top));
-                if ((lane & 15) == 0) p.xsf_out[t * groups + g] = __fdiv_rn(top, 448.0f);
+                *reinterpret_cast<uint2*>(p.xq_out + static_cast<int64_t>(t) * p.hidden + col) = quantise_exact(v, top);
+                if ((lane & 15) == 0) p.xsf_out[t * groups + g] = group_scale(top);
             }
         }
     }
@@ -222,7 +222,7 @@ __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int32_t 
 __device__ __forceinline__ void moe_finish_row(const MoeParams& p, float4 g4, float4 u4, bool do_clamp, int64_t place, int nt, int lane) {
     const float g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
     float v[4];
-    uint32_t top_bits = 0;
+    float top = 1.0e-4f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         float a = g[i], b = u[i];
@@ -231,12 +231,13 @@ __device__ __forceinline__ void moe_finish_row(const MoeParams& p, float4 g4, fl
             b = b < -p.clamp ? -p.clamp : (b > p.clamp ? p.clamp : b);
         }
         v[i] = silu_f(a) * b;
-        top_bits = max(top_bits, abs_bits(v[i]));
+        top = max_nan(top, fabsf(v[i]));
     }
-    const float top = group_top(__reduce_max_sync(0xffffffffu, top_bits));
-    const GroupQuotient quot(top);
-    *reinterpret_cast<uint32_t*>(p.act_q + place * p.inter + nt * 128 + lane * 4) = pack4_e4m3(quot(v[0]), quot(v[1]), quot(v[2]), quot(v[3]));
-    if (lane == 0) p.act_sf[place * p.act_sf_pitch + nt] = __fdiv_rn(top, 448.0f);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float mul = 448.0f * rcp_approx(top);
+    *reinterpret_cast<uint32_t*>(p.act_q + place * p.inter + nt * 128 + lane * 4) = pack4_e4m3(v[0] * mul, v[1] * mul, v[2] * mul, v[3] * mul);
+    if (lane == 0) p.act_sf[place * p.act_sf_pitch + nt] = group_scale(top);
 }
 __device__ __forceinline__ void add4(float4& a, const float4& b) { a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w; }
 
