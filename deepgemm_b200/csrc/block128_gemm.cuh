@@ -49,16 +49,39 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap
 }
 // Bounded wait like mbar_wait, for hand-overs that follow one another every few hundred cycles: the clock is not read before the wait
 // has failed a thousand times, because reading it costs more than such a hand-over.
-__device__ __forceinline__ bool mbar_wait_often(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t timeout_ns) {
+__device__ __forceinline__ int ld_shared_volatile(uint32_t addr) {
+    int v;
+    asm volatile("ld.volatile.shared.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void st_shared_volatile(uint32_t addr, int v) { asm volatile("st.volatile.shared.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+__device__ __forceinline__ bool mbar_wait_often(uint32_t bar, uint32_t parity, uint32_t abort_flag, uint64_t timeout_ns) {
     uint64_t t0 = 0;
     for (uint32_t it = 1;; ++it) {
         if (mbar_try_wait(bar, parity)) return true;
         if ((it & 1023u) != 0u) continue;
-        if (*abort_flag != 0) return false;
+        if (ld_shared_volatile(abort_flag) != 0) return false;
         const uint64_t t = global_timer_ns();
         if (t0 == 0) t0 = t;
-        else if (t - t0 > timeout_ns) { *abort_flag = 1; return false; }
+        else if (t - t0 > timeout_ns) { st_shared_volatile(abort_flag, 1); return false; }
     }
+}
+__device__ __forceinline__ float ld_shared_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+// threadIdx.x, read anew each time: what is kept beside the epilogue's 128 sums and 64 staged values makes it spill, and what can be worked
+// out again is therefore not kept.
+__device__ __forceinline__ int tid_again() {
+    int t;
+    asm volatile("mov.u32 %0, %%tid.x;" : "=r"(t));
+    return t;
+}
+__device__ __forceinline__ bool elect_lane() {                        // one lane of a converged warp
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ void mbar_arrive_n(uint32_t bar, uint32_t n) {
     asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar), "r"(n) : "memory");
@@ -131,29 +154,101 @@ __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kLeft> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
 
-// Adds kCols columns of one k block's accumulator (this warp's 32 lanes, from `taddr` on) times `s` to the sums; kLast: they are the
-// warp's last ones, the tensor core may have the buffer back (`arrivals` of the eight that its barrier counts).  Two sums with each fma: plain fma is as fast by itself, but takes twice the
-// issue slots, and the thread that issues the MMAs sits on one of the same four schedulers: beside plain fma four MMAs took 955 cycles,
-// beside fma.rn.f32x2 512, their own rate.  64 columns a step: 336 cycles for a k block, 394 with 32.
-template <int kCols, bool kLast, int kStep = 64>
-__device__ __forceinline__ void b128_promote(uint64_t* sum, uint32_t taddr, float s, uint32_t free_bar, uint32_t arrivals, int lane) {
+// 32 lanes x 16 consecutive columns of 32-bit
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+// Adds one k block's accumulator (kCols columns of this warp's 32 lanes from `taddr` on) to the sums, times row_scale * weight_scale of its
+// place in the ring of scales; then the tensor core may have the buffer back (`free_bar`; kRemote: that of the leader of a CTA pair).
+// 32 columns are on their way from TMEM while the 32 before them are added.  Two sums with each fma: plain fma is as fast by itself, but
+// takes twice the issue slots, and the thread that issues the MMAs sits on one of the same four schedulers: beside plain fma four MMAs took
+// 955 cycles, beside fma.rn.f32x2 512, their own rate.
+template <int kCols, bool kRemote = false>
+__device__ __forceinline__ void b128_promote(uint64_t* sum, uint32_t taddr, uint32_t row_scale, uint32_t weight_scale, uint32_t free_bar) {
+    constexpr int kStep = 16;
+    uint32_t v[2][kStep];
+    tmem_ld_32x16(taddr, v[0]);
+    const float s = ld_shared_f32(row_scale) * ld_shared_f32(weight_scale);
     const uint64_t s2 = pack_f32x2(s, s);
+    tmem_ld_wait();
 #pragma unroll
     for (int c = 0; c < kCols; c += kStep) {
-        uint32_t v[kStep / 32][32];
-#pragma unroll
-        for (int i = 0; i < kStep / 32; ++i) tmem_ld_32x32(taddr + c + 32 * i, v[i]);
-        tmem_ld_wait();
-        if (kLast && c + kStep >= kCols) {
+        uint32_t (&now)[kStep] = v[(c / kStep) & 1];
+        if (c + kStep < kCols) {
+            tmem_ld_32x16(taddr + c + kStep, v[((c / kStep) & 1) ^ 1]);
+        } else {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_n(free_bar, arrivals);
+            if (elect_lane()) {
+                if (kRemote) mbar_arrive_cluster(free_bar);
+                else mbar_arrive(free_bar);
+            }
         }
 #pragma unroll
-        for (int i = 0; i < kStep / 32; ++i)
+        for (int j = 0; j < kStep / 2; ++j) fma_f32x2(sum[c / 2 + j], pack_f32x2(__uint_as_float(now[2 * j]), __uint_as_float(now[2 * j + 1])), s2);
+        if (c + kStep < kCols) tmem_ld_wait();
+    }
+}
+
+// Rounds and stores this warp's part of a tile: rows row0 + lane, columns col0 .. col0 + kCols - 1.
+template <int kCols>
+__device__ __forceinline__ void b128_store(const B128GemmParams& p, const uint64_t* sum, int row0, int col0, bool row_ok, int lane, float* my_staging) {
+    if (p.out_vec32 && col0 + kCols <= p.n) {
+        if (row_ok) {
+            if (p.out_fp32) {
+                float* o = static_cast<float*>(p.out) + static_cast<int64_t>(row0 + lane) * p.out_stride + col0;
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-                fma_f32x2(sum[c / 2 + 16 * i + j], pack_f32x2(__uint_as_float(v[i][2 * j]), __uint_as_float(v[i][2 * j + 1])), s2);
+                for (int j = 0; j < kCols; j += 8) {
+                    uint32_t v[8];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { const float2 f = unpack_f32x2(sum[j / 2 + i]); v[2 * i] = __float_as_uint(f.x); v[2 * i + 1] = __float_as_uint(f.y); }
+                    st_global_32b(o + j, v);
+                }
+            } else {
+                __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + static_cast<int64_t>(row0 + lane) * p.out_stride + col0;
+#pragma unroll
+                for (int j = 0; j < kCols; j += 16) {
+                    uint32_t v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) { const float2 f = unpack_f32x2(sum[j / 2 + i]); v[i] = pack_bf16x2(f.x, f.y); }
+                    st_global_32b(o + j, v);
+                }
+            }
+        }
+    } else {
+        // any number of columns and any alignment: 16 columns at a time through shared memory, so that half a warp writes
+        // neighbouring columns of one row
+        const unsigned rows_ok = __ballot_sync(0xffffffffu, row_ok);
+#pragma unroll
+        for (int c = 0; c < kCols; c += 16) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { const float2 f = unpack_f32x2(sum[c / 2 + j]); my_staging[lane * 17 + 2 * j] = f.x; my_staging[lane * 17 + 2 * j + 1] = f.y; }
+            __syncwarp();
+            const int col = col0 + c + (lane & 15);
+            for (int r = lane >> 4; r < 32; r += 2) {
+                if (!((rows_ok >> r) & 1u) || col >= p.n) continue;
+                const int64_t at = static_cast<int64_t>(row0 + r) * p.out_stride + col;
+                if (p.out_fp32) static_cast<float*>(p.out)[at] = my_staging[r * 17 + (lane & 15)];
+                else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16(my_staging[r * 17 + (lane & 15)]);
+            }
+            __syncwarp();
+        }
+    }
+}
+
+// A 128-row block of a grouped layout: rows of another expert than its first one, or behind padding, are a mistake, reported and not written.
+__device__ __forceinline__ void b128_check_group(const B128GemmParams& p, int mt, int et) {
+    const int first = p.m_indices[mt * 128];
+    const int own = p.m_indices[mt * 128 + et];
+    if ((first >= p.experts || (own >= 0 && own != first)) && atomicCAS(p.status, 0, MM_ERR_BAD_GROUP_LAYOUT) == 0) {
+        p.status[1] = 0; p.status[2] = mt; p.status[3] = first; p.status[4] = own;
     }
 }
 
@@ -174,7 +269,7 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     auto tempty_bar = [&](int a) { return bars + 8u * (2 * kStages + kAccs + a); };
     constexpr int kTail = 8 * (2 * kStages + 2 * kAccs);
     static_assert(kTail + 16 <= S::kBarBytes, "barriers");
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(staging + S::kStagingBytes + kTail);
+    const uint32_t abort_flag = bars + kTail;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(staging + S::kStagingBytes + kTail + 8);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -192,7 +287,7 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) { mbar_init(full_bar(s), 3); mbar_init(empty_bar(s), 1); }
         for (int a = 0; a < kAccs; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), 8); }
-        *abort_flag = 0;
+        st_shared_volatile(abort_flag, 0);
         fence_barrier_init();
         prefetch_tensormap(&tm_a);
         prefetch_tensormap(&tm_b);
@@ -214,7 +309,7 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     };
 
     if (warp < 4) {
-        regs_dec<56>();
+        regs_dec<88>();
         if (warp == 0 && lane == 0) {
             // ------------------------------------------------------------------ TMA
             int stage = 0; uint32_t phase = 0;
@@ -300,102 +395,54 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
         __syncwarp();
     } else {
         // ---------------------------------------------------------------------- epilogue
-        regs_inc<224>();
-        const int q = warp & 3;                              // TMEM lane quarter of this warp
-        const int half = (warp - 4) >> 2;                    // which half of the columns
-        const int et = q * 32 + lane;                        // row of the tile
-        float* my_staging = reinterpret_cast<float*>(staging) + (warp - 4) * 32 * 17;
-        const float* my_scales = reinterpret_cast<const float*>(scales);
-        int acc = 0; uint32_t acc_phase = 0;
-        int slot = 0;
+        regs_inc<208>();                                         // 2 x 208 + 88 = 3 x 168, the registers of the launch
+        // row et of the tile is lane et % 32 of TMEM's quarter et / 32; warps 4-7 take the first half of the columns, 8-11 the second
+        const uint32_t my_tmem = tmem_base + (static_cast<uint32_t>(warp & 3) << 21) + ((warp - 4) >> 2) * kCols;
+        const uint32_t my_scale = smem_u32(scales) + (threadIdx.x & 127) * 4;
+        const uint32_t my_weight_scale = smem_u32(scales) + 512 + (kBN == 256 ? ((warp - 4) >> 2) * 4 : 0);
+        uint32_t n = 0;                                      // k blocks so far: accumulator n % kAccs, place in the ring of scales n % 16
         bool alive = true;
+#pragma unroll 1
         for (int tile = first_tile; tile < num_tiles && alive; tile += tile_step) {
-            int mt, nt;
-            b128_tile(p, tile, mt, nt);
-            const int e = tile_expert(mt);
             if (p.m_indices != nullptr) {
-                // rows of another expert than the block's first one, or behind padding, are a mistake in the layout: reported, not written
-                const int first = p.m_indices[mt * 128];
-                const int own = p.m_indices[mt * 128 + et];
-                if ((first >= p.experts || (own >= 0 && own != first)) && atomicCAS(p.status, 0, MM_ERR_BAD_GROUP_LAYOUT) == 0) {
-                    p.status[1] = 0; p.status[2] = mt; p.status[3] = first; p.status[4] = own;
-                }
+                int mt, nt;
+                b128_tile(p, tile, mt, nt);
+                b128_check_group(p, mt, threadIdx.x & 127);
+                if (tile_expert(mt) < 0) continue;
             }
-            if (e < 0) continue;
-            const int row = mt * 128 + et;
-            bool row_ok = row < p.m;
-            if (row_ok && p.m_indices != nullptr) row_ok = p.m_indices[row] == e;
             uint64_t sum[kCols / 2];
 #pragma unroll
             for (int j = 0; j < kCols / 2; ++j) sum[j] = 0ull;
 #pragma unroll 1
-            for (int kb = kb0; kb < kb1; ++kb) {
-                if (!mbar_wait_often(tfull_bar(acc), acc_phase, abort_flag, p.timeout_ns)) { alive = false; break; }
+            for (int left = kb1 - kb0; left > 0; --left, ++n) {
+                const uint32_t acc = n % kAccs;
+                if (!mbar_wait_often(tfull_bar(acc), (n / kAccs) & 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
                 tc_fence_after();
-                const float* sc = my_scales + slot * (S::kScaleBytes / 4);
-                const float s = sc[et] * sc[128 + (kBN == 256 ? half : 0)];
-                b128_promote<kCols, true>(sum, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * kBN + half * kCols, s, tempty_bar(acc), 1u, lane);
-                if (++acc == kAccs) { acc = 0; acc_phase ^= 1u; }
-                if (++slot == S::kScaleSlots) slot = 0;
+                const uint32_t slot = (n % S::kScaleSlots) * S::kScaleBytes;
+                b128_promote<kCols>(sum, my_tmem + acc * kBN, my_scale + slot, my_weight_scale + slot, tempty_bar(acc));
             }
             if (!alive) break;
             if (kSplit) {
                 // this CTA's part of the tile, for the cluster to add up: the operand ring is idle now (the last accumulator
                 // was complete, so every copy and every MMA of this CTA is done)
-                float* mine = reinterpret_cast<float*>(smem) + et * (kBN + 4) + half * kCols;
+                float* mine = reinterpret_cast<float*>(smem) + (threadIdx.x & 127) * (kBN + 4) + ((warp - 4) >> 2) * kCols;
 #pragma unroll
                 for (int j = 0; j < kCols; j += 4) *reinterpret_cast<float4*>(mine + j) = unpack_f32x4(sum[j / 2], sum[j / 2 + 1]);
                 continue;
             }
-            const int col0 = nt * kBN + half * kCols;
-            if (p.out_vec32 && col0 + kCols <= p.n) {
-                if (row_ok) {
-                    if (p.out_fp32) {
-                        float* o = static_cast<float*>(p.out) + row * p.out_stride + col0;
-#pragma unroll
-                        for (int j = 0; j < kCols; j += 8) {
-                            uint32_t v[8];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) { const float2 f = unpack_f32x2(sum[j / 2 + i]); v[2 * i] = __float_as_uint(f.x); v[2 * i + 1] = __float_as_uint(f.y); }
-                            st_global_32b(o + j, v);
-                        }
-                    } else {
-                        __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + row * p.out_stride + col0;
-#pragma unroll
-                        for (int j = 0; j < kCols; j += 16) {
-                            uint32_t v[8];
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) { const float2 f = unpack_f32x2(sum[j / 2 + i]); v[i] = pack_bf16x2(f.x, f.y); }
-                            st_global_32b(o + j, v);
-                        }
-                    }
-                }
-            } else {
-                // any number of columns and any alignment: 16 columns at a time through shared memory, so that half a warp writes
-                // neighbouring columns of one row
-                const unsigned rows_ok = __ballot_sync(0xffffffffu, row_ok);
-#pragma unroll
-                for (int c = 0; c < kCols; c += 16) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) { const float2 f = unpack_f32x2(sum[c / 2 + j]); my_staging[lane * 17 + 2 * j] = f.x; my_staging[lane * 17 + 2 * j + 1] = f.y; }
-                    __syncwarp();
-                    const int col = col0 + c + (lane & 15);
-                    for (int r = lane >> 4; r < 32; r += 2) {
-                        if (!((rows_ok >> r) & 1u) || col >= p.n) continue;
-                        const int64_t at = (mt * 128 + q * 32 + r) * p.out_stride + col;
-                        if (p.out_fp32) static_cast<float*>(p.out)[at] = my_staging[r * 17 + (lane & 15)];
-                        else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16(my_staging[r * 17 + (lane & 15)]);
-                    }
-                    __syncwarp();
-                }
-            }
+            int mt, nt;
+            b128_tile(p, tile, mt, nt);
+            const int t = tid_again() - 128, row = mt * 128 + (t & 127);
+            bool row_ok = row < p.m;
+            if (row_ok && p.m_indices != nullptr) row_ok = p.m_indices[row] == tile_expert(mt);
+            b128_store<kCols>(p, sum, row & ~31, nt * kBN + (t >> 7) * kCols, row_ok, t & 31, reinterpret_cast<float*>(staging) + (t >> 5) * 32 * 17);
         }
     }
 
     if (kSplit) {
         __syncwarp();
         cluster_sync_all();                                  // every part of the tile is in shared memory
-        if (warp >= 4 && *abort_flag == 0 && first_tile < num_tiles) {
+        if (warp >= 4 && ld_shared_volatile(abort_flag) == 0 && first_tile < num_tiles) {
             int mt, nt;
             b128_tile(p, first_tile, mt, nt);
             const int e = tile_expert(mt);
@@ -434,7 +481,7 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
         cluster_sync_all();                                  // nobody leaves while its part may still be read
     }
 
-    if (*abort_flag != 0) {
+    if (ld_shared_volatile(abort_flag) != 0) {
         // a bounded wait expired: give copies that may still be in flight time to land, then report
         const uint64_t t0 = global_timer_ns();
         while (global_timer_ns() - t0 < 1000000ull) __nanosleep(1000);

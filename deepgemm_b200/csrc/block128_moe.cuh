@@ -181,7 +181,7 @@ struct MoeSegment {
 
 // Shared memory behind the operand ring
 struct MoeWords {
-    volatile int abort;
+    int abort;
     uint32_t tmem;
     volatile int last;                                   // the boss's answer to the other epilogue warps
     int blocks, most;                                    // blocks of routes, routes of the most popular expert
@@ -243,14 +243,33 @@ __device__ __forceinline__ void add4(float4& a, const float4& b) { a.x += b.x; a
 
 // Bounded wait until *p (written by other CTAs, released) has reached `want`.  One thread of a CTA asks, and not without pause: with every
 // warp of every CTA asking (1480 pollers), the counts themselves got through so slowly that a single token took 80 to 150 us.
-__device__ __forceinline__ bool moe_wait_count(const int* p, int want, volatile int* abort_flag, uint64_t timeout_ns) {
+__device__ __forceinline__ bool moe_wait_count(const int* p, int want, uint32_t abort_flag, uint64_t timeout_ns) {
     const uint64_t t0 = global_timer_ns();
     while (ld_acquire_gpu(p) < want) {
-        if (*abort_flag != 0) return false;
-        if (global_timer_ns() - t0 > timeout_ns) { *abort_flag = 1; return false; }
+        if (ld_shared_volatile(abort_flag) != 0) return false;
+        if (global_timer_ns() - t0 > timeout_ns) { st_shared_volatile(abort_flag, 1); return false; }
         __nanosleep(100);
     }
     return true;
+}
+// b128_promote for 64 columns, without its overlap: these tiles wait for HBM, not for their sums.  `arrivals` of the eight that the barrier
+// of the accumulator counts, if kLast.
+template <bool kLast>
+__device__ __forceinline__ void moe_promote(uint64_t* sum, uint32_t taddr, float s, uint32_t free_bar, uint32_t arrivals) {
+    const uint64_t s2 = pack_f32x2(s, s);
+#pragma unroll
+    for (int c = 0; c < 64; c += 32) {
+        uint32_t v[32];
+        tmem_ld_32x32(taddr + c, v);
+        tmem_ld_wait();
+        if (kLast && c == 32) {
+            tc_fence_before();
+            __syncwarp();
+            if (elect_lane()) mbar_arrive_n(free_bar, arrivals);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) fma_f32x2(sum[c / 2 + j], pack_f32x2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), s2);
+    }
 }
 // Whether a phase is complete, without the pause that try_wait may make
 __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
@@ -263,13 +282,13 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 // Bounded wait for something that takes a tile's time
-__device__ __forceinline__ bool mbar_wait_asleep(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t timeout_ns) {
+__device__ __forceinline__ bool mbar_wait_asleep(uint32_t bar, uint32_t parity, uint32_t abort_flag, uint64_t timeout_ns) {
     uint64_t t0 = 0;
     while (!mbar_try_wait(bar, parity)) {
-        if (*abort_flag != 0) return false;
+        if (ld_shared_volatile(abort_flag) != 0) return false;
         const uint64_t t = global_timer_ns();
         if (t0 == 0) t0 = t;
-        else if (t - t0 > timeout_ns) { *abort_flag = 1; return false; }
+        else if (t - t0 > timeout_ns) { st_shared_volatile(abort_flag, 1); return false; }
         __nanosleep(40);
     }
     return true;
@@ -281,14 +300,14 @@ __device__ __forceinline__ int ld_acquire_cta(uint32_t addr) {
     return v;
 }
 // Bounded wait, a warp at a time, until this CTA knows that the activations of block of routes `rb` are finished; returns how many are, or 0.
-__device__ __forceinline__ int moe_wait_ready(uint32_t ready, int rb, int lane, volatile int* abort_flag, uint64_t timeout_ns) {
+__device__ __forceinline__ int moe_wait_ready(uint32_t ready, int rb, int lane, uint32_t abort_flag, uint64_t timeout_ns) {
     int n = 0;
     if (lane == 0) {
         const uint64_t t0 = global_timer_ns();
         while ((n = ld_acquire_cta(ready)) <= rb) {
             n = 0;
-            if (*abort_flag != 0) break;
-            if (global_timer_ns() - t0 > timeout_ns) { *abort_flag = 1; break; }
+            if (ld_shared_volatile(abort_flag) != 0) break;
+            if (global_timer_ns() - t0 > timeout_ns) { st_shared_volatile(abort_flag, 1); break; }
         }
     }
     n = __shfl_sync(0xffffffffu, n, 0);
@@ -325,7 +344,7 @@ __device__ __forceinline__ bool moe_finish_tile(const MoeParams& p, const MoeSme
     auto sync = [&]() {
         __syncwarp();
         if (lane == 0) mbar_arrive(sm.finish_bar());
-        const bool ok = mbar_wait_often(sm.finish_bar(), phase, &sm.words->abort, p.timeout_ns);
+        const bool ok = mbar_wait_often(sm.finish_bar(), phase, smem_u32(&sm.words->abort), p.timeout_ns);
         phase ^= 1u;
         return ok;
     };
@@ -433,10 +452,10 @@ __device__ __forceinline__ bool moe_finish_tile(const MoeParams& p, const MoeSme
 // slots, four columns a thread.  `tiles`: how many there are.
 __device__ __forceinline__ void moe_combine(const MoeParams& p, const MoeSmem& sm, int tiles, uint32_t phase) {
     const int lane = threadIdx.x & 31;
-    if (threadIdx.x == 128 && !moe_wait_count(p.counters + kMoeCtrTiles2, tiles, &sm.words->abort, p.timeout_ns)) return;
+    if (threadIdx.x == 128 && !moe_wait_count(p.counters + kMoeCtrTiles2, tiles, smem_u32(&sm.words->abort), p.timeout_ns)) return;
     __syncwarp();
     if (lane == 0) mbar_arrive(sm.finish_bar());
-    if (!mbar_wait_often(sm.finish_bar(), phase, &sm.words->abort, p.timeout_ns)) return;
+    if (!mbar_wait_often(sm.finish_bar(), phase, smem_u32(&sm.words->abort), p.timeout_ns)) return;
     const int cols4 = p.hidden / 4;
     for (int i = blockIdx.x * 128 + threadIdx.x - 128; i < p.tokens * cols4; i += gridDim.x * 128) {
         const int t = i / cols4, col = (i - t * cols4) * 4;
@@ -469,7 +488,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
     auto tempty_bar = [&](int a) { return sm.bars + 8u * (2 * kMoeMaxStages + 2 + a); };
     auto sfull_bar = [&](int c) { return sm.bars + 8u * (2 * kMoeMaxStages + 4 + c); };
     auto sempty_bar = [&](int c) { return sm.bars + 8u * (2 * kMoeMaxStages + 4 + kMoeSegments + c); };
-    volatile int* abort_flag = &sm.words->abort;
+    const uint32_t abort_flag = smem_u32(&sm.words->abort);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -478,7 +497,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
         for (int c = 0; c < kMoeSegments; ++c) { mbar_init(sfull_bar(c), 1); mbar_init(sempty_bar(c), 15); }
         for (int b = 0; b < 2; ++b) { mbar_init(sm.turn_full(b), 8); mbar_init(sm.turn_empty(b), 4); }
         mbar_init(sm.finish_bar(), 4);
-        *abort_flag = 0;
+        st_shared_volatile(abort_flag, 0);
         st_release_cta(smem_u32(&sm.words->ready), 0);
         fence_barrier_init();
         prefetch_tensormap(&tm_w1);
@@ -814,8 +833,8 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                     const float* sc = sm.scale + slot * (kMoeScaleBytes / 4);
                     const float s_row = sc[et];
                     const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * 256;
-                    b128_promote<64, false, 32>(sum, t_addr + col_a, s_row * sc[sb_a], 0, 0, lane);
-                    b128_promote<64, true, 32>(sum + 32, t_addr + col_b, s_row * sc[sb_b], tempty_bar(acc), arrivals, lane);
+                    moe_promote<false>(sum, t_addr + col_a, s_row * sc[sb_a], 0, 0);
+                    moe_promote<true>(sum + 32, t_addr + col_b, s_row * sc[sb_b], tempty_bar(acc), arrivals);
                     if (++slot == kMoeScaleSlots) slot = 0;
                     if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
                 }
@@ -865,7 +884,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
         }
     }
 
-    if (*abort_flag != 0) {
+    if (ld_shared_volatile(abort_flag) != 0) {
         // a bounded wait expired: give copies that may still be in flight time to land, then report
         const uint64_t t0 = global_timer_ns();
         while (global_timer_ns() - t0 < 1000000ull) __nanosleep(1000);
