@@ -5,14 +5,13 @@
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
-#include <stdlib.h>
+
 #include <mutex>
 
 #include "../../include/megamoe_b200.h"
 #include "block128.cuh"
 #include "block128_gemm.cuh"
 #include "block128_moe.cuh"
-#include "block128_pair.cuh"
 #include "layout.h"
 
 // abi.cu: error message, launch counter and wait limit of the library
@@ -81,7 +80,6 @@ int device_of(Device** out) {
         B_CUDA(cudaFuncSetAttribute(mm::block128_gemm_kernel<256, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, mm::B128Shape<256>::kSmemBytes));
         B_CUDA(cudaFuncSetAttribute(mm::block128_gemm_kernel<128, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, mm::B128Shape<128>::kSmemBytes));
         B_CUDA(cudaFuncSetAttribute(mm::block128_gemm_kernel<128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, mm::B128Shape<128>::kSmemBytes));
-        B_CUDA(cudaFuncSetAttribute(mm::block128_gemm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, mm::kB128PairSmemBytes));
         B_CUDA(cudaFuncSetAttribute(mm::moe_experts_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, mm::kMoeSmemBytes));
         d.ready = true;
     }
@@ -293,21 +291,15 @@ int mm_fp8_gemm_block128(const void* a, int64_t a_stride, const float* sa, int64
     p.n_tiles = bn == 256 ? (n + 255) / 256 : n_sf;
     int split = 1;
     while (bn == 128 && !m_indices && split < 8 && tiles * split * 2 <= d->sms && kb >= split * 4) split *= 2;
-    const bool pair = getenv("PAIR") ? atoi(getenv("PAIR")) : 0;
-    if (pair) p.n_tiles = (n + 255) / 256;
-    const int b_box = pair ? 128 : bn;
     CUtensorMap tm_a, tm_b;
     if (int rc = byte_map(a, (uint64_t)k, (uint64_t)m, (uint64_t)a_stride, 0, 0, (uint32_t)p.a_box_rows, &tm_a)) return rc;
     if (p.tiled) {
-        if (int rc = byte_map(b, 128, (uint64_t)experts * p.tiled_n_blocks * kb * 256, 128, 0, 0, (uint32_t)b_box, &tm_b)) return rc;
+        if (int rc = byte_map(b, 128, (uint64_t)experts * p.tiled_n_blocks * kb * 256, 128, 0, 0, (uint32_t)bn, &tm_b)) return rc;
     } else {
-        if (int rc = byte_map(b, (uint64_t)k, (uint64_t)n, (uint64_t)k, (uint64_t)experts, (uint64_t)n * k, (uint32_t)b_box, &tm_b)) return rc;
+        if (int rc = byte_map(b, (uint64_t)k, (uint64_t)n, (uint64_t)k, (uint64_t)experts, (uint64_t)n * k, (uint32_t)bn, &tm_b)) return rc;
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream_);
-    if (pair) {
-        p.a_box_rows = 128;
-        mm::block128_gemm_pair_kernel<<<d->sms / 2 * 2, mm::kB128Threads, mm::kB128PairSmemBytes, st>>>(tm_a, tm_b, p);
-    } else if (split > 1) {
+    if (split > 1) {
         cudaLaunchConfig_t cfg;
         memset(&cfg, 0, sizeof(cfg));
         cfg.gridDim = dim3((unsigned)(tiles * split));

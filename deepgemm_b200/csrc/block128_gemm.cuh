@@ -166,11 +166,12 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
 }
 
 // Adds one k block's accumulator (kCols columns of this warp's 32 lanes from `taddr` on) to the sums, times row_scale * weight_scale of its
-// place in the ring of scales; then the tensor core may have the buffer back (`free_bar`; kRemote: that of the leader of a CTA pair).
-// 32 columns are on their way from TMEM while the 32 before them are added.  Two sums with each fma: plain fma is as fast by itself, but
+// place in the ring of scales; then the tensor core may have the buffer back (`free_bar`).  16 columns are on their way from TMEM while
+// the 16 before them are added (with 32, the sums and what is staged do not fit the registers any more, and a spilled word in this loop costs
+// a fifth of the rate).  Two sums with each fma: plain fma is as fast by itself, but
 // takes twice the issue slots, and the thread that issues the MMAs sits on one of the same four schedulers: beside plain fma four MMAs took
 // 955 cycles, beside fma.rn.f32x2 512, their own rate.
-template <int kCols, bool kRemote = false>
+template <int kCols>
 __device__ __forceinline__ void b128_promote(uint64_t* sum, uint32_t taddr, uint32_t row_scale, uint32_t weight_scale, uint32_t free_bar) {
     constexpr int kStep = 16;
     uint32_t v[2][kStep];
@@ -186,10 +187,7 @@ __device__ __forceinline__ void b128_promote(uint64_t* sum, uint32_t taddr, uint
         } else {
             tc_fence_before();
             __syncwarp();
-            if (elect_lane()) {
-                if (kRemote) mbar_arrive_cluster(free_bar);
-                else mbar_arrive(free_bar);
-            }
+            if (elect_lane()) mbar_arrive(free_bar);
         }
 #pragma unroll
         for (int j = 0; j < kStep / 2; ++j) fma_f32x2(sum[c / 2 + j], pack_f32x2(__uint_as_float(now[2 * j]), __uint_as_float(now[2 * j + 1])), s2);
