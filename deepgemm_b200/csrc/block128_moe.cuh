@@ -183,7 +183,7 @@ struct MoeSegment {
 struct MoeWords {
     int abort;
     uint32_t tmem;
-    volatile int last;                                   // the boss's answer to the other epilogue warps
+    volatile int last[2];                                // the boss's answer to the other finishing warps, one for each tile in turn
     int blocks, most;                                    // blocks of routes, routes of the most popular expert
     int ready;                                           // blocks of routes whose activations this CTA knows to be finished
     MoeList list[2];                                     // of either product
@@ -356,9 +356,9 @@ __device__ __forceinline__ bool moe_finish_tile(const MoeParams& p, const MoeSme
     if (!whole) {
         // the parts are added up by whoever brings the last one, in the order of the chunks
         release();                                       // parts have memory of their own
-        if (boss) sm.words->last = atomic_add_acq_rel(p.counters + (kind ? p.ctr_tile2 : p.ctr_tile1) + tile, units) + units == l.kb;
+        if (boss) sm.words->last[buffer] = atomic_add_acq_rel(p.counters + (kind ? p.ctr_tile2 : p.ctr_tile1) + tile, units) + units == l.kb;
         if (!sync()) return false;
-        if (sm.words->last == 0) return true;
+        if (sm.words->last[buffer] == 0) return true;    // (written again two tiles on, behind a barrier of the tile between)
         c0 = l.chunk_of(tile * l.kb);
         c1 = l.chunk_of(tile * l.kb + l.kb - 1);
     }
@@ -745,7 +745,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                             if (lane == 0) st_release_cta(smem_u32(&sm.words->ready), ready_blocks);
                             __syncwarp();                            // what lane 0 has acquired, the others may read
                         } else {
-                            if (ld_acquire_cta(smem_u32(&sm.words->ready)) <= rb) drain();
+                            if (!__all_sync(0xffffffffu, ld_acquire_cta(smem_u32(&sm.words->ready)) > rb)) drain();
                             ready_blocks = moe_wait_ready(smem_u32(&sm.words->ready), rb, lane, abort_flag, p.timeout_ns);
                             if (ready_blocks == 0) { alive = false; break; }
                         }
