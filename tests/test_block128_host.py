@@ -74,3 +74,84 @@ def test_python_checks_on_cpu_tensors():
         megamoe.cast_to_fp8_block128(x.double())
     with pytest.raises(TypeError):
         megamoe.cast_weight_to_fp8_block128(x[0])
+
+
+def test_layer_entry_point_refuses(built_lib):
+    def call(x=P, fp8=0, xs=256, xsf=None, logits=P, ls=8, idx=None, w=None, w1=P, work=P, y=P, t=4, e=8, k=2, h=256, i=128, clamp=float("inf")):
+        return built_lib.mm_moe_few_tokens(x, fp8, xs, xsf, logits, ls, idx, 0, w, w1, P, P, P, 0, t, e, k, h, i, clamp, work, 1 << 40, y, None)
+    _refused(built_lib, call(k=9), "topk")
+    _refused(built_lib, call(k=0), "topk")
+    _refused(built_lib, call(e=64, k=33), "topk")
+    _refused(built_lib, call(e=2000), "experts")
+    _refused(built_lib, call(h=200), "multiples of 128")
+    _refused(built_lib, call(i=100), "multiples of 128")
+    _refused(built_lib, call(h=65536, xs=65536), "at most")
+    _refused(built_lib, call(t=2049), "routes")
+    _refused(built_lib, call(clamp=0.0), "clamp")
+    _refused(built_lib, call(clamp=float("nan")), "clamp")
+    _refused(built_lib, call(w1=None), "null")
+    _refused(built_lib, call(fp8=1), "null")
+    _refused(built_lib, call(fp8=1, xsf=P, xs=512), "contiguous")
+    _refused(built_lib, call(idx=P, w=P), "either")
+    _refused(built_lib, call(logits=None), "either")
+    _refused(built_lib, call(logits=None, idx=P), "either")
+    _refused(built_lib, call(x=P + 8), "aligned")
+    _refused(built_lib, call(xs=248), "aligned")
+    _refused(built_lib, call(work=P + 16), "aligned")
+    _refused(built_lib, call(ls=7), "stride")
+    assert call(t=0) == 0
+    _refused(built_lib, built_lib.mm_moe_few_tokens_workspace(4, 8, 2, 256, 128, None), "null")
+    _refused(built_lib, built_lib.mm_block128_read_status(None, None), "null")
+
+
+def test_layer_python_checks(monkeypatch):
+    """What the layer's Python entry refuses, on CPU tensors that it is told to take for a GPU's."""
+    import megamoe
+    from deepgemm_b200.megamoe import block128
+    monkeypatch.setattr(block128, "_device_index", lambda *a: 0)
+    e, k, h, i, t = 4, 2, 256, 128, 3
+    codes = lambda *s: torch.zeros(s, dtype=torch.uint8).view(torch.float8_e4m3fn)   # noqa: E731
+    good = dict(x=torch.zeros((t, h), dtype=torch.bfloat16), l1_weights=(codes(e, 2 * i, h), torch.ones((e, 2, 2))), l2_weights=(codes(e, h, i), torch.ones((e, 2, 1))),
+                router_logits=torch.zeros((t, e)), num_topk=k)
+    chosen = dict(router_logits=None, num_topk=None, topk_idx=torch.zeros((t, k), dtype=torch.int32), topk_weights=torch.ones((t, k)))
+    bad = [
+        (dict(x=torch.zeros((t, h))), "bfloat16"),
+        (dict(x=(codes(t, h), torch.ones((t, 1)))), "scales of x"),
+        (dict(x=torch.zeros((t, 128), dtype=torch.bfloat16)), "do not match"),
+        (dict(l1_weights=(codes(e, i, h), good["l1_weights"][1])), "do not match"),
+        (dict(l1_weights=(codes(e, 2 * i, 2 * h)[:, :, ::2], good["l1_weights"][1])), "contiguous"),
+        (dict(l2_weights=(good["l2_weights"][0], torch.ones((e, 2, 2)))), "do not match"),
+        (dict(l2_weights=(torch.zeros((e, h, i)), good["l2_weights"][1])), "e4m3"),
+        (dict(router_logits=None), "either"),
+        (dict(topk_idx=chosen["topk_idx"]), "either"),
+        (dict(num_topk=None), "num_topk"),
+        (dict(num_topk=e + 1), "topk must be"),
+        (dict(router_logits=torch.zeros((t, e), dtype=torch.bfloat16)), "fp32"),
+        (dict(chosen, topk_weights=None), "both be"),
+        (dict(chosen, topk_idx=torch.zeros((t, k), dtype=torch.int16)), "int32 or int64"),
+        (dict(chosen, num_topk=1), "does not match"),
+        (dict(activation_clamp=-1.0), "positive"),
+        (dict(out=torch.zeros((t, h))), "out must be"),
+        (dict(x=torch.zeros((2049, h), dtype=torch.bfloat16), router_logits=torch.zeros((2049, e))), "4096 routes"),
+    ]
+    for change, words in bad:
+        with pytest.raises((RuntimeError, ValueError), match=words):
+            megamoe.fp8_moe_few_tokens(**{**good, **change})
+
+
+def test_product_python_checks(monkeypatch):
+    import megamoe
+    from deepgemm_b200.megamoe import block128
+    monkeypatch.setattr(block128, "_device_index", lambda *a: 0)
+    codes = lambda *s: torch.zeros(s, dtype=torch.uint8).view(torch.float8_e4m3fn)   # noqa: E731
+    a, b, w = (codes(128, 256), torch.ones((128, 2))), (codes(64, 256), torch.ones((1, 2))), (codes(3, 64, 256), torch.ones((3, 1, 2)))
+    for args, kw, words in (((a, (b[0], torch.ones((2, 2)))), {}, "weight scales"), (((a[0], torch.ones((128, 1))), b), {}, "with scales"),
+                            ((a, b), dict(out_dtype=torch.float16), "bfloat16 or float32"), ((a, b), dict(out=torch.zeros((128, 65))), "out must be"),
+                            (((a[0][:, :200], a[1]), (b[0][:, :200], b[1])), {}, "multiple of 16"), (((a[0].float(), a[1]), b), {}, "e4m3"), ((a, w), {}, "2D")):
+        with pytest.raises(RuntimeError, match=words):
+            megamoe.fp8_gemm_nt_block128(*args, **kw)
+    d, idx = torch.zeros((128, 64), dtype=torch.bfloat16), torch.zeros(128, dtype=torch.int32)
+    for args, words in (((a, w, d.half(), idx), "contiguous bfloat16"), ((a, w, d, idx.long()), "int32"), ((a, b, d, idx), "expects weights"),
+                        ((a, w, d[:, :48].contiguous(), idx), "do not match"), (((a[0][:100], a[1][:100]), w, d[:100], idx[:100]), "multiple of 128")):
+        with pytest.raises(RuntimeError, match=words):
+            megamoe.m_grouped_fp8_gemm_nt_contiguous_block128(*args)
