@@ -120,7 +120,7 @@ int byte_map(const void* ptr, uint64_t inner, uint64_t rows, uint64_t row_stride
 // Work memory of mm_moe_few_tokens, in bytes from its start
 struct MoeWork {
     int64_t counters, route_expert, route_w, xq, xsf, act_q, act_sf, rows_out, parts, total;
-    int num_counters, ctr_done1, ctr_tile1, ctr_tile2, part_rows, act_sf_pitch;
+    int num_counters, ctr_done1, ctr_tile1, part_rows, act_sf_pitch;
 };
 
 MoeWork moe_work(int T, int E, int K, int H, int I, bool cast, int ctas) {
@@ -129,11 +129,10 @@ MoeWork moe_work(int T, int E, int K, int H, int I, bool cast, int ctas) {
     auto take = [&](int64_t bytes) { const int64_t o = at; at = (at + bytes + 255) / 256 * 256; return o; };
     const int64_t routes = (int64_t)T * K;
     const int64_t blocks = (routes < E ? routes : E) + routes / 128;
-    const int64_t nt1 = I / 128, nt2 = (H + 255) / 256;
+    const int64_t nt1 = I / 128;
     w.ctr_done1 = 32;
     w.ctr_tile1 = w.ctr_done1 + (int)blocks;
-    w.ctr_tile2 = w.ctr_tile1 + (int)(blocks * nt1);
-    w.num_counters = w.ctr_tile2 + (int)(blocks * nt2);
+    w.num_counters = w.ctr_tile1 + (int)(blocks * nt1);
     w.part_rows = (int)(routes < 128 ? routes : 128);
     w.counters = take((int64_t)w.num_counters * 4);
     w.route_expert = take(routes * 4);
@@ -364,7 +363,7 @@ int mm_moe_few_tokens(const void* x, int x_is_fp8, int64_t x_stride, const float
     p.route_w = reinterpret_cast<float*>(base + w.route_w);
     p.counters = reinterpret_cast<int*>(base + w.counters);
     p.num_counters = w.num_counters;
-    p.ctr_done1 = w.ctr_done1; p.ctr_tile1 = w.ctr_tile1; p.ctr_tile2 = w.ctr_tile2;
+    p.ctr_done1 = w.ctr_done1; p.ctr_tile1 = w.ctr_tile1;
     p.s1 = s1; p.s2 = s2; p.tiled = tiled ? 1 : 0;
     p.act_q = base + w.act_q; p.act_sf = reinterpret_cast<float*>(base + w.act_sf); p.act_sf_pitch = w.act_sf_pitch;
     p.rows_out = reinterpret_cast<float*>(base + w.rows_out);

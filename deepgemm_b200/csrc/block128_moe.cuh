@@ -40,7 +40,7 @@ constexpr int kMoePlanBytes = kMoeMaxRoutes * 2 + kMoeMaxBlocks * 8 + kMoeMaxRou
 constexpr int kMoeTurnRows = 6, kMoeTurnPitch = 260;    // fp32 rows that go from the summing to the finishing warps, in two buffers
 constexpr int kMoeThreads = 512;
 constexpr int kMoeSegments = 8;
-constexpr int kMoeCtrTiles1 = 8, kMoeCtrTiles2 = 16;
+constexpr int kMoeCtrTiles1 = 8, kMoeCtrUnits2 = 16;
 constexpr int kMoeTailBytes = 768;        // barriers and MoeWords
 // Scales of a unit: 128 rows, then two of the weights.  As in block128_gemm.cuh: stages + accumulators + 1 units may be on their way.
 constexpr int kMoeScaleSlots = 8, kMoeScaleBytes = 544;
@@ -60,15 +60,15 @@ struct MoeParams {
     uint8_t* xq_out; float* xsf_out;
     int* route_expert; float* route_w;       // [tokens * topk], -1 = none
     int* counters; int num_counters;
-    // counters: [0] claims, [kMoeCtrTiles1] and [kMoeCtrTiles2] finished tiles of either product, [ctr_done1 ..) of the first one by
-    // block of routes, [ctr_tile1 ..) and [ctr_tile2 ..) k blocks that have arrived for each tile that was cut
-    int ctr_done1, ctr_tile1, ctr_tile2;
+    // counters: [0] claims, [kMoeCtrTiles1] finished tiles of the first product, [ctr_done1 ..) the same by block of routes, [ctr_tile1 ..)
+    // k blocks that have arrived for each of its tiles that was cut, [kMoeCtrUnits2] k blocks of the second product whose sums are written
+    int ctr_done1, ctr_tile1;
     const float* s1; const float* s2;
     int tiled;
     // [routes][inter] and [routes][inter / 128], by place in the sorted list.  A row of scales has 128-byte lines of its own: they are
     // read through L1, which must not hold a line that another expert's tiles are still writing to
     uint8_t* act_q; float* act_sf; int act_sf_pitch;
-    float* rows_out;                         // [routes][hidden]: weighted rows of the second product, by route
+    float* rows_out;                         // [routes][hidden]: weighted rows of the second product, by route, where a tile is whole
     float* parts; int part_rows;             // [2 products][chunks][2][part_rows][256], then [CTAs][2][part_rows][256] for tiles that are whole
     __nv_bfloat16* y;
     float clamp;
@@ -82,35 +82,35 @@ __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.laun
 // kPer: experts per lane.  Ties go to the lower index; NaN and -inf logits are never chosen.
 template <int kPer>
 __device__ __forceinline__ void moe_topk(const MoeParams& p, int t, int lane) {
-    float v[kPer];
+    // Floats as integers of the same order, 0 for what cannot be chosen: two warp reductions find a maximum and its lowest index, where
+    // comparing pairs of floats and indexes took ten shuffles.
+    uint32_t v[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int e = lane + 32 * i;
         const float l = e < p.experts ? p.logits[t * p.logits_stride + e] : -INFINITY;
-        v[i] = l == l ? l : -INFINITY;
+        const uint32_t bits = __float_as_uint(l == 0.0f ? 0.0f : l);                     // -0 and 0 are a tie
+        v[i] = l > -INFINITY ? (bits >> 31 ? ~bits : bits | 0x80000000u) : 0u;
     }
     float sel = 0.0f, sum = 0.0f, top = 0.0f;
     int sel_e = -1;
     for (int k = 0; k < p.topk; ++k) {
-        float best = -INFINITY;
-        int best_e = -1;
+        uint32_t best = 0;
+        int best_i = 0;
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
-            if (v[i] > best) { best = v[i]; best_e = lane + 32 * i; }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float ob = __shfl_xor_sync(0xffffffffu, best, o);
-            const int oe = __shfl_xor_sync(0xffffffffu, best_e, o);
-            if (ob > best || (ob == best && oe >= 0 && oe < best_e)) { best = ob; best_e = oe; }
-        }
-        if (best_e < 0) break;                                       // nothing left to choose from
-        if (k == 0) top = best;
-        const float w = best == top ? 1.0f : expf(best - top);       // equal infinities share alike
+            if (v[i] > best) { best = v[i]; best_i = i; }
+        const uint32_t most = __reduce_max_sync(0xffffffffu, best);
+        if (most == 0) break;                                        // nothing left to choose from
+        const int best_e = static_cast<int>(__reduce_min_sync(0xffffffffu, best == most ? static_cast<uint32_t>(lane + 32 * best_i) : 0xffffffffu));
+        const float value = __uint_as_float(most >> 31 ? most & 0x7fffffffu : ~most);
+        if (k == 0) top = value;
+        const float w = value == top ? 1.0f : expf(value - top);     // equal infinities share alike
         sum += w;
         if (lane == k) { sel = w; sel_e = best_e; }
         if ((best_e & 31) == lane) {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) if (i == (best_e >> 5)) v[i] = -INFINITY;
+            for (int i = 0; i < kPer; ++i) if (i == (best_e >> 5)) v[i] = 0u;
         }
     }
     if (lane < p.topk) {
@@ -352,19 +352,29 @@ __device__ __forceinline__ bool moe_finish_tile(const MoeParams& p, const MoeSme
         __syncwarp();
         if (lane == 0) mbar_arrive(sm.turn_empty(buffer));
     };
+    if (kind) {
+        // rows of a whole tile are in their place already, parts are added up by the combine
+        release();
+        if (boss) {
+            __threadfence();
+            atomicAdd(p.counters + kMoeCtrUnits2, units);
+        }
+        return true;
+    }
     int c0 = g.chunk, c1 = g.chunk;
     if (!whole) {
         // the parts are added up by whoever brings the last one, in the order of the chunks
         release();                                       // parts have memory of their own
-        if (boss) sm.words->last[buffer] = atomic_add_acq_rel(p.counters + (kind ? p.ctr_tile2 : p.ctr_tile1) + tile, units) + units == l.kb;
+        if (boss) sm.words->last[buffer] = atomic_add_acq_rel(p.counters + p.ctr_tile1 + tile, units) + units == l.kb;
         if (!sync()) return false;
         if (sm.words->last[buffer] == 0) return true;    // (written again two tiles on, behind a barrier of the tile between)
         c0 = l.chunk_of(tile * l.kb);
         c1 = l.chunk_of(tile * l.kb + l.kb - 1);
     }
-    // Four columns each from two places (gate and up, or two runs of outputs) of two rows, the second one four behind: eight loads in
+    // Four columns each of gate and up of two rows, the second one four behind: eight loads in
     // flight, two parts at a time, added in order.  v[row][place].
-    auto join = [&](int row, int col_a, int col_b, float4 (&v)[2][2]) {
+    auto join = [&](int row, float4 (&v)[2][2]) {
+        const int col_a = lane * 4, col_b = 128 + lane * 4;
         const bool two = row + 4 < rows;
         if (turn) {
             const float* in = my_turn + row * kMoeTurnPitch;
@@ -383,7 +393,7 @@ __device__ __forceinline__ bool moe_finish_tile(const MoeParams& p, const MoeSme
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 if (ch + i > c1) continue;
-                const float* in = moe_part(p, l, kind, ch + i, tile, whole, buffer) + row * 256;
+                const float* in = moe_part(p, l, 0, ch + i, tile, whole, buffer) + row * 256;
                 f[i][0][0] = __ldcg(reinterpret_cast<const float4*>(in + col_a));
                 f[i][0][1] = __ldcg(reinterpret_cast<const float4*>(in + col_b));
                 if (two) {
@@ -400,78 +410,97 @@ __device__ __forceinline__ bool moe_finish_tile(const MoeParams& p, const MoeSme
             }
         }
     };
-    if (kind == 0) {
-        // a row at a time for each warp: with one thread to a row, as the sums were held, a tile of few rows would keep eight warps
-        // waiting for the few threads that have any
-        const bool do_clamp = p.clamp < 3.0e38f;
-        for (int r = fw; r < rows; r += 8) {
-            float4 v[2][2];
-            join(r, lane * 4, 128 + lane * 4, v);
-            moe_finish_row(p, v[0][0], v[0][1], do_clamp, static_cast<int64_t>(g.first) + r, nt, lane);
-            if (r + 4 < rows) moe_finish_row(p, v[1][0], v[1][1], do_clamp, static_cast<int64_t>(g.first) + r + 4, nt, lane);
-        }
-        if (whole) release();
-        if (!sync()) return false;
-        if (boss) {
-            __threadfence();
-            atomicAdd(p.counters + p.ctr_done1 + rb, 1);
-            atomicAdd(p.counters + kMoeCtrTiles1, 1);
-        }
-        return true;
+    // a row at a time for each warp: with one thread to a row, as the sums were held, a tile of few rows would keep eight warps
+    // waiting for the few threads that have any
+    const bool do_clamp = p.clamp < 3.0e38f;
+    for (int r = fw; r < rows; r += 8) {
+        float4 v[2][2];
+        join(r, v);
+        moe_finish_row(p, v[0][0], v[0][1], do_clamp, static_cast<int64_t>(g.first) + r, nt, lane);
+        if (r + 4 < rows) moe_finish_row(p, v[1][0], v[1][1], do_clamp, static_cast<int64_t>(g.first) + r + 4, nt, lane);
     }
-    const int cols = min(256, p.hidden - nt * 256);
-    if (whole) {
-        release();                                       // the rows are in their place already
-    } else {
-        for (int r = fw; r < rows; r += 8) {
-            float4 v[2][2];
-            join(r, lane * 4, 128 + lane * 4, v);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (r + 4 * i >= rows) continue;
-                const uint32_t rr = sm.route[g.first + r + 4 * i];
-                const float w = p.route_w[rr];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int col = lane * 4 + 128 * j;
-                    const float4 t = v[i][j];
-                    if (col < cols) *reinterpret_cast<float4*>(p.rows_out + static_cast<int64_t>(rr) * p.hidden + nt * 256 + col) = make_float4(t.x * w, t.y * w, t.z * w, t.w * w);
-                }
-            }
-        }
-    }
+    if (whole) release();
     if (!sync()) return false;
     if (boss) {
         __threadfence();
-        atomicAdd(p.counters + kMoeCtrTiles2, 1);
+        atomicAdd(p.counters + p.ctr_done1 + rb, 1);
+        atomicAdd(p.counters + kMoeCtrTiles1, 1);
     }
     return true;
 }
 
-// The combine, by the finishing warps of every CTA once all tiles of the second product are finished: each token's rows, in the order of its
-// slots, four columns a thread.  `tiles`: how many there are.
-__device__ __forceinline__ void moe_combine(const MoeParams& p, const MoeSmem& sm, int tiles, uint32_t phase) {
-    const int lane = threadIdx.x & 31;
-    if (threadIdx.x == 128 && !moe_wait_count(p.counters + kMoeCtrTiles2, tiles, smem_u32(&sm.words->abort), p.timeout_ns)) return;
-    __syncwarp();
+// The combine, by the finishing warps of every CTA once the sums of all `units` of the second product are written: each token's rows, in the
+// order of its slots, four columns a thread.  A tile that was cut is read as its parts, in the order of the chunks: adding them up
+// first, by whoever brings the last one, and reading the sum then made the end of a call for one token 7 us long instead of 4.
+__device__ __forceinline__ void moe_combine(const MoeParams& p, const MoeSmem& sm, uint8_t* ring, int units, uint32_t phase) {
+    const int tid = threadIdx.x - 128, lane = threadIdx.x & 31;
+    const MoeList& l = sm.words->list[1];
+    const int nt2 = (p.hidden + 255) / 256;
+    // The operand ring has done its work.  Of each route: first tile of its block | row << 16; of each tile: place of its first part | parts
+    // << 16, or 0 parts if it is whole.
+    uint32_t* place = reinterpret_cast<uint32_t*>(ring);
+    uint32_t* parts_of = place + kMoeMaxRoutes;
+    const bool cut = l.shares;                                       // (fewer tiles than 16 for each CTA, and a GPU has fewer than 1024 SMs)
+    static_assert(kMoeMaxRoutes * 4 + kMoeStreamTiles * 1024 * 4 <= kMoeRingBytes && kMoeStreamTiles * 1024 <= 65536, "places and parts");
+    const int64_t step = static_cast<int64_t>(p.part_rows) * 256;    // from a tile's first part to its second; two of these to each one after (moe_part)
+    const float* parts2 = p.parts + static_cast<int64_t>(gridDim.x) * 2 * step;      // of the second product
+    if (cut) {
+        const int blocks = sm.words->blocks;
+        for (int b = tid >> 5; b < blocks; b += 4) {
+            const uint2 blk = sm.block[b];
+            for (uint32_t r = lane; r < blk.x >> 16; r += 32) place[sm.route[blk.y + r]] = static_cast<uint32_t>(b * nt2) | r << 16;
+        }
+        // (the divisions of chunk_of here, once for each tile and while others still work: 24 of them in a thread's way to its loads took 6 us)
+        for (int t = tid; t < l.tiles; t += 128) {
+            const int c0 = l.chunk_of(t * l.kb), n = l.chunk_of(t * l.kb + l.kb - 1) - c0 + 1;
+            parts_of[t] = static_cast<uint32_t>(c0 * 2 + 1) | static_cast<uint32_t>(n == 1 ? 0 : n) << 16;
+        }
+    }
+    const bool ok = tid != 0 || moe_wait_count(p.counters + kMoeCtrUnits2, units, smem_u32(&sm.words->abort), p.timeout_ns);
+    if (!__all_sync(0xffffffffu, ok)) return;
     if (lane == 0) mbar_arrive(sm.finish_bar());
     if (!mbar_wait_often(sm.finish_bar(), phase, smem_u32(&sm.words->abort), p.timeout_ns)) return;
     const int cols4 = p.hidden / 4;
-    for (int i = blockIdx.x * 128 + threadIdx.x - 128; i < p.tokens * cols4; i += gridDim.x * 128) {
+    for (int i = blockIdx.x * 128 + tid; i < p.tokens * cols4; i += gridDim.x * 128) {
         const int t = i / cols4, col = (i - t * cols4) * 4;
         const int r0 = t * p.topk;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < p.topk; s += 8) {
-            float4 f[8];
-            bool ok[8];
+        constexpr int kSlots = 8;
+        for (int s = 0; s < p.topk; s += kSlots) {
+            float4 f[kSlots], f2[kSlots];
+            float w[kSlots];
+            int n[kSlots];                                           // parts, 0: no route, -1: a row that is whole
+            const float* src[kSlots];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < kSlots; ++j) {
                 const int r = r0 + s + j;
-                ok[j] = s + j < p.topk && ((sm.valid[r >> 5] >> (r & 31)) & 1u);
-                if (ok[j]) f[j] = __ldcg(reinterpret_cast<const float4*>(p.rows_out + static_cast<int64_t>(r) * p.hidden + col));
+                n[j] = 0;
+                if (s + j < p.topk && ((sm.valid[r >> 5] >> (r & 31)) & 1u)) {
+                    n[j] = -1;
+                    src[j] = p.rows_out + static_cast<int64_t>(r) * p.hidden + col;
+                    if (cut) {
+                        const uint32_t at = place[r];
+                        const uint32_t parts = parts_of[(at & 0xffff) + (col >> 8)];
+                        if (parts >> 16) {
+                            n[j] = static_cast<int>(parts >> 16);
+                            src[j] = parts2 + (parts & 0xffff) * step + (at >> 16) * 256 + (col & 255);
+                            w[j] = p.route_w[r];
+                            f2[j] = __ldcg(reinterpret_cast<const float4*>(src[j] + step));
+                        }
+                    }
+                    f[j] = __ldcg(reinterpret_cast<const float4*>(src[j]));
+                }
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) if (ok[j]) add4(a, f[j]);
+            for (int j = 0; j < kSlots; ++j) {
+                if (n[j] == 0) continue;
+                if (n[j] > 0) {
+                    add4(f[j], f2[j]);
+                    for (int c = 2; c < n[j]; ++c) add4(f[j], __ldcg(reinterpret_cast<const float4*>(src[j] + (2 * c - 1) * step)));
+                    f[j] = make_float4(f[j].x * w[j], f[j].y * w[j], f[j].z * w[j], f[j].w * w[j]);
+                }
+                add4(a, f[j]);
+            }
         }
         *reinterpret_cast<uint2*>(p.y + static_cast<int64_t>(t) * p.hidden + col) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
     }
@@ -509,58 +538,85 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
     }
     pdl_wait();                                          // routes, cast x and zeroed counters of the first launch
 
-    // ---- the plan, by every CTA for itself: routes sorted by expert (stable), blocks of up to 128 routes
+    // ---- the plan, by every CTA for itself: routes sorted by expert (stable), blocks of up to 128 routes.  Each warp counts and later
+    // places a run of the routes; between the two the counts become places, by warp for each expert and by expert.
     const int routes = p.tokens * p.topk;
     {
-        int* s_off = reinterpret_cast<int*>(smem);                   // the operand ring is not in use yet
-        uint16_t* s_id = reinterpret_cast<uint16_t*>(smem + (MM_MAX_EXPERTS + 32) * 4);
-        for (int e = threadIdx.x; e < p.experts; e += blockDim.x) s_off[e] = 0;
+        constexpr int kWarps = kMoeThreads / 32;
+        uint32_t* s_first = reinterpret_cast<uint32_t*>(smem);       // [experts]; the operand ring is not in use yet
+        uint16_t* s_id = reinterpret_cast<uint16_t*>(s_first + MM_MAX_EXPERTS);
+        uint16_t* s_hist = s_id + kMoeMaxRoutes;                     // [warps][experts, even]
+        const int pitch = (p.experts + 1) & ~1;
+        static_assert(MM_MAX_EXPERTS * 4 + kMoeMaxRoutes * 2 + kWarps * MM_MAX_EXPERTS * 2 <= kMoeRingBytes, "the plan");
+        uint16_t* hist = s_hist + warp * pitch;
+        const int run = (routes + 32 * kWarps - 1) / (32 * kWarps) * 32, run0 = warp * run, run1 = min(routes, run0 + run);
+        for (int e = lane * 2; e < pitch; e += 64) *reinterpret_cast<uint32_t*>(hist + e) = 0;
+        __syncwarp();
+        for (int r0 = run0; r0 < run1; r0 += 32) {
+            const int r = r0 + lane;
+            const int e = r < run1 ? p.route_expert[r] : -1;
+            const uint32_t same = __match_any_sync(0xffffffffu, e);
+            const uint32_t valid = __ballot_sync(0xffffffffu, e >= 0);
+            if (r < run1) s_id[r] = static_cast<uint16_t>(e);        // -1: 0xffff
+            if (e >= 0 && (same >> lane) == 1u) hist[e] += __popc(same);                 // the group's last lane
+            if (lane == 0) sm.valid[r0 / 32] = valid;
+            __syncwarp();
+        }
         __syncthreads();
-        for (int r = threadIdx.x; r < routes; r += blockDim.x) {
-            const int e = p.route_expert[r];
-            s_id[r] = static_cast<uint16_t>(e < 0 ? 0xffff : e);
-            if (e >= 0) atomicAdd(&s_off[e], 1);
+        for (int e = threadIdx.x; e < p.experts; e += kMoeThreads) {
+            uint32_t n = 0;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const uint32_t c = s_hist[w * pitch + e];
+                s_hist[w * pitch + e] = static_cast<uint16_t>(n);
+                n += c;
+            }
+            s_first[e] = n;
         }
         __syncthreads();
         if (warp == 0) {
-            int off = 0, blocks = 0, most = 0;
-            for (int e0 = 0; e0 < p.experts; e0 += 32) {             // counts -> first places, and the blocks of each expert
-                const int e = e0 + lane;
-                const int n = e < p.experts ? s_off[e] : 0;
-                const int b = (n + 127) >> 7;
-                int n_scan = n, b_scan = b;
+            // counts -> first places, and the blocks of each expert; a lane takes neighbouring experts
+            const int per = (p.experts + 31) / 32, e0 = lane * per, e1 = min(p.experts, e0 + per);
+            uint32_t n_own = 0, b_own = 0, most = 0;
+            for (int e = e0; e < e1; ++e) {
+                const uint32_t n = s_first[e];
+                n_own += n; b_own += (n + 127) >> 7; most = max(most, n);
+            }
+            uint32_t n_scan = n_own, b_scan = b_own;
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int a = __shfl_up_sync(0xffffffffu, n_scan, o), c = __shfl_up_sync(0xffffffffu, b_scan, o);
-                    if (lane >= o) { n_scan += a; b_scan += c; }
-                }
-                const int first = off + n_scan - n;
-                most = max(most, n);
-                for (int i = 0; i < b; ++i)
-                    sm.block[blocks + b_scan - b + i] = make_uint2(static_cast<uint32_t>(e) | static_cast<uint32_t>(min(128, n - 128 * i)) << 16, first + 128 * i);
-                if (e < p.experts) s_off[e] = first;
-                off += __shfl_sync(0xffffffffu, n_scan, 31);
-                blocks += __shfl_sync(0xffffffffu, b_scan, 31);
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t a = __shfl_up_sync(0xffffffffu, n_scan, o), c = __shfl_up_sync(0xffffffffu, b_scan, o);
+                if (lane >= o) { n_scan += a; b_scan += c; }
+            }
+            const int blocks = static_cast<int>(__shfl_sync(0xffffffffu, b_scan, 31));
+            uint32_t at = n_scan - n_own, b = b_scan - b_own;
+            for (int e = e0; e < e1; ++e) {
+                const uint32_t n = s_first[e];
+                s_first[e] = at;
+                for (uint32_t i = 0; i < n; i += 128) sm.block[b++] = make_uint2(static_cast<uint32_t>(e) | min(128u, n - i) << 16, at + i);
+                at += n;
             }
             most = __reduce_max_sync(0xffffffffu, most);
             if (lane == 0) {
                 sm.words->blocks = blocks;
-                sm.words->most = most;
+                sm.words->most = static_cast<int>(most);
                 sm.words->list[0] = moe_list(blocks * (p.inter / 128), p.hidden / 128, gridDim.x);
                 sm.words->list[1] = moe_list(blocks * ((p.hidden + 255) / 256), p.inter / 128, gridDim.x);
             }
-            __syncwarp();
-            for (int r0 = 0; r0 < routes; r0 += 32) {                // place every route, 32 at a time
-                const int r = r0 + lane;
-                const uint32_t e = r < routes ? s_id[r] : 0xffffu;
-                const uint32_t same = __match_any_sync(0xffffffffu, e);
-                if (e != 0xffffu) sm.route[s_off[e] + __popc(same & ((1u << lane) - 1u))] = static_cast<uint16_t>(r);
-                const uint32_t valid = __ballot_sync(0xffffffffu, e != 0xffffu);
-                if (lane == 0) sm.valid[r0 / 32] = valid;
-                __syncwarp();
-                if (e != 0xffffu && (same >> lane) == 1u) s_off[e] += __popc(same);      // the group's last lane
-                __syncwarp();
+        }
+        __syncthreads();
+        for (int r0 = run0; r0 < run1; r0 += 32) {
+            const int r = r0 + lane;
+            const uint32_t e = r < run1 ? s_id[r] : 0xffffu;
+            const uint32_t same = __match_any_sync(0xffffffffu, e);
+            uint32_t before = 0;
+            if (e != 0xffffu) {
+                before = hist[e];
+                sm.route[s_first[e] + before + __popc(same & ((1u << lane) - 1u))] = static_cast<uint16_t>(r);
             }
+            __syncwarp();
+            if (e != 0xffffu && (same >> lane) == 1u) hist[e] = static_cast<uint16_t>(before + __popc(same));
+            __syncwarp();
         }
         fence_proxy_async_smem();                                    // these words become TMA destinations
     }
@@ -791,7 +847,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
             const MoeSegment* g = segment_at(at);
             if (g == nullptr) break;
             if (g->kind < 0) {
-                if (n_blocks > 0) moe_combine(p, sm, n_blocks * nt2, sync_phase);
+                if (n_blocks > 0) moe_combine(p, sm, smem, n_blocks * nt2 * kb2, sync_phase);
                 break;
             }
             if (!mbar_wait_asleep(sm.turn_full(buffer), buffer_phase, abort_flag, p.timeout_ns)) break;
