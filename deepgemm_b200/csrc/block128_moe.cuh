@@ -460,49 +460,64 @@ __device__ __forceinline__ void moe_combine(const MoeParams& p, const MoeSmem& s
     if (!__all_sync(0xffffffffu, ok)) return;
     if (lane == 0) mbar_arrive(sm.finish_bar());
     if (!mbar_wait_often(sm.finish_bar(), phase, smem_u32(&sm.words->abort), p.timeout_ns)) return;
-    const int cols4 = p.hidden / 4;
-    for (int i = blockIdx.x * 128 + tid; i < p.tokens * cols4; i += gridDim.x * 128) {
-        const int t = i / cols4, col = (i - t * cols4) * 4;
-        const int r0 = t * p.topk;
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        constexpr int kSlots = 8;
-        for (int s = 0; s < p.topk; s += kSlots) {
-            float4 f[kSlots], f2[kSlots];
-            float w[kSlots];
-            int n[kSlots];                                           // parts, 0: no route, -1: a row that is whole
-            const float* src[kSlots];
+    // A warp takes 64 columns of a token: `group` slots side by side, 32 / group lanes to each, then a sum over the slots in a fixed order.
+    // (Eight slots one after the other in each thread, unrolled, were code that every SM ran once: fetching it took 4 us.)
+    int group = 1;
+    while (group < 8 && group < p.topk) group *= 2;
+    const int lanes = 32 / group, my_slot = lane / lanes, my_col = lane % lanes * 4;
+    const int strips = p.hidden / 64;
+#pragma unroll 1
+    for (int i = (tid >> 5) * gridDim.x + blockIdx.x; i < p.tokens * strips; i += gridDim.x * 4) {
+        const int t = i / strips, col0 = (i - t * strips) * 64;
+#pragma unroll 1
+        for (int c0 = 0; c0 < 64; c0 += lanes * 16) {                // up to four runs of four columns a lane; with one slot half the lanes have none
+            const int c = c0 + my_col, col = col0 + c;
+            float4 a[4];
 #pragma unroll
-            for (int j = 0; j < kSlots; ++j) {
-                const int r = r0 + s + j;
-                n[j] = 0;
-                if (s + j < p.topk && ((sm.valid[r >> 5] >> (r & 31)) & 1u)) {
-                    n[j] = -1;
-                    src[j] = p.rows_out + static_cast<int64_t>(r) * p.hidden + col;
-                    if (cut) {
-                        const uint32_t at = place[r];
-                        const uint32_t parts = parts_of[(at & 0xffff) + (col >> 8)];
-                        if (parts >> 16) {
-                            n[j] = static_cast<int>(parts >> 16);
-                            src[j] = parts2 + (parts & 0xffff) * step + (at >> 16) * 256 + (col & 255);
-                            w[j] = p.route_w[r];
-                            f2[j] = __ldcg(reinterpret_cast<const float4*>(src[j] + step));
-                        }
+            for (int j = 0; j < 4; ++j) a[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+            for (int s = my_slot; s < p.topk; s += group) {
+                const int r = t * p.topk + s;
+                if (c >= 64 || !((sm.valid[r >> 5] >> (r & 31)) & 1u)) continue;
+                const float* src = p.rows_out + static_cast<int64_t>(r) * p.hidden + col;
+                float w = 1.0f;
+                int n = 1;                                           // parts
+                if (cut) {
+                    const uint32_t at = place[r], parts = parts_of[(at & 0xffff) + (col >> 8)];
+                    if (parts >> 16) {
+                        n = static_cast<int>(parts >> 16);
+                        src = parts2 + (parts & 0xffff) * step + (at >> 16) * 256 + (col & 255);
+                        w = p.route_w[r];
                     }
-                    f[j] = __ldcg(reinterpret_cast<const float4*>(src[j]));
                 }
-            }
+                float4 f[2][4];
 #pragma unroll
-            for (int j = 0; j < kSlots; ++j) {
-                if (n[j] == 0) continue;
-                if (n[j] > 0) {
-                    add4(f[j], f2[j]);
-                    for (int c = 2; c < n[j]; ++c) add4(f[j], __ldcg(reinterpret_cast<const float4*>(src[j] + (2 * c - 1) * step)));
-                    f[j] = make_float4(f[j].x * w[j], f[j].y * w[j], f[j].z * w[j], f[j].w * w[j]);
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        f[k][j] = k < n && c + j * lanes * 4 < 64 ? __ldcg(reinterpret_cast<const float4*>(src + k * step + j * lanes * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) add4(f[0][j], f[1][j]);
+#pragma unroll 1
+                for (int k = 2; k < n; ++k)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (c + j * lanes * 4 < 64) add4(f[0][j], __ldcg(reinterpret_cast<const float4*>(src + (2 * k - 1) * step + j * lanes * 4)));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { a[j].x = fmaf(f[0][j].x, w, a[j].x); a[j].y = fmaf(f[0][j].y, w, a[j].y); a[j].z = fmaf(f[0][j].z, w, a[j].z); a[j].w = fmaf(f[0][j].w, w, a[j].w); }
+            }
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+#pragma unroll 1
+                for (int o = lanes; o < 32; o *= 2) {
+                    a[j].x += __shfl_xor_sync(0xffffffffu, a[j].x, o); a[j].y += __shfl_xor_sync(0xffffffffu, a[j].y, o);
+                    a[j].z += __shfl_xor_sync(0xffffffffu, a[j].z, o); a[j].w += __shfl_xor_sync(0xffffffffu, a[j].w, o);
                 }
-                add4(a, f[j]);
+                if (my_slot == 0 && c + j * lanes * 4 < 64)
+                    *reinterpret_cast<uint2*>(p.y + static_cast<int64_t>(t) * p.hidden + col + j * lanes * 4) = make_uint2(pack_bf16x2(a[j].x, a[j].y), pack_bf16x2(a[j].z, a[j].w));
             }
         }
-        *reinterpret_cast<uint2*>(p.y + static_cast<int64_t>(t) * p.hidden + col) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
     }
 }
 
@@ -536,11 +551,10 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
         tmem_alloc(smem_u32(&sm.words->tmem), 512);
         tmem_relinquish();
     }
-    pdl_wait();                                          // routes, cast x and zeroed counters of the first launch
-
     // ---- the plan, by every CTA for itself: routes sorted by expert (stable), blocks of up to 128 routes.  Each warp counts and later
     // places a run of the routes; between the two the counts become places, by warp for each expert and by expert.
     const int routes = p.tokens * p.topk;
+    int first_claim = 0;                                             // its answer is not needed before the plan
     {
         constexpr int kWarps = kMoeThreads / 32;
         uint32_t* s_first = reinterpret_cast<uint32_t*>(smem);       // [experts]; the operand ring is not in use yet
@@ -550,8 +564,12 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
         static_assert(MM_MAX_EXPERTS * 4 + kMoeMaxRoutes * 2 + kWarps * MM_MAX_EXPERTS * 2 <= kMoeRingBytes, "the plan");
         uint16_t* hist = s_hist + warp * pitch;
         const int run = (routes + 32 * kWarps - 1) / (32 * kWarps) * 32, run0 = warp * run, run1 = min(routes, run0 + run);
-        for (int e = lane * 2; e < pitch; e += 64) *reinterpret_cast<uint32_t*>(hist + e) = 0;
+        const int runs = (routes + run - 1) / run;                   // warps that have one
+        if (warp < runs)
+            for (int e = lane * 2; e < pitch; e += 64) *reinterpret_cast<uint32_t*>(hist + e) = 0;
         __syncwarp();
+        pdl_wait();                                                  // routes, cast x and zeroed counters of the first launch
+        if (threadIdx.x == 0) first_claim = atomicAdd(p.counters, 1);
         for (int r0 = run0; r0 < run1; r0 += 32) {
             const int r = r0 + lane;
             const int e = r < run1 ? p.route_expert[r] : -1;
@@ -565,8 +583,8 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
         __syncthreads();
         for (int e = threadIdx.x; e < p.experts; e += kMoeThreads) {
             uint32_t n = 0;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
+#pragma unroll 4
+            for (int w = 0; w < runs; ++w) {
                 const uint32_t c = s_hist[w * pitch + e];
                 s_hist[w * pitch + e] = static_cast<uint16_t>(n);
                 n += c;
@@ -650,7 +668,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
             if (lane == 0) {
                 int stage = 0; uint32_t phase = 0;
                 Place at;
-                bool alive = true;
+                bool alive = true, first = true;
                 auto publish = [&](const MoeSegment& g) {
                     if (!mbar_wait_often(sempty_bar(at.slot), at.phase ^ 1u, abort_flag, p.timeout_ns)) return false;
                     sm.words->segment[at.slot] = g;
@@ -661,7 +679,8 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                 while (alive) {
                     // Not before the copies of the last chunk are under way: whoever claims ahead takes a second share while others have
                     // none.  The ring holds more work than the claim takes.
-                    const int id = chunks > 0 ? atomicAdd(p.counters, 1) : 0;
+                    const int id = first ? first_claim : atomicAdd(p.counters, 1);
+                    first = false;
                     if (id >= chunks) break;
                     MoeSegment g;
                     g.kind = id >= chunks1 ? 1 : 0;
@@ -783,6 +802,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                     const float* sb = kind ? p.s2 + (static_cast<int64_t>(g.expert) * kb1 + n_block) * kb2
                                            : p.s1 + (static_cast<int64_t>(g.expert) * 2 * nt1 + n_block) * kb1;
                     if (kind && rb >= ready_blocks) {
+                        if (l64 >= 62) asm volatile("prefetch.global.L2 [%0];" ::"l"(sb + g.k0));        // (a line, 32 k blocks, of what comes from HBM)
                         // The rows this product reads.  One warp asks for both, and if it has to wait, everything filled so far is handed
                         // over first, because the tiles that finish those rows may be this CTA's own.
                         if (warp == 2) {
