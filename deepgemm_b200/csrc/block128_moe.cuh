@@ -13,7 +13,8 @@
 // chunks that CTAs claim from one counter.  While tiles are few (under 16 per SM), a chunk is an equal share of the whole list, cut
 // wherever the share ends, and the parts of a tile meet in memory: whoever brings the last part adds them up in order.  Else a chunk is
 // a tile.  Weights need nothing but the routes, so the TMA warp runs ahead into the second product, up to the depth of its ring, while the
-// activations of the first are still being finished; only the token operand waits for them.
+// activations of the first are still being finished; only the token operand waits for them.  (Prefetching more of them to L2 meanwhile took
+// bandwidth from CTAs that were still at the first product: 8 blocks for each CTA made 48 us of T = 1 into 51, 24 made 87 us of T = 33 into 93.)
 //
 // A chunk of the second product is claimed only after every chunk of the first one has been, and by a CTA that runs; so what a CTA waits
 // for is always being worked on, however many of the CTAs are resident, and two such launches may share a GPU.
@@ -213,10 +214,6 @@ struct MoeSmem {
     __device__ __forceinline__ uint32_t turn_empty(int b) const { return bars + 8u * (kBars - 3 + b); }
     __device__ __forceinline__ uint32_t finish_bar() const { return bars + 8u * (kBars - 1); }
 };
-
-__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int32_t c0, int32_t c1) {
-    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1) : "memory");
-}
 
 // silu(gate) * up of one row's block of 128, four columns a lane, and its cast
 __device__ __forceinline__ void moe_finish_row(const MoeParams& p, float4 g4, float4 u4, bool do_clamp, int64_t place, int nt, int lane) {
@@ -690,15 +687,6 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                     const int per_block = g.kind ? nt2 : nt1;        // tiles go block by block: the second product begins with what was finished first
                     int u = l.start(g.chunk);
                     const int end = l.start(g.chunk + 1);
-                    if (g.kind && p.tiled && l.shares) {
-                        // HBM has nothing to do until the activations of the first product are finished: what of this share the ring
-                        // does not hold goes to L2 meanwhile
-                        for (int v = u + stages; v < min(end, u + stages + 8); ++v) {
-                            const int tile = v / l.kb, rb = tile / nt2;
-                            const int64_t to = (static_cast<int64_t>(sm.block[rb].x & 0xffff) * nt2 + tile - rb * nt2) * l.kb + v - tile * l.kb;
-                            tma_prefetch_2d(map, 0, static_cast<int32_t>(to * 256));
-                        }
-                    }
                     while (u < end && alive) {
                         g.tile = u / l.kb;
                         g.k0 = u - g.tile * l.kb;

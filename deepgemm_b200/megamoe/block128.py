@@ -396,14 +396,15 @@ def norm_gate_residual(y: Optional[torch.Tensor], residual: torch.Tensor, *, pos
             post_ptr = post_weight.data_ptr()
         if gate is not None:
             gate_kind = _type_of(name, gate)
-            if gate.dim() == 1:
-                gate = gate.unsqueeze(0)
-            if gate.dim() != 2 or gate.shape[0] not in (1, t) or gate.shape[1] not in (1, h):
+            shape = gate.shape
+            if gate.dim() == 1 and shape[0] == h:                    # (as it is: a view would take a microsecond)
+                gate, gate_cols = _dense(gate, 16), 1
+            elif gate.dim() == 2 and shape[0] in (1, t) and shape[1] in (1, h):
+                if shape[1] == h:
+                    gate, gate_cols = _rows_of(gate, 16), 1
+                gate_rows = gate.stride(0) if shape[0] == t and t > 1 else 0
+            elif gate.dim() != 1 or shape[0] != 1:                   # [1]: one number for all
                 raise ValueError(f"{name}: gate must be [{h}], [{t}, 1] or [{t}, {h}]")
-            if gate.shape[1] == h:
-                gate = _rows_of(gate, 16)
-                gate_cols = 1
-            gate_rows = gate.stride(0) if gate.shape[0] == t and t > 1 else 0
             gate_ptr = gate.data_ptr()
     normed = codes = scales = None
     if pre_weight is not None:
