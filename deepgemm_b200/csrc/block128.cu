@@ -61,8 +61,22 @@ typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void
 struct Device {
     bool ready = false;
     int sms = 0;
+    int clusters[4] = {0, 0, 0, 0};      // of 1, 2, 4 and 8 CTAs of the split product that are resident at once
     int* status = nullptr;
 };
+
+// Launch of the split product: `tiles` clusters of `split` CTAs
+void split_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, int64_t tiles, int split, cudaStream_t st) {
+    memset(cfg, 0, sizeof(*cfg));
+    cfg->gridDim = dim3((unsigned)(tiles * split));
+    cfg->blockDim = dim3(mm::kB128Threads);
+    cfg->dynamicSmemBytes = mm::B128Shape<128>::kSmemBytes;
+    cfg->stream = st;
+    attr->id = cudaLaunchAttributeClusterDimension;
+    attr->val.clusterDim.x = (unsigned)split; attr->val.clusterDim.y = 1; attr->val.clusterDim.z = 1;
+    cfg->attrs = attr;
+    cfg->numAttrs = 1;
+}
 
 int device_of(Device** out) {
     static Device devices[kMaxDevices];
@@ -81,6 +95,13 @@ int device_of(Device** out) {
         B_CUDA(cudaFuncSetAttribute(mm::block128_gemm_kernel<128, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, mm::B128Shape<128>::kSmemBytes));
         B_CUDA(cudaFuncSetAttribute(mm::block128_gemm_kernel<128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, mm::B128Shape<128>::kSmemBytes));
         B_CUDA(cudaFuncSetAttribute(mm::moe_experts_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, mm::kMoeSmemBytes));
+        d.clusters[0] = d.sms;
+        for (int i = 1; i < 4; ++i) {
+            cudaLaunchConfig_t cfg;
+            cudaLaunchAttribute attr;
+            split_config(&cfg, &attr, d.sms, 1 << i, nullptr);
+            B_CUDA(cudaOccupancyMaxActiveClusters(&d.clusters[i], mm::block128_gemm_kernel<128, true>, &cfg));
+        }
         d.ready = true;
     }
     *out = &d;
@@ -281,15 +302,19 @@ int mm_fp8_gemm_block128(const void* a, int64_t a_stride, const float* sa, int64
     p.timeout_ns = mm_detail_pipe_timeout_ns();
     p.m_tiles = (m + 127) / 128;
     p.a_box_rows = m >= 128 ? 128 : (m + 7) / 8 * 8;
-    // Tile width and split of K: 256 columns when that fills the SMs, else 128 columns, and as long as that leaves SMs
-    // idle the k blocks of a tile are divided among up to eight CTAs.
+    // Tile width and split of K.  A turn of the SMs with tiles of 128 columns takes 0.7 of the time of one with 256 (1024 x 4096 x 4096: 29 us in
+    // two turns of 128, 21 in one of 256), so 128 is taken where that makes less.  The k blocks of a tile are then divided among up to
+    // eight CTAs, as long as all clusters are resident at once (1 x 4096 x 4096: 8.2 us with four CTAs to a tile, 11.0 with two, 15.0 with
+    // one) and each CTA keeps a few blocks.
     const int64_t tiles256 = (int64_t)p.m_tiles * ((n + 255) / 256), tiles128 = (int64_t)p.m_tiles * n_sf;
-    const int bn = tiles256 >= d->sms ? 256 : 128;
+    const int64_t turns256 = (tiles256 + d->sms - 1) / d->sms, turns128 = (tiles128 + d->sms - 1) / d->sms;
+    const int bn = turns128 * 7 < turns256 * 10 ? 128 : 256;
     const int64_t tiles = bn == 256 ? tiles256 : tiles128;
     B_REQUIRE(tiles < kMaxDim, "mm_fp8_gemm_block128: too many tiles");
     p.n_tiles = bn == 256 ? (n + 255) / 256 : n_sf;
-    int split = 1;
-    while (bn == 128 && !m_indices && split < 8 && tiles * split * 2 <= d->sms && kb >= split * 4) split *= 2;
+    int log_split = 0;
+    while (bn == 128 && !m_indices && log_split < 3 && tiles <= d->clusters[log_split + 1] && kb >= (4 << log_split)) ++log_split;
+    const int split = 1 << log_split;
     CUtensorMap tm_a, tm_b;
     if (int rc = byte_map(a, (uint64_t)k, (uint64_t)m, (uint64_t)a_stride, 0, 0, (uint32_t)p.a_box_rows, &tm_a)) return rc;
     if (p.tiled) {
@@ -300,16 +325,8 @@ int mm_fp8_gemm_block128(const void* a, int64_t a_stride, const float* sa, int64
     cudaStream_t st = static_cast<cudaStream_t>(stream_);
     if (split > 1) {
         cudaLaunchConfig_t cfg;
-        memset(&cfg, 0, sizeof(cfg));
-        cfg.gridDim = dim3((unsigned)(tiles * split));
-        cfg.blockDim = dim3(mm::kB128Threads);
-        cfg.dynamicSmemBytes = mm::B128Shape<128>::kSmemBytes;
-        cfg.stream = st;
         cudaLaunchAttribute attr;
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = (unsigned)split; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
+        split_config(&cfg, &attr, tiles, split, st);
         B_CUDA(cudaLaunchKernelEx(&cfg, mm::block128_gemm_kernel<128, true>, tm_a, tm_b, p));
     } else {
         const unsigned grid = (unsigned)(tiles < d->sms ? tiles : d->sms);
