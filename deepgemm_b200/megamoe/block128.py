@@ -58,17 +58,24 @@ def _device_index(name: str, *tensors: Optional[torch.Tensor]) -> int:
     return index
 
 
-def _rows_of(t: torch.Tensor, align: int) -> torch.Tensor:
-    """`t` [rows, k] as it is if its rows are dense and start on `align`-byte boundaries, else a contiguous copy."""
+def _rows_of(t: torch.Tensor, align: int) -> Tuple[torch.Tensor, int]:
+    """`t` [rows, k] as it is if its rows are dense and start on `align`-byte boundaries, else a contiguous copy; and the elements from
+    a row to the next (the stride of a single row says nothing)."""
+    rows, k = t.shape
     pitch, step = t.stride()
-    if step == 1 and t.data_ptr() % align == 0 and (t.shape[0] <= 1 or (pitch >= t.shape[1] and (pitch * t.element_size()) % align == 0)):
-        return t
+    if rows <= 1:
+        pitch = k
+    if step == 1 and pitch >= k and t.data_ptr() % align == 0 and (pitch * t.element_size()) % align == 0:
+        return t, pitch
+    return _dense(t, align), k
+
+
+def _dense(t: torch.Tensor, align: int) -> torch.Tensor:
     t = t.contiguous()
-    return t if t.data_ptr() % align == 0 and (t.shape[0] <= 1 or (t.stride(0) * t.element_size()) % align == 0) else t.clone()
+    return t if t.data_ptr() % align == 0 else t.clone()
 
 
 def _pitch(t: torch.Tensor) -> int:
-    """Elements from a row to the next; the stride of a single row says nothing."""
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
@@ -91,8 +98,7 @@ def cast_to_fp8_block128(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     if rows:
         stride = k
         if not x.is_contiguous() or x.data_ptr() % 16 != 0:
-            x = _rows_of(x if x.dim() == 2 else x.reshape(-1, k), 16)
-            stride = _pitch(x)
+            x, stride = _rows_of(x if x.dim() == 2 else x.reshape(-1, k), 16)
         _call(index, _lib.lib().mm_cast_block128, x.data_ptr(), kind, rows, k, stride, q.data_ptr(), sf.data_ptr())
     return q, sf
 
@@ -134,11 +140,6 @@ def _scale_rows(sf: torch.Tensor) -> torch.Tensor:
     return sf if sf.is_contiguous() or (sf.stride(1) == 1 and sf.stride(0) >= sf.shape[1]) else sf.contiguous()
 
 
-def _dense(t: torch.Tensor, align: int) -> torch.Tensor:
-    t = t.contiguous()
-    return t if t.data_ptr() % align == 0 else t.clone()
-
-
 def fp8_gemm_nt_block128(a: Tuple[torch.Tensor, torch.Tensor], b: Tuple[torch.Tensor, torch.Tensor], out: Optional[torch.Tensor] = None,
                          out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """out[M, N] = a [M, K] . b [N, K]^T with a = (e4m3, scales [M, ceil(K/128)]), b = (e4m3, scales [ceil(N/128), ceil(K/128)]).
@@ -164,8 +165,8 @@ def fp8_gemm_nt_block128(a: Tuple[torch.Tensor, torch.Tensor], b: Tuple[torch.Te
         raise RuntimeError(f"{name}: the output is bfloat16 or float32")
     if m == 0 or n == 0:
         return out
-    a_q, b_q, a_sf, b_sf = _rows_of(a_q, 16), _dense(b_q, 16), _scale_rows(a_sf), b_sf.contiguous()
-    _call(index, _lib.lib().mm_fp8_gemm_block128, a_q.data_ptr(), _pitch(a_q), a_sf.data_ptr(), _pitch(a_sf), b_q.data_ptr(),
+    (a_q, a_pitch), b_q, a_sf, b_sf = _rows_of(a_q, 16), _dense(b_q, 16), _scale_rows(a_sf), b_sf.contiguous()
+    _call(index, _lib.lib().mm_fp8_gemm_block128, a_q.data_ptr(), a_pitch, a_sf.data_ptr(), _pitch(a_sf), b_q.data_ptr(),
           b_sf.data_ptr(), 1, 0, None, out.data_ptr(), pitch, out.dtype == torch.float32, m, n, k)
     return out
 
@@ -200,8 +201,8 @@ def m_grouped_fp8_gemm_nt_contiguous_block128(a: Tuple[torch.Tensor, torch.Tenso
     if rows and n and w.shape[0] == 0:
         raise RuntimeError(f"{name}: no experts")
     if rows and n:
-        a_q, w, a_sf, w_sf, m_indices = _rows_of(a_q, 16), _dense(w, 16), _scale_rows(a_sf), w_sf.contiguous(), m_indices.contiguous()
-        _call(index, _lib.lib().mm_fp8_gemm_block128, a_q.data_ptr(), _pitch(a_q), a_sf.data_ptr(), _pitch(a_sf), w.data_ptr(),
+        (a_q, a_pitch), w, a_sf, w_sf, m_indices = _rows_of(a_q, 16), _dense(w, 16), _scale_rows(a_sf), w_sf.contiguous(), m_indices.contiguous()
+        _call(index, _lib.lib().mm_fp8_gemm_block128, a_q.data_ptr(), a_pitch, a_sf.data_ptr(), _pitch(a_sf), w.data_ptr(),
               w_sf.data_ptr(), w.shape[0], tiled, m_indices.data_ptr(), d.data_ptr(), n, d.dtype == torch.float32, rows, n, k)
     if check:
         check_block128_status(index)
@@ -306,8 +307,7 @@ def fp8_moe_few_tokens(x, l1_weights: Tuple[torch.Tensor, torch.Tensor], l2_weig
     if t == 0:
         return out
     if x_sf is None:
-        x = _rows_of(x, 32)              # 16 values
-        stride = _pitch(x)
+        x, stride = _rows_of(x, 32)      # 16 values
     else:
         x, x_sf, stride = x.contiguous(), x_sf.contiguous(), h
         if x.data_ptr() % 16 != 0:
@@ -383,12 +383,12 @@ def norm_gate_residual(y: Optional[torch.Tensor], residual: torch.Tensor, *, pos
     y_kind = gate_kind = post_kind = pre_kind = normed_kind = gate_rows = gate_cols = 0
     y_ptr = post_ptr = gate_ptr = pre_ptr = normed_ptr = codes_ptr = scales_ptr = new_ptr = None
     y_stride = h
-    r = _rows_of(residual, 16)
+    r, r_stride = _rows_of(residual, 16)
     residual_out = residual
     if y is not None:
         y_kind = _type_of(name, y)
-        y = _rows_of(y, 16)
-        y_ptr, y_stride = y.data_ptr(), _pitch(y)
+        y, y_stride = _rows_of(y, 16)
+        y_ptr = y.data_ptr()
         residual_out = torch.empty_like(residual, memory_format=torch.contiguous_format)
         new_ptr = residual_out.data_ptr()
         if post_weight is not None:
@@ -401,8 +401,11 @@ def norm_gate_residual(y: Optional[torch.Tensor], residual: torch.Tensor, *, pos
                 gate, gate_cols = _dense(gate, 16), 1
             elif gate.dim() == 2 and shape[0] in (1, t) and shape[1] in (1, h):
                 if shape[1] == h:
-                    gate, gate_cols = _rows_of(gate, 16), 1
-                gate_rows = gate.stride(0) if shape[0] == t and t > 1 else 0
+                    (gate, gate_rows), gate_cols = _rows_of(gate, 16), 1
+                else:
+                    gate_rows = gate.stride(0)
+                if shape[0] == 1:
+                    gate_rows = 0
             elif gate.dim() != 1 or shape[0] != 1:                   # [1]: one number for all
                 raise ValueError(f"{name}: gate must be [{h}], [{t}, 1] or [{t}, {h}]")
             gate_ptr = gate.data_ptr()
@@ -431,7 +434,7 @@ def norm_gate_residual(y: Optional[torch.Tensor], residual: torch.Tensor, *, pos
         if normed is None and codes is None:
             pre_ptr = None
     if t and (y is not None or pre_ptr is not None):
-        _call(index, _lib.lib().mm_norm_gate_residual, y_ptr, y_kind, y_stride, r.data_ptr(), r_kind, _pitch(r), post_ptr, post_kind, gate_ptr,
+        _call(index, _lib.lib().mm_norm_gate_residual, y_ptr, y_kind, y_stride, r.data_ptr(), r_kind, r_stride, post_ptr, post_kind, gate_ptr,
               gate_kind, gate_rows, gate_cols, pre_ptr, pre_kind, new_ptr, normed_ptr, normed_kind, codes_ptr, scales_ptr, quant_kind, t, h,
               residual_scale, eps, weight_offset)
     return NormOutputs(residual_out, normed, codes, scales)
