@@ -153,7 +153,7 @@ MoeWork moe_work(int T, int E, int K, int H, int I, bool cast, int ctas) {
     const int64_t nt1 = I / 128;
     w.ctr_done1 = 32;
     w.ctr_tile1 = w.ctr_done1 + (int)blocks;
-    w.num_counters = w.ctr_tile1 + (int)(blocks * nt1);
+    w.num_counters = w.ctr_tile1 + (int)(blocks * nt1 * 4);
     w.part_rows = (int)(routes < 128 ? routes : 128);
     w.counters = take((int64_t)w.num_counters * 4);
     w.route_expert = take(routes * 4);

@@ -41,7 +41,7 @@ constexpr int kMoePlanBytes = kMoeMaxRoutes * 2 + kMoeMaxBlocks * 8 + kMoeMaxRou
 constexpr int kMoeTurnRows = 6, kMoeTurnPitch = 260;    // fp32 rows that go from the summing to the finishing warps, in two buffers
 constexpr int kMoeThreads = 512;
 constexpr int kMoeSegments = 8;
-constexpr int kMoeCtrTiles1 = 8, kMoeCtrUnits2 = 16;
+constexpr int kMoeCtrRows1 = 8, kMoeCtrUnits2 = 16;
 constexpr int kMoeTailBytes = 768;        // barriers and MoeWords
 // Scales of a unit: 128 rows, then two of the weights.  As in block128_gemm.cuh: stages + accumulators + 1 units may be on their way.
 constexpr int kMoeScaleSlots = 8, kMoeScaleBytes = 544;
@@ -61,8 +61,9 @@ struct MoeParams {
     uint8_t* xq_out; float* xsf_out;
     int* route_expert; float* route_w;       // [tokens * topk], -1 = none
     int* counters; int num_counters;
-    // counters: [0] claims, [kMoeCtrTiles1] finished tiles of the first product, [ctr_done1 ..) the same by block of routes, [ctr_tile1 ..)
-    // k blocks that have arrived for each of its tiles that was cut, [kMoeCtrUnits2] k blocks of the second product whose sums are written
+    // counters: [0] claims, [kMoeCtrRows1] finished tiles of the first product (times the warps that finish their rows), [ctr_done1 ..) the
+    // same by block of routes, [ctr_tile1 ..) k blocks that have arrived for each of its tiles that was cut, by warp, [kMoeCtrUnits2] k
+    // blocks of the second product whose sums are written
     int ctr_done1, ctr_tile1;
     const float* s1; const float* s2;
     int tiled;
@@ -184,8 +185,7 @@ struct MoeSegment {
 struct MoeWords {
     int abort;
     uint32_t tmem;
-    volatile int last[2];                                // the boss's answer to the other finishing warps, one for each tile in turn
-    int blocks, most;                                    // blocks of routes, routes of the most popular expert
+    int blocks, most, finishers;                         // blocks of routes, routes of the most popular expert, sum of moe_finishers
     int ready;                                           // blocks of routes whose activations this CTA knows to be finished
     MoeList list[2];                                     // of either product
     MoeSegment segment[kMoeSegments];
@@ -325,26 +325,30 @@ __device__ __forceinline__ float* moe_part(const MoeParams& p, const MoeList& l,
     return p.parts + at * p.part_rows * 256;
 }
 
-// What the four finishing warps do with a tile, or a part of one, once its sums have been written down.  False if a wait has run out.
-__device__ __forceinline__ bool moe_finish_tile(const MoeParams& p, const MoeSmem& sm, const MoeSegment& g, int buffer, uint32_t& phase) {
-    const int kind = g.kind, tile = g.tile, rb = g.block, nt = g.out, units = g.k1 - g.k0;
+// Warps that finish rows of a tile: row r belongs to warp r % 4
+__device__ __forceinline__ int moe_finishers(int rows) { return min(4, rows); }
+
+// What a finishing warp does with a tile, or a part of one, once its sums have been written down (buffer `buffer` full in `phase`).  Each of
+// the four counts for itself and its own rows: counting for all of them took two barriers of the four in every tile.  False if a wait
+// has run out.
+__device__ __forceinline__ bool moe_finish_tile(const MoeParams& p, const MoeSmem& sm, const MoeSegment& g, int buffer, uint32_t phase) {
+    const int kind = g.kind, tile = g.tile, units = g.k1 - g.k0, rows = g.rows;
     const MoeList& l = sm.words->list[kind];
     const int fw = (threadIdx.x >> 5) - 4, lane = threadIdx.x & 31;
-    const bool boss = threadIdx.x == 128;
     const bool whole = units == l.kb;
-    const int rows = g.rows;
-    const bool turn = whole && rows <= kMoeTurnRows;
-    const float* my_turn = sm.turn + buffer * kMoeTurnRows * kMoeTurnPitch;
-    // Barrier of the four warps, bounded like every other wait: a warp that has given up does not hold the others.  What the warps
-    // wrote before it (and the summing warps before the buffer was full) is released to the GPU by the boss's count behind it, and
-    // what that count acquired they may read behind the next one (from L2: another SM has written it).
-    auto sync = [&]() {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(sm.finish_bar());
-        const bool ok = mbar_wait_often(sm.finish_bar(), phase, smem_u32(&sm.words->abort), p.timeout_ns);
-        phase ^= 1u;
-        return ok;
-    };
+    const bool mine = fw < moe_finishers(rows);
+    // where the sums are (the divisions while others still work)
+    const float* src = nullptr;
+    int n = 1;
+    if (kind == 0 && mine) {
+        int c0 = g.chunk;
+        if (!whole) {
+            c0 = l.chunk_of(tile * l.kb);
+            n = l.chunk_of(tile * l.kb + l.kb - 1) - c0 + 1;
+        }
+        src = moe_part(p, l, 0, c0, tile, whole, buffer);
+    }
+    if (!mbar_wait_asleep(sm.turn_full(buffer), phase, smem_u32(&sm.words->abort), p.timeout_ns)) return false;
     auto release = [&]() {                               // the buffer's values have been read
         __syncwarp();
         if (lane == 0) mbar_arrive(sm.turn_empty(buffer));
@@ -352,76 +356,63 @@ __device__ __forceinline__ bool moe_finish_tile(const MoeParams& p, const MoeSme
     if (kind) {
         // rows of a whole tile are in their place already, parts are added up by the combine
         release();
-        if (boss) {
+        if (fw == 0 && lane == 0) {
             __threadfence();
             atomicAdd(p.counters + kMoeCtrUnits2, units);
         }
         return true;
     }
-    int c0 = g.chunk, c1 = g.chunk;
+    if (!whole || !mine) release();                      // parts have memory of their own
+    if (!mine) return true;
     if (!whole) {
-        // the parts are added up by whoever brings the last one, in the order of the chunks
-        release();                                       // parts have memory of their own
-        if (boss) sm.words->last[buffer] = atomic_add_acq_rel(p.counters + p.ctr_tile1 + tile, units) + units == l.kb;
-        if (!sync()) return false;
-        if (sm.words->last[buffer] == 0) return true;    // (written again two tiles on, behind a barrier of the tile between)
-        c0 = l.chunk_of(tile * l.kb);
-        c1 = l.chunk_of(tile * l.kb + l.kb - 1);
+        // the parts are added up by whoever brings the last one, in the order of the chunks (read from L2: other SMs wrote them)
+        int have = 0;
+        if (lane == 0) have = atomic_add_acq_rel(p.counters + p.ctr_tile1 + tile * 4 + fw, units) + units;
+        if (__shfl_sync(0xffffffffu, have, 0) != l.kb) return true;
     }
-    // Four columns each of gate and up of two rows, the second one four behind: eight loads in
-    // flight, two parts at a time, added in order.  v[row][place].
-    auto join = [&](int row, float4 (&v)[2][2]) {
-        const int col_a = lane * 4, col_b = 128 + lane * 4;
-        const bool two = row + 4 < rows;
-        if (turn) {
-            const float* in = my_turn + row * kMoeTurnPitch;
-            v[0][0] = *reinterpret_cast<const float4*>(in + col_a);
-            v[0][1] = *reinterpret_cast<const float4*>(in + col_b);
-            if (two) {
-                v[1][0] = *reinterpret_cast<const float4*>(in + 4 * kMoeTurnPitch + col_a);
-                v[1][1] = *reinterpret_cast<const float4*>(in + 4 * kMoeTurnPitch + col_b);
-            }
-            return;
-        }
+    const bool turn = whole && rows <= kMoeTurnRows;
+    const float* my_turn = sm.turn + buffer * kMoeTurnRows * kMoeTurnPitch;
+    const int64_t step = static_cast<int64_t>(p.part_rows) * 256;        // from the first part to the second; two of these to each one after (moe_part)
+    const bool do_clamp = p.clamp < 3.0e38f;
+    // A row at a time, four columns each of gate and up in a lane (with one thread to a row, as the sums were held, a tile of few rows would
+    // keep eight warps waiting for the few threads that have any); two rows' loads and two parts' in flight.
+    for (int r = fw; r < rows; r += 8) {
+        const bool two = r + 4 < rows;
+        float4 v[2][2];                                  // [row][gate, up]
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i >> 1][i & 1] = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int ch = c0; ch <= c1; ch += 2) {
-            float4 f[2][2][2];
+        if (turn) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (ch + i > c1) continue;
-                const float* in = moe_part(p, l, 0, ch + i, tile, whole, buffer) + row * 256;
-                f[i][0][0] = __ldcg(reinterpret_cast<const float4*>(in + col_a));
-                f[i][0][1] = __ldcg(reinterpret_cast<const float4*>(in + col_b));
-                if (two) {
-                    f[i][1][0] = __ldcg(reinterpret_cast<const float4*>(in + 4 * 256 + col_a));
-                    f[i][1][1] = __ldcg(reinterpret_cast<const float4*>(in + 4 * 256 + col_b));
-                }
-            }
+            for (int i = 0; i < 4; ++i)
+                if (i < 2 || two) v[i >> 1][i & 1] = *reinterpret_cast<const float4*>(my_turn + (r + (i & 2) * 2) * kMoeTurnPitch + (i & 1) * 128 + lane * 4);
+        } else {
+            const float* in = src + r * 256 + lane * 4;
+#pragma unroll 1
+            for (int c = 0; c < n; c += 2) {
+                float4 f[2][4];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (ch + i > c1) continue;
-                add4(v[0][0], f[i][0][0]);
-                add4(v[0][1], f[i][0][1]);
-                if (two) { add4(v[1][0], f[i][1][0]); add4(v[1][1], f[i][1][1]); }
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (c + k < n && (i < 2 || two))
+                            f[k][i] = __ldcg(reinterpret_cast<const float4*>(in + (c + k == 0 ? 0 : 2 * (c + k) - 1) * step + (i & 2) * 512 + (i & 1) * 128));
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (c + k < n && (i < 2 || two)) add4(v[i >> 1][i & 1], f[k][i]);
             }
         }
-    };
-    // a row at a time for each warp: with one thread to a row, as the sums were held, a tile of few rows would keep eight warps
-    // waiting for the few threads that have any
-    const bool do_clamp = p.clamp < 3.0e38f;
-    for (int r = fw; r < rows; r += 8) {
-        float4 v[2][2];
-        join(r, v);
-        moe_finish_row(p, v[0][0], v[0][1], do_clamp, static_cast<int64_t>(g.first) + r, nt, lane);
-        if (r + 4 < rows) moe_finish_row(p, v[1][0], v[1][1], do_clamp, static_cast<int64_t>(g.first) + r + 4, nt, lane);
+#pragma unroll 1
+        for (int i = 0; i < (two ? 2 : 1); ++i)
+            moe_finish_row(p, i ? v[1][0] : v[0][0], i ? v[1][1] : v[0][1], do_clamp, static_cast<int64_t>(g.first) + r + 4 * i, g.out, lane);
     }
     if (whole) release();
-    if (!sync()) return false;
-    if (boss) {
+    __syncwarp();
+    if (lane == 0) {
         __threadfence();
-        atomicAdd(p.counters + p.ctr_done1 + rb, 1);
-        atomicAdd(p.counters + kMoeCtrTiles1, 1);
+        atomicAdd(p.counters + p.ctr_done1 + g.block, 1);
+        atomicAdd(p.counters + kMoeCtrRows1, 1);
     }
     return true;
 }
@@ -429,7 +420,7 @@ __device__ __forceinline__ bool moe_finish_tile(const MoeParams& p, const MoeSme
 // The combine, by the finishing warps of every CTA once the sums of all `units` of the second product are written: each token's rows, in the
 // order of its slots, four columns a thread.  A tile that was cut is read as its parts, in the order of the chunks: adding them up
 // first, by whoever brings the last one, and reading the sum then made the end of a call for one token 7 us long instead of 4.
-__device__ __forceinline__ void moe_combine(const MoeParams& p, const MoeSmem& sm, uint8_t* ring, int units, uint32_t phase) {
+__device__ __forceinline__ void moe_combine(const MoeParams& p, const MoeSmem& sm, uint8_t* ring, int units) {
     const int tid = threadIdx.x - 128, lane = threadIdx.x & 31;
     const MoeList& l = sm.words->list[1];
     const int nt2 = (p.hidden + 255) / 256;
@@ -456,7 +447,7 @@ __device__ __forceinline__ void moe_combine(const MoeParams& p, const MoeSmem& s
     const bool ok = tid != 0 || moe_wait_count(p.counters + kMoeCtrUnits2, units, smem_u32(&sm.words->abort), p.timeout_ns);
     if (!__all_sync(0xffffffffu, ok)) return;
     if (lane == 0) mbar_arrive(sm.finish_bar());
-    if (!mbar_wait_often(sm.finish_bar(), phase, smem_u32(&sm.words->abort), p.timeout_ns)) return;
+    if (!mbar_wait_often(sm.finish_bar(), 0, smem_u32(&sm.words->abort), p.timeout_ns)) return;
     // A warp takes 64 columns of a token: `group` slots side by side, 32 / group lanes to each, then a sum over the slots in a fixed order.
     // (Eight slots one after the other in each thread, unrolled, were code that every SM ran once: fetching it took 4 us.)
     int group = 1;
@@ -592,10 +583,11 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
         if (warp == 0) {
             // counts -> first places, and the blocks of each expert; a lane takes neighbouring experts
             const int per = (p.experts + 31) / 32, e0 = lane * per, e1 = min(p.experts, e0 + per);
-            uint32_t n_own = 0, b_own = 0, most = 0;
+            uint32_t n_own = 0, b_own = 0, most = 0, fin = 0;
             for (int e = e0; e < e1; ++e) {
                 const uint32_t n = s_first[e];
                 n_own += n; b_own += (n + 127) >> 7; most = max(most, n);
+                fin += 4 * (n >> 7) + min(4u, n & 127u);
             }
             uint32_t n_scan = n_own, b_scan = b_own;
 #pragma unroll
@@ -612,9 +604,11 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                 at += n;
             }
             most = __reduce_max_sync(0xffffffffu, most);
+            fin = __reduce_add_sync(0xffffffffu, fin);
             if (lane == 0) {
                 sm.words->blocks = blocks;
                 sm.words->most = static_cast<int>(most);
+                sm.words->finishers = static_cast<int>(fin);
                 sm.words->list[0] = moe_list(blocks * (p.inter / 128), p.hidden / 128, gridDim.x);
                 sm.words->list[1] = moe_list(blocks * ((p.hidden + 255) / 256), p.inter / 128, gridDim.x);
             }
@@ -795,14 +789,14 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                         // over first, because the tiles that finish those rows may be this CTA's own.
                         if (warp == 2) {
                             auto look = [&]() {                      // lane 0: all tiles of the first product, or at least this block's
-                                const int all = ld_acquire_gpu(p.counters + kMoeCtrTiles1), own = ld_acquire_gpu(p.counters + p.ctr_done1 + rb);
-                                return all >= n_blocks * nt1 ? n_blocks : own >= nt1 ? rb + 1 : 0;
+                                const int all = ld_acquire_gpu(p.counters + kMoeCtrRows1), own = ld_acquire_gpu(p.counters + p.ctr_done1 + rb);
+                                return all >= sm.words->finishers * nt1 ? n_blocks : own >= moe_finishers(rows) * nt1 ? rb + 1 : 0;
                             };
                             ready_blocks = __shfl_sync(0xffffffffu, lane == 0 ? look() : 0, 0);
                             if (ready_blocks == 0) {
                                 drain();
                                 int n = 0;
-                                if (lane == 0 && moe_wait_count(p.counters + p.ctr_done1 + rb, nt1, abort_flag, p.timeout_ns)) n = max(look(), rb + 1);
+                                if (lane == 0 && moe_wait_count(p.counters + p.ctr_done1 + rb, moe_finishers(rows) * nt1, abort_flag, p.timeout_ns)) n = max(look(), rb + 1);
                                 ready_blocks = __shfl_sync(0xffffffffu, n, 0);
                             }
                             if (ready_blocks == 0) { alive = false; break; }
@@ -849,17 +843,16 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                  i += static_cast<int64_t>(gridDim.x) * 128)
                 reinterpret_cast<uint4*>(p.y)[i] = make_uint4(0, 0, 0, 0);
         }
-        int buffer = 0; uint32_t buffer_phase = 0, sync_phase = 0;
+        int buffer = 0; uint32_t buffer_phase = 0;
         Place at;
         while (true) {
             const MoeSegment* g = segment_at(at);
             if (g == nullptr) break;
             if (g->kind < 0) {
-                if (n_blocks > 0) moe_combine(p, sm, smem, n_blocks * nt2 * kb2, sync_phase);
+                if (n_blocks > 0) moe_combine(p, sm, smem, n_blocks * nt2 * kb2);
                 break;
             }
-            if (!mbar_wait_asleep(sm.turn_full(buffer), buffer_phase, abort_flag, p.timeout_ns)) break;
-            if (!moe_finish_tile(p, sm, *g, buffer, sync_phase)) break;
+            if (!moe_finish_tile(p, sm, *g, buffer, buffer_phase)) break;
             __syncwarp();
             if (lane == 0) segment_done(at);
             step(at);
