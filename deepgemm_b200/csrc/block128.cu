@@ -177,6 +177,8 @@ int moe_check_shape(int T, int E, int K, int H, int I) {
     return 0;
 }
 
+// rows that are read 16 bytes at a time
+bool row_aligned(int64_t stride, int type) { return stride % (type == mm::B128_FP32 ? 4 : 8) == 0; }
 bool known_type(int t) { return t == mm::B128_BF16 || t == mm::B128_FP16 || t == mm::B128_FP32; }
 
 }  // namespace
@@ -185,7 +187,7 @@ extern "C" {
 
 int mm_cast_block128(const void* x, int type, int64_t rows, int k, int64_t row_stride, void* q, float* sf, void* stream_) {
     B_REQUIRE(known_type(type), "mm_cast_block128: unknown type");
-    B_REQUIRE(rows >= 0 && k > 0 && k % 8 == 0 && row_stride >= k && row_stride % 8 == 0, "mm_cast_block128: k and the row stride must be multiples of 8");
+    B_REQUIRE(rows >= 0 && k > 0 && k % 8 == 0 && row_stride >= k && row_aligned(row_stride, type), "mm_cast_block128: k must come in multiples of 8, the row stride in multiples of 16 bytes");
     if (rows == 0) return 0;
     B_REQUIRE(x && q && sf, "mm_cast_block128: null pointer");
     B_REQUIRE(aligned(x, 16) && aligned(q, 8) && aligned(sf, 4), "mm_cast_block128: x must be 16-byte, q 8-byte aligned");
@@ -240,8 +242,8 @@ int mm_norm_gate_residual(const void* y, int y_type, int64_t y_stride, const voi
     B_REQUIRE(r && (y ? r_out != nullptr : !post && !gate && !r_out), "mm_norm_gate_residual: null pointer (a norm or gate needs y, y needs a new residual)");
     B_REQUIRE(pre || (!x_out && quant == 0), "mm_norm_gate_residual: outputs of the second norm need its weight");
     B_REQUIRE(quant == 0 || (q && sf), "mm_norm_gate_residual: null pointer");
-    B_REQUIRE(r_stride >= hidden && (!y || y_stride >= hidden) && r_stride % 8 == 0 && y_stride % 8 == 0 && (gate_col_stride == 0 || gate_col_stride == 1) &&
-              gate_row_stride >= 0 && (gate_col_stride == 0 || gate_row_stride % 8 == 0), "mm_norm_gate_residual: bad strides");
+    B_REQUIRE(r_stride >= hidden && (!y || y_stride >= hidden) && row_aligned(r_stride, r_type) && row_aligned(y_stride, y_type) && (gate_col_stride == 0 || gate_col_stride == 1) &&
+              gate_row_stride >= 0 && (gate_col_stride == 0 || row_aligned(gate_row_stride, gate_type)), "mm_norm_gate_residual: bad strides");
     B_REQUIRE(aligned(y, 16) && aligned(r, 16) && aligned(post, 16) && aligned(pre, 16) && (gate_col_stride == 0 || aligned(gate, 16)) && aligned(r_out, 16) &&
               aligned(x_out, 16) && aligned(q, 8) && aligned(sf, 4), "mm_norm_gate_residual: pointers must be 16-byte aligned (codes 8)");
     Device* d;

@@ -142,7 +142,7 @@ int mm_set_tile_trace(void* device_words, int max_tiles, int cta);
  * type: 0 = bf16, 1 = fp16, 2 = fp32.  Row strides are in elements.  All calls are asynchronous on `stream`, allocate nothing and
  * may be captured into a CUDA graph. */
 
-/* Activations [rows, k] (k and row_stride multiples of 8): top = max(amax of 128 values, 1e-4), sf[rows][ceil(k/128)] = top / 448,
+/* Activations [rows, k] (k a multiple of 8, rows 16-byte aligned): top = max(amax of 128 values, 1e-4), sf[rows][ceil(k/128)] = top / 448,
  * q = e4m3(448 x / top).  A block that holds an infinity or a NaN gets NaN codes and a scale that is not finite. */
 int mm_cast_block128(const void* x, int type, int64_t rows, int k, int64_t row_stride, void* q, float* sf, void* stream);
 

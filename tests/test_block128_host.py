@@ -14,6 +14,8 @@ def test_cast_entry_points_refuse(built_lib):
     _refused(built_lib, f(P, 3, 4, 128, 128, P, P, None), "unknown type")
     _refused(built_lib, f(P, 0, 4, 12, 16, P, P, None), "multiples of 8")
     _refused(built_lib, f(P, 0, 4, 128, 120, P, P, None), "multiples of 8")
+    _refused(built_lib, f(P, 0, 4, 128, 132, P, P, None), "16 bytes")
+    _refused(built_lib, f(P, 2, 4, 128, 130, P, P, None), "16 bytes")
     _refused(built_lib, f(P, 0, -1, 128, 128, P, P, None), "multiples of 8")
     _refused(built_lib, f(None, 0, 4, 128, 128, P, P, None), "null")
     _refused(built_lib, f(P + 8, 0, 4, 128, 128, P, P, None), "aligned")

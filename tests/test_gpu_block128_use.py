@@ -224,3 +224,16 @@ def test_more_than_2_31_elements(g):
     assert out.numel() > 2 ** 31
     want, bound = ref.product_and_bound(ref.by_row(q[-100:], sf[-100:]), ref.by_block(*b))
     _assert_product(out[-100:], want, bound)
+
+
+def test_fp32_rows_that_begin_at_any_16_bytes(g):
+    """Rows of four more values than a multiple of eight: aligned for 16-byte loads, so they are read where they are."""
+    import megamoe
+    wide = torch.randn((7, 5 * 64 + 4), generator=g).cuda()
+    x, near = wide[:, 4:4 + 64], wide[:, 4:4 + 64].contiguous()
+    for a, b in zip(megamoe.cast_to_fp8_block128(x), megamoe.cast_to_fp8_block128(near)):
+        assert torch.equal(_bits(a), _bits(b))
+    y, r, gate, pre = wide[:, 68:132], x, wide[:, 200:264], torch.ones(64, device="cuda")
+    for a, b in zip(megamoe.norm_gate_residual(y, r, gate=gate, pre_weight=pre, quant="channelwise"),
+                    megamoe.norm_gate_residual(y.contiguous(), near, gate=gate.contiguous(), pre_weight=pre, quant="channelwise")):
+        assert torch.equal(_bits(a), _bits(b))
