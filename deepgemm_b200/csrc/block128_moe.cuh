@@ -801,7 +801,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                             if (ready_blocks == 0) {
                                 drain();
                                 int n = 0;
-                                if (lane == 0 && moe_wait_count(p.counters + p.ctr_done1 + rb, moe_finishers(rows) * nt1, abort_flag, p.timeout_ns)) n = max(look(), rb + 1);
+                                if (lane == 0 && moe_wait_count(p.counters + p.ctr_done1 + rb, moe_finishers(rows) * nt1, abort_flag, p.timeout_ns)) n = rb + 1;
                                 ready_blocks = __shfl_sync(0xffffffffu, n, 0);
                             }
                             if (ready_blocks == 0) { alive = false; break; }
