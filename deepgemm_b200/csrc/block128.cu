@@ -95,6 +95,12 @@ int device_of(Device** out) {
         B_CUDA(cudaFuncSetAttribute(mm::block128_gemm_kernel<128, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, mm::B128Shape<128>::kSmemBytes));
         B_CUDA(cudaFuncSetAttribute(mm::block128_gemm_kernel<128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, mm::B128Shape<128>::kSmemBytes));
         B_CUDA(cudaFuncSetAttribute(mm::moe_experts_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, mm::kMoeSmemBytes));
+#define B_STAGED(V, R) B_CUDA(cudaFuncSetAttribute(mm::norm_gate_residual_kernel<V, mm::B128_BF16, R, mm::B128_FP32, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * mm::kNormMaxHidden))
+        B_STAGED(1, mm::B128_BF16);
+        B_STAGED(1, mm::B128_FP32);
+        B_STAGED(2, mm::B128_BF16);
+        B_STAGED(2, mm::B128_FP32);
+#undef B_STAGED
         d.clusters[0] = d.sms;
         for (int i = 1; i < 4; ++i) {
             cudaLaunchConfig_t cfg;
@@ -234,7 +240,7 @@ int mm_norm_gate_residual(const void* y, int y_type, int64_t y_stride, const voi
                           const void* gate, int gate_type, int64_t gate_row_stride, int gate_col_stride, const void* pre, int pre_type,
                           void* r_out, void* x_out, int x_type, void* q, float* sf, int quant, int tokens, int hidden, float alpha, float eps,
                           float offset, void* stream_) {
-    B_REQUIRE(tokens >= 0 && hidden > 0 && hidden % 8 == 0 && hidden <= 16384, "mm_norm_gate_residual: hidden must be a multiple of 8, at most 16384");
+    B_REQUIRE(tokens >= 0 && hidden > 0 && hidden % 8 == 0 && hidden <= mm::kNormMaxHidden, "mm_norm_gate_residual: hidden must be a multiple of 8, at most 16384");
     B_REQUIRE(quant >= 0 && quant <= 2, "mm_norm_gate_residual: unknown cast");
     B_REQUIRE(known_type(y_type) && known_type(r_type) && known_type(post_type) && known_type(gate_type) && known_type(pre_type) && known_type(x_type),
               "mm_norm_gate_residual: unknown type");
@@ -265,14 +271,23 @@ int mm_norm_gate_residual(const void* y, int y_type, int64_t y_stride, const voi
     cudaStream_t st = static_cast<cudaStream_t>(stream_);
     const bool usual = (!y || y_type == mm::B128_BF16) && (!x_out || x_type == mm::B128_BF16) && (!post || post_type == mm::B128_FP32) &&
                        (!pre || pre_type == mm::B128_FP32) && (!gate || gate_type == mm::B128_FP32);
-#define B_NORM(V)                                                                                                                                           \
-    do {                                                                                                                                                    \
-        if (usual && r_type == mm::B128_BF16) mm::norm_gate_residual_kernel<V, mm::B128_BF16, mm::B128_BF16, mm::B128_FP32><<<(unsigned)blocks, threads, 0, st>>>(p);   \
-        else if (usual && r_type == mm::B128_FP32) mm::norm_gate_residual_kernel<V, mm::B128_BF16, mm::B128_FP32, mm::B128_FP32><<<(unsigned)blocks, threads, 0, st>>>(p); \
-        else mm::norm_gate_residual_kernel<V, mm::kAny, mm::kAny, mm::kAny><<<(unsigned)blocks, threads, 0, st>>>(p);                                     \
+    // Weights in shared memory, already with their offset and a gate that is the same for all rows, where a block does two rows or more
+    // (of 4096: 8192 rows 55 us instead of 61, 1200 14.3 instead of 14.8; 700, which make 592 blocks, 9.9 instead of 8.3).
+    const bool staged = tokens >= 2 * blocks;
+#define B_NORM(V, R)                                                                                                                                  \
+    do {                                                                                                                                              \
+        if (staged) mm::norm_gate_residual_kernel<V, mm::B128_BF16, R, mm::B128_FP32, true><<<(unsigned)blocks, threads, 8 * (size_t)hidden, st>>>(p); \
+        else mm::norm_gate_residual_kernel<V, mm::B128_BF16, R, mm::B128_FP32, false><<<(unsigned)blocks, threads, 0, st>>>(p);                       \
     } while (0)
-    if (two) B_NORM(2);
-    else B_NORM(1);
+#define B_NORM_TYPES(V)                                                                                                                               \
+    do {                                                                                                                                              \
+        if (usual && r_type == mm::B128_BF16) B_NORM(V, mm::B128_BF16);                                                                               \
+        else if (usual && r_type == mm::B128_FP32) B_NORM(V, mm::B128_FP32);                                                                          \
+        else mm::norm_gate_residual_kernel<V, mm::kAny, mm::kAny, mm::kAny, false><<<(unsigned)blocks, threads, 0, st>>>(p);                          \
+    } while (0)
+    if (two) B_NORM_TYPES(2);
+    else B_NORM_TYPES(1);
+#undef B_NORM_TYPES
 #undef B_NORM
     B_LAUNCHED();
     return 0;

@@ -266,19 +266,50 @@ __device__ __forceinline__ float squares(const F8& x, float before) {
     return f.x + f.y;
 }
 
+constexpr int kNormMaxHidden = 16384;
+
 // One row per block at a time, kVec vectors of 8 values per thread (vector i of a thread is number i * blockDim + threadIdx of the row).
 // The next row's values are loaded while this one is reduced.  kY, kR and kWeight: the types of y, of the residual, and of the weights
 // and the gate, or kAny; with types of its own the normed output is bf16.
-// Measured at 8192 x 4096 in bf16 with codes by blocks: 62 us, 4.9 TB/s of the bytes it must move (a plain copy: 6.5).  The first
-// form, without the prefetch and the two-wide arithmetic, took 107; one vector per thread 68, four 69, two rows at a time 60 to 76.
-template <int kVec, int kY, int kR, int kWeight>
+// kStaged: the weights of y (with a gate that is the same for all rows) and of r' are worked out once into shared memory.
+// Measured at 8192 x 4096 in bf16 with codes by blocks: 55 us, 5.5 TB/s of the bytes it must move (a plain copy: 6.5); instructions and the
+// three waits of a row share what is left.  With weights read and added up in every row 61; the first form, without the prefetch and the
+// two-wide arithmetic either, took 107; one vector per thread 68, four 69, two rows at a time 60 to 76 (all three before staging).
+template <int kVec, int kY, int kR, int kWeight, bool kStaged>
 __global__ void __launch_bounds__(1024) norm_gate_residual_kernel(const __grid_constant__ NormParams p) {
     __shared__ __align__(16) float s_sum[3][32];
+    extern __shared__ __align__(16) float s_weight[];                // kStaged: [2][hidden], of y and of r'
     const int vecs = p.hidden >> 3;
     const float inv_h = 1.0f / static_cast<float>(p.hidden);
     const auto add = [](float a, float b) { return a + b; };
     const uint64_t offset2 = pair(p.offset, p.offset), alpha2 = pair(p.alpha, p.alpha);
     for (int i = threadIdx.x; i < 3 * 32; i += blockDim.x) (&s_sum[0][0])[i] = 0.0f;
+    const bool channel_gate = p.gate != nullptr && p.gate_col_stride && p.gate_row_stride == 0;
+    const bool staged_y = kStaged && (p.post != nullptr || channel_gate);
+    if (kStaged) {
+        for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
+            F8 w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w.v[j] = pair(1.0f, 1.0f);
+            if (p.post != nullptr) {
+                w = load8<kWeight>(p.post, v * 8, p.w_post_type);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w.v[j] = add2(w.v[j], offset2);
+            }
+            if (channel_gate) {
+                const F8 g = load8<kWeight>(p.gate, v * 8, p.gate_type);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w.v[j] = mul2(w.v[j], g.v[j]);
+            }
+            store8<B128_FP32>(s_weight, v * 8, B128_FP32, w);
+            if (p.pre != nullptr) {
+                w = load8<kWeight>(p.pre, v * 8, p.w_pre_type);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w.v[j] = add2(w.v[j], offset2);
+                store8<B128_FP32>(s_weight, p.hidden + v * 8, B128_FP32, w);
+            }
+        }
+    }
     __syncthreads();
     Raw8 y_next[kVec], r_next[kVec];
     auto fetch = [&](int row) {
@@ -314,12 +345,17 @@ __global__ void __launch_bounds__(1024) norm_gate_residual_kernel(const __grid_c
             for (int i = 0; i < kVec; ++i) {
                 const int v = i * blockDim.x + threadIdx.x;
                 if (v >= vecs) continue;
-                if (p.post != nullptr) {
+                if (staged_y) {
+                    const F8 w = load8<B128_FP32>(s_weight, v * 8, B128_FP32);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) y[i].v[j] = mul2(y[i].v[j], w.v[j]);
+                }
+                if (!kStaged && p.post != nullptr) {
                     const F8 w = load8<kWeight>(p.post, v * 8, p.w_post_type);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) y[i].v[j] = mul2(y[i].v[j], add2(w.v[j], offset2));
                 }
-                if (p.gate != nullptr && p.gate_col_stride) {
+                if (p.gate != nullptr && p.gate_col_stride && !(kStaged && channel_gate)) {
                     const F8 g = load8<kWeight>(p.gate, row * p.gate_row_stride + v * 8, p.gate_type);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) y[i].v[j] = mul2(y[i].v[j], g.v[j]);
@@ -343,9 +379,16 @@ __global__ void __launch_bounds__(1024) norm_gate_residual_kernel(const __grid_c
                 const int v = i * blockDim.x + threadIdx.x;
                 const int64_t at = row * p.hidden + v * 8;
                 if (v < vecs) {
-                    const F8 w = load8<kWeight>(p.pre, v * 8, p.w_pre_type);
+                    F8 w;
+                    if (kStaged) {
+                        w = load8<B128_FP32>(s_weight, p.hidden + v * 8, B128_FP32);
+                    } else {
+                        w = load8<kWeight>(p.pre, v * 8, p.w_pre_type);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) r[i].v[j] = mul2(mul2(r[i].v[j], n2), add2(w.v[j], offset2));
+                        for (int j = 0; j < 4; ++j) w.v[j] = add2(w.v[j], offset2);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) r[i].v[j] = mul2(mul2(r[i].v[j], n2), w.v[j]);
                     if (p.x_out != nullptr) store8<kY == kAny ? kAny : B128_BF16>(p.x_out, at, p.x_type, r[i]);
                 }
                 if (p.quant == 1) {                  // 16 neighbouring threads hold one group

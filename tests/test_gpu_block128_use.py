@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import block128_ref as ref
-from test_gpu_block128 import _assert_product, _norm_ref
+from test_gpu_block128 import _assert_product, _norm_ref, test_norm as _check_norm
 from test_gpu_few_tokens import assert_layer, choose, layer64, make
 
 pytestmark = pytest.mark.gpu
@@ -237,3 +237,28 @@ def test_fp32_rows_that_begin_at_any_16_bytes(g):
     for a, b in zip(megamoe.norm_gate_residual(y, r, gate=gate, pre_weight=pre, quant="channelwise"),
                     megamoe.norm_gate_residual(y.contiguous(), near, gate=gate.contiguous(), pre_weight=pre, quant="channelwise")):
         assert torch.equal(_bits(a), _bits(b))
+
+
+@pytest.mark.parametrize("t,h", [(1300, 4096), (1250, 4104), (301, 16384), (2500, 2056)])
+@pytest.mark.parametrize("rt,gate,quant", [(torch.bfloat16, "channel", "block128"), (torch.float32, "channel", "channelwise"), (torch.bfloat16, "token", None),
+                                           (torch.bfloat16, None, "channelwise"), (torch.float32, "full", "block128")])
+def test_norm_of_many_rows(g, t, h, rt, gate, quant):
+    """Several rows for each block of threads: weights are worked out once, with the gate if it is the same for all rows."""
+    _check_norm(g, t, h, quant, torch.bfloat16, rt, torch.float32, gate)
+
+
+def test_norm_of_many_rows_without_its_parts(g):
+    import megamoe
+    t, h = 1300, 4096
+    y, r = torch.randn((t, h), generator=g).cuda().bfloat16(), torch.randn((t, h), generator=g).cuda().bfloat16()
+    pre, gate = torch.rand(h, generator=g).cuda() + 0.5, torch.randn(h, generator=g).cuda()
+    # (rows alone take the other path: one row for each block of threads)
+    for kw in (dict(pre_weight=pre), dict(gate=gate), dict(gate=gate, pre_weight=pre, weight_offset=1.0), dict(post_weight=pre)):
+        many, few = megamoe.norm_gate_residual(y, r, **kw), megamoe.norm_gate_residual(y[:9], r[:9], **kw)
+        for a, b in zip(many, few):
+            assert (a is None) == (b is None)
+            if a is not None:           # the same roundings but for the order of the sum of squares and of weight and gate
+                assert bool(((a[:9].float() - b.float()).abs() <= 2.0 ** -7 * b.float().abs() + 2.0 ** -8 * r[:9].float().abs()).all())
+    first = megamoe.norm_gate_residual(None, r, pre_weight=pre)
+    want, _, x, xmag = _norm_ref(None, r.cpu(), None, None, 1.0, pre.cpu(), 1e-6, 0.0)
+    assert first.residual is r and bool(((first.normed.cpu().double() - x).abs() <= 64 * 2.0 ** -24 * xmag + 2.0 ** -8 * (x.abs() + 64 * 2.0 ** -24 * xmag)).all())
