@@ -292,14 +292,14 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
         prefetch_tensormap(&tm_a);
         prefetch_tensormap(&tm_b);
     }
-    if (warp == 2) {
-        tmem_alloc(smem_u32(tmem_slot), 512);
-        tmem_relinquish();
-    }
-    tc_fence_before();
     __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem_base = *tmem_slot;
+    // TMEM is allocated while the first copies are on their way; the MMA warp and the epilogue meet behind it
+    auto tmem_ready = [&]() {
+        tc_fence_before();
+        named_bar_sync(1, kB128Threads - 96);
+        tc_fence_after();
+        return *static_cast<volatile uint32_t*>(tmem_slot);
+    };
 
     // expert of an m tile (grouped: of its first row), or -1 when there is nothing to do; every role asks and skips alike
     auto tile_expert = [&](int mt) {
@@ -331,12 +331,15 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                     if (++stage == kStages) { stage = 0; phase ^= 1u; }
                 }
             }
-        } else if (warp == 1 && lane == 0) {
+        } else if (warp == 1) {
             // ------------------------------------------------------------------ MMA
             constexpr uint32_t idesc = umma_idesc_f8(128, kBN);
+            tmem_alloc(smem_u32(tmem_slot), 512);
+            tmem_relinquish();
+            const uint32_t tmem_base = tmem_ready();
             int stage = 0; uint32_t phase = 0;
             int acc = 0; uint32_t acc_phase = 0;
-            bool alive = true;
+            bool alive = lane == 0;
             for (int tile = first_tile; tile < num_tiles && alive; tile += tile_step) {
                 int mt, nt;
                 b128_tile(p, tile, mt, nt);
@@ -396,6 +399,7 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     } else {
         // ---------------------------------------------------------------------- epilogue
         regs_inc<208>();                                         // 2 x 208 + 88 = 3 x 168, the registers of the launch
+        const uint32_t tmem_base = tmem_ready();
         // row et of the tile is lane et % 32 of TMEM's quarter et / 32; warps 4-7 take the first half of the columns, 8-11 the second
         const uint32_t my_tmem = tmem_base + (static_cast<uint32_t>(warp & 3) << 21) + ((warp - 4) >> 2) * kCols;
         const uint32_t my_scale = smem_u32(scales) + (threadIdx.x & 127) * 4;
@@ -491,9 +495,9 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 2) {
+    if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem_base, 512);
+        tmem_dealloc(*tmem_slot, 512);
     }
 }
 
