@@ -330,7 +330,7 @@ int mm_fp8_gemm_block128(const void* a, int64_t a_stride, const float* sa, int64
     B_REQUIRE(tiles < kMaxDim, "mm_fp8_gemm_block128: too many tiles");
     p.n_tiles = bn == 256 ? (n + 255) / 256 : n_sf;
     int log_split = 0;
-    while (bn == 128 && !m_indices && log_split < 3 && tiles <= d->clusters[log_split + 1] && kb >= (4 << log_split)) ++log_split;
+    while (bn == 128 && !m_indices && (2 << log_split) <= mm::kB128MaxSplit && tiles <= d->clusters[log_split + 1] && kb >= (4 << log_split)) ++log_split;
     const int split = 1 << log_split;
     CUtensorMap tm_a, tm_b;
     if (int rc = byte_map(a, (uint64_t)k, (uint64_t)m, (uint64_t)a_stride, 0, 0, (uint32_t)p.a_box_rows, &tm_a)) return rc;

@@ -24,6 +24,7 @@
 namespace mm {
 
 constexpr int kB128Threads = 384;
+constexpr int kB128MaxSplit = 8;           // CTAs that share a tile: the largest portable cluster
 
 struct B128GemmParams {
     int m, n, k_blocks;
@@ -449,34 +450,29 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
         if (warp >= 4 && ld_shared_volatile(abort_flag) == 0 && first_tile < num_tiles) {
             int mt, nt;
             b128_tile(p, first_tile, mt, nt);
-            const int e = tile_expert(mt);
-            const int rows = e < 0 ? 0 : min(128, p.m - mt * 128);
-            constexpr int kPer = kBN / 32;                   // columns of a lane: 4 at a time
+            // rows part, part + split, .. of the tile are this CTA's: a warp to a row, four columns a lane
+            static_assert(!kSplit || kBN == 128, "a warp holds a row of a split tile");
+            const int rows = min(128, p.m - mt * 128), col = nt * kBN + lane * 4;
             for (int r = part + (warp - 4) * split; r < rows; r += 8 * split) {
-                const int row = mt * 128 + r;
-                if (p.m_indices != nullptr && p.m_indices[row] != e) continue;
+                const uint32_t at = smem_base + static_cast<uint32_t>(r * (kBN + 4) + lane * 4) * 4;
+                float4 v[kB128MaxSplit], t = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int c0 = 0; c0 < kPer; c0 += 4) {
-                    const int c = (c0 / 4) * 128 + lane * 4;
-                    const uint32_t at = smem_base + static_cast<uint32_t>(r * (kBN + 4) + c) * 4;
-                    float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int i = 0; i < split; ++i) {
-                        const float4 v = ld_shared_cluster_f4(mapa_shared(at, i));
-                        t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w;
-                    }
-                    const int col = nt * kBN + c;
-                    const float f[4] = {t.x, t.y, t.z, t.w};
-                    const int64_t o = row * p.out_stride + col;
-                    if (p.out_vec32 && col + 4 <= p.n) {
-                        if (p.out_fp32) *reinterpret_cast<float4*>(static_cast<float*>(p.out) + o) = t;
-                        else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + o) = make_uint2(pack_bf16x2(t.x, t.y), pack_bf16x2(t.z, t.w));
-                    } else {
+                for (int i = 0; i < kB128MaxSplit; ++i)                  // all on their way before the first is added
+                    if (i < split) v[i] = ld_shared_cluster_f4(mapa_shared(at, i));
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            if (col + j >= p.n) continue;
-                            if (p.out_fp32) static_cast<float*>(p.out)[o + j] = f[j];
-                            else static_cast<__nv_bfloat16*>(p.out)[o + j] = __float2bfloat16(f[j]);
-                        }
+                for (int i = 0; i < kB128MaxSplit; ++i)
+                    if (i < split) { t.x += v[i].x; t.y += v[i].y; t.z += v[i].z; t.w += v[i].w; }
+                const float f[4] = {t.x, t.y, t.z, t.w};
+                const int64_t o = (mt * 128 + r) * p.out_stride + col;
+                if (p.out_vec32 && col + 4 <= p.n) {
+                    if (p.out_fp32) *reinterpret_cast<float4*>(static_cast<float*>(p.out) + o) = t;
+                    else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + o) = make_uint2(pack_bf16x2(t.x, t.y), pack_bf16x2(t.z, t.w));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (col + j >= p.n) continue;
+                        if (p.out_fp32) static_cast<float*>(p.out)[o + j] = f[j];
+                        else static_cast<__nv_bfloat16*>(p.out)[o + j] = __float2bfloat16(f[j]);
                     }
                 }
             }
