@@ -150,7 +150,7 @@ struct MoeWork {
     int num_counters, ctr_done1, ctr_tile1, part_rows, act_sf_pitch;
 };
 
-MoeWork moe_work(int T, int E, int K, int H, int I, bool cast, int ctas) {
+MoeWork moe_work(int T, int E, int K, int H, int I, int ctas) {
     MoeWork w;
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t o = at; at = (at + bytes + 255) / 256 * 256; return o; };
@@ -164,8 +164,8 @@ MoeWork moe_work(int T, int E, int K, int H, int I, bool cast, int ctas) {
     w.counters = take((int64_t)w.num_counters * 4);
     w.route_expert = take(routes * 4);
     w.route_w = take(routes * 4);
-    w.xq = take(cast ? (int64_t)T * H : 0);
-    w.xsf = take(cast ? (int64_t)T * (H / 128) * 4 : 0);
+    w.xq = take((int64_t)T * H);
+    w.xsf = take((int64_t)T * (H / 128) * 4);
     w.act_q = take(routes * I);
     w.act_sf_pitch = (I / 128 + 31) / 32 * 32;
     w.act_sf = take(routes * w.act_sf_pitch * 4);
@@ -359,7 +359,7 @@ int mm_moe_few_tokens_workspace(int T, int E, int K, int H, int I, int64_t* byte
     if (int rc = moe_check_shape(T, E, K, H, I)) return rc;
     Device* d;
     if (int rc = device_of(&d)) return rc;
-    *bytes = moe_work(T, E, K, H, I, true, d->sms).total;
+    *bytes = moe_work(T, E, K, H, I, d->sms).total;
     return 0;
 }
 
@@ -377,7 +377,7 @@ int mm_moe_few_tokens(const void* x, int x_is_fp8, int64_t x_stride, const float
     B_REQUIRE(!logits || logits_stride >= E, "mm_moe_few_tokens: bad logits stride");
     Device* d;
     if (int rc = device_of(&d)) return rc;
-    const MoeWork w = moe_work(T, E, K, H, I, true, d->sms);
+    const MoeWork w = moe_work(T, E, K, H, I, d->sms);
     B_REQUIRE(work_bytes >= w.total, "mm_moe_few_tokens: needs %lld bytes of work memory, has %lld", (long long)w.total, (long long)work_bytes);
     uint8_t* base = static_cast<uint8_t*>(work);
     mm::MoeParams p;
