@@ -322,6 +322,10 @@ __device__ __forceinline__ int atomic_add_acq_rel(int* p, int v) {
     return old;
 }
 
+// Rows of a tile in each quarter of TMEM.  Up to 64 of them take an MMA with M = 64 (16 lanes of each quarter): the same time, half of the
+// tensor core's power.
+__device__ __forceinline__ int moe_lanes(int rows) { return rows <= 64 ? 16 : 32; }
+
 // Work memory for the sums of a tile, [part_rows][256]: of a part, by the chunk that brought it (a chunk holds two at most, one that its
 // beginning cuts off and one its end), or of a whole tile, two for each CTA in turn.
 __device__ __forceinline__ float* moe_part(const MoeParams& p, const MoeList& l, int kind, int ch, int tile, bool whole, int buffer) {
@@ -722,7 +726,6 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
         } else if (warp == 1) {
             // ------------------------------------------------------------------ MMA
             if (lane == 0) {
-                constexpr uint32_t idesc = umma_idesc_f8(128, 256);
                 int stage = 0; uint32_t phase = 0;
                 int acc = 0; uint32_t acc_phase = 0;
                 Place at;
@@ -731,6 +734,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                     const MoeSegment* g = segment_at(at);
                     if (g == nullptr || g->kind < 0) break;
                     const int units = g->k1 - g->k0;
+                    const uint32_t idesc = moe_lanes(g->rows) == 16 ? umma_idesc_f8(64, 256) : umma_idesc_f8(128, 256);
                     segment_done(at);
                     step(at);
                     for (int u = 0; u < units; ++u) {
@@ -868,7 +872,6 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
         // ---------------------------------------------------------------------- sums
         regs_inc<176>();
         const int q = warp & 3, half = (warp - 8) >> 2;
-        const int et = q * 32 + lane;
         int acc = 0; uint32_t acc_phase = 0;
         int slot = 0;                                                // place of the next unit in the ring of scales
         int buffer = 0; uint32_t buffer_phase = 0;
@@ -878,13 +881,14 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
             const MoeSegment* g = segment_at(at);
             if (g == nullptr || g->kind < 0) break;
             const int units = g->k1 - g->k0;
-            if (q * 32 < g->rows) {
+            const int lanes = moe_lanes(g->rows), et = lane < lanes ? q * lanes + lane : 127;                            // row of the tile; 127: none
+            if (q * lanes < g->rows) {
                 // column parts A and B of this thread: gate and up, or two neighbouring runs of 64 outputs
                 const int col_a = g->kind ? half * 128 : half * 64, col_b = g->kind ? col_a + 64 : col_a + 128;
                 const int sb_a = g->kind ? 128 + half : 128, sb_b = g->kind ? 128 + half : 129;
                 // Warps without a row of the tile take no part in this: waiting beside the others they slow them down.  The barrier
                 // that gives the accumulator back counts all eight, so the warps of the first rows arrive for the idle ones.
-                const uint32_t arrivals = q == 0 ? 5u - static_cast<uint32_t>((g->rows + 31) >> 5) : 1u;
+                const uint32_t arrivals = q == 0 ? 5u - static_cast<uint32_t>((g->rows + lanes - 1) / lanes) : 1u;
                 uint64_t sum[64];                                    // pairs: 64 columns of part A, 64 of part B
 #pragma unroll
                 for (int j = 0; j < 64; ++j) sum[j] = 0ull;
@@ -903,7 +907,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                 if (!alive || !mbar_wait_often(sm.turn_empty(buffer), buffer_phase ^ 1u, abort_flag, p.timeout_ns)) break;
                 // Where the sums go next: rows of activations that are finished here to shared memory if they fit; else, and parts of a
                 // tile, to work memory; whole rows of outputs straight to their place.
-                if (et < g->rows) {
+                if (lane < lanes && et < g->rows) {
                     const MoeList& l = sm.words->list[g->kind];
                     const bool whole = g->k1 - g->k0 == l.kb;
                     if (g->kind && whole) {
