@@ -21,7 +21,8 @@
 // for is always being worked on, however many of the CTAs are resident, and two such launches may share a GPU.
 //
 // Measured: 1 token, 256 experts, top-6, 4096 / 2048: 47 us (151 MB; 3.2 TB/s over the whole call, the streams themselves run at 6); 33 tokens,
-// 64 experts, top-8, 2048 / 1024: 87 us (398 MB, 4.6 TB/s).  What bounds it at one token are the latencies around the streams: 8 us until the first
+// 64 experts, top-8, 2048 / 1024: 87 us (398 MB, 4.6 TB/s); 128 tokens, else as the first: 680 us alone, 740 in a loop, where the power cap
+// sets the clock.  What bounds it at one token are the latencies around the streams: 8 us until the first
 // copy, 8 from the last sums of the first product to its activations being known everywhere, 4 for the combine.
 //
 // Tile = up to 128 routes of one expert x 256 weight rows (first product: 128 gate rows and their 128 up rows, so that a tile holds
@@ -37,8 +38,8 @@ namespace mm {
 constexpr int kMoeMaxRoutes = 4096;
 constexpr int kMoeMaxBlocks = MM_MAX_EXPERTS + kMoeMaxRoutes / 128;      // of up to 128 routes of one expert
 constexpr int kMoeBBytes = 256 * 128;
-// The operand ring: four stages with room for 128 token rows, or five with room for 48 where no expert has more.  (An MMA reads 128 rows
-// either way; those behind the last route are whatever the ring holds there, and their sums are not looked at.)
+// The operand ring: four stages with room for 128 token rows, or five with room for 48 where no expert has more.  (An MMA reads 64
+// or 128 rows either way; those behind the last route are zeroes, or what follows in the ring, and their sums are not looked at.)
 constexpr int kMoeMaxStages = 5, kMoeFewRows = 48;
 constexpr int kMoeRingBytes = 4 * (128 * 128 + kMoeBBytes);
 static_assert(kMoeMaxStages * (kMoeFewRows * 128 + kMoeBBytes) <= kMoeRingBytes, "the ring of few rows");
@@ -323,8 +324,10 @@ __device__ __forceinline__ int atomic_add_acq_rel(int* p, int v) {
 }
 
 // Rows of a tile in each quarter of TMEM.  Up to 64 of them take an MMA with M = 64 (16 lanes of each quarter): the same time, half of the
-// tensor core's power.
+// tensor core's power (128 tokens in a loop: 780 us instead of 880).
 __device__ __forceinline__ int moe_lanes(int rows) { return rows <= 64 ? 16 : 32; }
+
+__device__ __forceinline__ void st_shared_zero16(uint32_t addr) { asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0) : "memory"); }
 
 // Work memory for the sums of a tile, [part_rows][256]: of a part, by the chunk that brought it (a chunk holds two at most, one that its
 // beginning cuts off and one its end), or of a whole tile, two for each CTA in turn.
@@ -763,6 +766,9 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
             int ready_blocks = 0;                                    // this CTA's chunks of the second product go up in blocks of routes
             Place at;
             bool alive = true;
+            // Rows behind a tile's last one are read by its MMAs all the same; zeroes there cost the least power (128 tokens in a loop: 737
+            // us instead of 761).  Rows that a stage may hold, a byte for each stage.
+            uint64_t filled = 0x0101010101010101ull * (few_rows ? kMoeFewRows : 128u);
             auto hand_over = [&]() {
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -832,6 +838,11 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                             cp_async_16(dst + r * 128 + ((piece ^ (r & 7)) << 4), src + static_cast<int64_t>(row) * pitch + k * 128 + piece * 16);
                         }
                         cp_async_commit();
+                        const int before = static_cast<int>(filled >> (8 * stage)) & 255;
+                        if (before != rows) {
+                            for (int r = rows + (l64 >> 3); r < before; r += 8) st_shared_zero16(dst + r * 128 + piece * 16);
+                            filled ^= static_cast<uint64_t>(before ^ rows) << (8 * stage);
+                        }
                         ++pending;
                         if (++stage == stages) { stage = 0; phase ^= 1u; }
                         if (pending > kAhead) {
