@@ -322,7 +322,7 @@ int mm_fp8_gemm_block128(const void* a, int64_t a_stride, const float* sa, int64
     // Tile width and split of K.  A turn of the SMs with tiles of 128 columns takes 0.7 of the time of one with 256 (1024 x 4096 x 4096: 29 us in
     // two turns of 128, 21 in one of 256), so 128 is taken where that makes less.  The k blocks of a tile are then divided among up to
     // eight CTAs, as long as all clusters are resident at once (1 x 4096 x 4096: 8.2 us with four CTAs to a tile, 11.0 with two, 15.0 with
-    // one) and each CTA keeps a few blocks.
+    // one, before the parts were read side by side) and each CTA keeps a few blocks.
     const int64_t tiles256 = (int64_t)p.m_tiles * ((n + 255) / 256), tiles128 = (int64_t)p.m_tiles * n_sf;
     const int64_t turns256 = (tiles256 + d->sms - 1) / d->sms, turns128 = (tiles128 + d->sms - 1) / d->sms;
     const int bn = turns128 * 7 < turns256 * 10 ? 128 : 256;

@@ -415,6 +415,13 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                 b128_check_group(p, mt, threadIdx.x & 127);
                 if (tile_expert(mt) < 0) continue;
             }
+            // A split tile has few rows, as a rule; warps without any only hand the accumulators back.
+            bool idle = false;
+            if (kSplit) {
+                int mt, nt;
+                b128_tile(p, tile, mt, nt);
+                idle = mt * 128 + (warp & 3) * 32 >= p.m;
+            }
             uint64_t sum[kCols / 2];
 #pragma unroll
             for (int j = 0; j < kCols / 2; ++j) sum[j] = 0ull;
@@ -422,11 +429,16 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
             for (int left = kb1 - kb0; left > 0; --left, ++n) {
                 const uint32_t acc = n % kAccs;
                 if (!mbar_wait_often(tfull_bar(acc), (n / kAccs) & 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
+                if (kSplit && idle) {
+                    if (elect_lane()) mbar_arrive(tempty_bar(acc));
+                    continue;
+                }
                 tc_fence_after();
                 const uint32_t slot = (n % S::kScaleSlots) * S::kScaleBytes;
                 b128_promote<kCols>(sum, my_tmem + acc * kBN, my_scale + slot, my_weight_scale + slot, tempty_bar(acc));
             }
             if (!alive) break;
+            if (kSplit && idle) continue;
             if (kSplit) {
                 // this CTA's part of the tile, for the cluster to add up: the operand ring is idle now (the last accumulator
                 // was complete, so every copy and every MMA of this CTA is done)
