@@ -162,6 +162,8 @@ constexpr int kCastGroups = 4;
 template <int kType, bool kFlat>
 __global__ void __launch_bounds__(256) cast_block128_kernel(const void* __restrict__ x, int64_t row_stride, uint32_t groups,
                                                             uint32_t groups_per_row, int k, uint8_t* __restrict__ q, float* __restrict__ sf) {
+    pdl_launch();
+    pdl_wait();
     const uint32_t lane16 = threadIdx.x & 15;
     const uint32_t first = blockIdx.x * (16 * kCastGroups) + (threadIdx.x >> 4);
     F8 v[kCastGroups];
@@ -277,6 +279,7 @@ constexpr int kNormMaxHidden = 16384;
 // two-wide arithmetic either, took 107; one vector per thread 68, four 69, two rows at a time 60 to 76 (all three before staging).
 template <int kVec, int kY, int kR, int kWeight, bool kStaged>
 __global__ void __launch_bounds__(1024) norm_gate_residual_kernel(const __grid_constant__ NormParams p) {
+    pdl_launch();
     __shared__ __align__(16) float s_sum[3][32];
     extern __shared__ __align__(16) float s_weight[];                // kStaged: [2][hidden], of y and of r'
     const int vecs = p.hidden >> 3;
@@ -284,6 +287,7 @@ __global__ void __launch_bounds__(1024) norm_gate_residual_kernel(const __grid_c
     const auto add = [](float a, float b) { return a + b; };
     const uint64_t offset2 = pair(p.offset, p.offset), alpha2 = pair(p.alpha, p.alpha);
     for (int i = threadIdx.x; i < 3 * 32; i += blockDim.x) (&s_sum[0][0])[i] = 0.0f;
+    pdl_wait();
     const bool channel_gate = p.gate != nullptr && p.gate_col_stride && p.gate_row_stride == 0;
     const bool staged_y = kStaged && (p.post != nullptr || channel_gate);
     if (kStaged) {

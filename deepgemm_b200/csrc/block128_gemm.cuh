@@ -293,6 +293,8 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
         prefetch_tensormap(&tm_a);
         prefetch_tensormap(&tm_b);
     }
+    pdl_launch();
+    pdl_wait();
     __syncthreads();
     // TMEM is allocated while the first copies are on their way; the MMA warp and the epilogue meet behind it
     auto tmem_ready = [&]() {

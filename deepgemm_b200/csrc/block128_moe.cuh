@@ -84,9 +84,6 @@ struct MoeParams {
     uint64_t timeout_ns;
 };
 
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // kPer: experts per lane.  Ties go to the lower index; NaN and -inf logits are never chosen.
 template <int kPer>
 __device__ __forceinline__ void moe_topk(const MoeParams& p, int t, int lane) {
@@ -130,6 +127,7 @@ __device__ __forceinline__ void moe_topk(const MoeParams& p, int t, int lane) {
 
 __global__ void __launch_bounds__(256) moe_route_kernel(const MoeParams p) {
     pdl_launch();
+    pdl_wait();
     const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < p.num_counters; i += gridDim.x * blockDim.x) p.counters[i] = 0;
     if (warp == 0) {
@@ -526,6 +524,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t smem_base = smem_u32(smem);
     const MoeSmem sm(smem);
+    pdl_launch();
     auto full_bar = [&](int s) { return sm.bars + 8u * s; };
     auto empty_bar = [&](int s) { return sm.bars + 8u * (kMoeMaxStages + s); };
     auto tfull_bar = [&](int a) { return sm.bars + 8u * (2 * kMoeMaxStages + a); };

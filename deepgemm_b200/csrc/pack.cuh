@@ -6,6 +6,11 @@
 
 namespace mm {
 
+// A kernel launched with programmatic stream serialization may start while the one before it in the stream drains: it waits, in every
+// block, before it reads or writes global memory; and it lets the next one start as soon as all of its blocks have.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 __device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 

@@ -262,3 +262,49 @@ def test_norm_of_many_rows_without_its_parts(g):
     first = megamoe.norm_gate_residual(None, r, pre_weight=pre)
     want, _, x, xmag = _norm_ref(None, r.cpu(), None, None, 1.0, pre.cpu(), 1e-6, 0.0)
     assert first.residual is r and bool(((first.normed.cpu().double() - x).abs() <= 64 * 2.0 ** -24 * xmag + 2.0 ** -8 * (x.abs() + 64 * 2.0 ** -24 * xmag)).all())
+
+
+def test_captured_behind_copies_and_other_streams(g):
+    """First kernel of a graph, or behind a copy, a memset or an event of another stream: every kind of edge before a call."""
+    import megamoe
+    block = Block(g)
+    host = torch.randn((6, 512), generator=g).pin_memory()
+    r, other = torch.zeros((6, 512), device="cuda"), torch.zeros((6, 512), device="cuda")
+    raw = torch.zeros((6, 512), dtype=torch.uint8, device="cuda").view(ref.E4M3)
+    block(r)
+    q0, s0 = megamoe.cast_to_fp8_block128(r)
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        first = megamoe.cast_to_fp8_block128(r)                     # the graph's first node
+        other.copy_(r)                                              # device to device
+        second = megamoe.cast_to_fp8_block128(other)
+        r.copy_(host, non_blocking=True)                            # host to device
+        out = block(r)
+        raw.view(torch.uint8).zero_()
+        product = megamoe.fp8_gemm_nt_block128((raw, s0), block.shared)
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            beside = megamoe.norm_gate_residual(out["routed"], r, pre_weight=block.pre, quant="block128")
+        main.wait_stream(side)
+        joined = megamoe.fp8_gemm_nt_block128((beside.codes, beside.scales), block.shared)
+    for _ in range(3):
+        before = torch.randn((6, 512), generator=g)
+        r.copy_(before)
+        host.copy_(torch.randn((6, 512), generator=g))
+        raw.view(torch.uint8).fill_(0x38)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        q, s = megamoe.cast_to_fp8_block128(before.cuda())
+        for a in (first, second):
+            assert torch.equal(_bits(a[0]), _bits(q)) and torch.equal(a[1], s)
+        want = block(host.cuda())
+        for name in want:
+            assert torch.equal(_bits(out[name]), _bits(want[name])), name
+        assert bool((product == 0).all())
+        n = megamoe.norm_gate_residual(want["routed"], host.cuda(), pre_weight=block.pre, quant="block128")
+        assert torch.equal(_bits(beside.codes), _bits(n.codes))
+        assert torch.equal(joined, megamoe.fp8_gemm_nt_block128((n.codes, n.scales), block.shared))
+    megamoe.check_block128_status()
