@@ -160,8 +160,8 @@ __device__ __forceinline__ F8 zero8() { return F8{{0ull, 0ull, 0ull, 0ull}}; }
 constexpr int kCastGroups = 4;
 
 template <int kType, bool kFlat>
-__global__ void __launch_bounds__(256) cast_block128_kernel(const void* __restrict__ x, int64_t row_stride, uint32_t groups,
-                                                            uint32_t groups_per_row, int k, uint8_t* __restrict__ q, float* __restrict__ sf) {
+__global__ void __launch_bounds__(256) cast_block128_kernel(const void* x, int64_t row_stride, uint32_t groups, uint32_t groups_per_row,
+                                                            int k, uint8_t* q, float* sf) {      // (no __restrict__: a load that counts as invariant could pass pdl_wait)
     pdl_launch();
     pdl_wait();
     const uint32_t lane16 = threadIdx.x & 15;
