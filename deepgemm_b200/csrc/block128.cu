@@ -19,8 +19,9 @@ void mm_detail_set_error(const char* msg);
 void mm_detail_count_launch();
 uint64_t mm_detail_pipe_timeout_ns();
 
-// First failed wait or bad layout of any of these operators on a device since it was last read; written by kernels only then.
-__device__ int g_b128_status[8];
+// First failed wait or bad layout of any of these operators on a device since it was last read (b128_report); written by kernels only then.
+// [8 .. 12]: what the last read took.
+__device__ int g_b128_status[16];
 
 namespace {
 
@@ -431,8 +432,11 @@ int mm_block128_read_status(void* stream_, int32_t* out5) {
     Device* d;
     if (int rc = device_of(&d)) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream_);
-    B_CUDA(cudaMemcpyAsync(out5, d->status, 5 * sizeof(int32_t), cudaMemcpyDeviceToHost, st));
-    B_CUDA(cudaMemsetAsync(d->status, 0, 8 * sizeof(int), st));
+    static std::mutex mu;                // one reader at a time: they share the words that a read takes the report to
+    std::lock_guard<std::mutex> lk(mu);
+    mm::b128_take_status_kernel<<<1, 1, 0, st>>>(d->status, d->status + 8);
+    B_LAUNCHED();
+    B_CUDA(cudaMemcpyAsync(out5, d->status + 8, 5 * sizeof(int32_t), cudaMemcpyDeviceToHost, st));
     B_CUDA(cudaStreamSynchronize(st));
     return 0;
 }

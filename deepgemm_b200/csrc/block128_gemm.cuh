@@ -244,13 +244,34 @@ __device__ __forceinline__ void b128_store(const B128GemmParams& p, const uint64
     }
 }
 
+// Status words of a device: [0] code of the first failure since the last read, [1 .. 4] its details, [5] whether a failure has been claimed.
+// The claim comes first and the code last, so that a reader on another stream finds either nothing yet or all of it.
+__device__ __forceinline__ void b128_report(int* status, int code, int phase, int block, int expected, int observed) {
+    if (atomicCAS(status + 5, 0, 1) != 0) return;
+    volatile int* s = status;
+    s[1] = phase; s[2] = block; s[3] = expected; s[4] = observed;
+    __threadfence();
+    atomicExch(status, code);
+}
+// Hands the report over, if there is one, and makes room for the next.  Copying and clearing as two operations of a stream lost what another
+// stream's kernel reported between them (one of eight reports in a loop of reads), or saw its code without its details.
+__global__ void b128_take_status_kernel(int* status, int* taken) {
+    const int code = ld_acquire_gpu(status);
+    volatile const int* s = status;
+    taken[0] = code;
+    for (int i = 1; i < 5; ++i) taken[i] = code != 0 ? s[i] : 0;
+    if (code == 0) return;
+    __threadfence();
+    atomicExch(status, 0);
+    __threadfence();
+    atomicExch(status + 5, 0);
+}
+
 // A 128-row block of a grouped layout: rows of another expert than its first one, or behind padding, are a mistake, reported and not written.
 __device__ __forceinline__ void b128_check_group(const B128GemmParams& p, int mt, int et) {
     const int first = p.m_indices[mt * 128];
     const int own = p.m_indices[mt * 128 + et];
-    if ((first >= p.experts || (own >= 0 && own != first)) && atomicCAS(p.status, 0, MM_ERR_BAD_GROUP_LAYOUT) == 0) {
-        p.status[1] = 0; p.status[2] = mt; p.status[3] = first; p.status[4] = own;
-    }
+    if (first >= p.experts || (own >= 0 && own != first)) b128_report(p.status, MM_ERR_BAD_GROUP_LAYOUT, 0, mt, first, own);
 }
 
 template <int kBN, bool kSplit>
@@ -499,9 +520,7 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
         // a bounded wait expired: give copies that may still be in flight time to land, then report
         const uint64_t t0 = global_timer_ns();
         while (global_timer_ns() - t0 < 1000000ull) __nanosleep(1000);
-        if (threadIdx.x == 0 && atomicCAS(p.status, 0, MM_ERR_PIPE_TIMEOUT) == 0) {
-            p.status[1] = 20; p.status[2] = blockIdx.x; p.status[3] = num_tiles; p.status[4] = 0;
-        }
+        if (threadIdx.x == 0) b128_report(p.status, MM_ERR_PIPE_TIMEOUT, 20, blockIdx.x, num_tiles, 0);
     }
     tc_fence_before();
     __syncthreads();

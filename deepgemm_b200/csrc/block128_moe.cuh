@@ -964,9 +964,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
         // a bounded wait expired: give copies that may still be in flight time to land, then report
         const uint64_t t0 = global_timer_ns();
         while (global_timer_ns() - t0 < 1000000ull) __nanosleep(1000);
-        if (threadIdx.x == 0 && atomicCAS(p.status, 0, MM_ERR_PIPE_TIMEOUT) == 0) {
-            p.status[1] = 30; p.status[2] = blockIdx.x; p.status[3] = chunks; p.status[4] = 0;
-        }
+        if (threadIdx.x == 0) b128_report(p.status, MM_ERR_PIPE_TIMEOUT, 30, blockIdx.x, chunks, 0);
     }
     tc_fence_before();
     __syncthreads();

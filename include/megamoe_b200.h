@@ -184,7 +184,8 @@ int mm_moe_few_tokens(const void* x, int x_is_fp8, int64_t x_stride, const float
                       void* y, void* stream);
 
 /* First failure on the current device that these operators have met since the last call, as {code, phase, block, expected, observed},
- * and clears it; code 0 = none.  Synchronises the stream. */
+ * and clears it; code 0 = none.  Synchronises the stream.  Any stream will do, also while others run these operators: a report is
+ * taken whole, by this read or by a later one. */
 int mm_block128_read_status(void* stream, int32_t* out5);
 
 /* JSON description of the build.  Replaces get_mega_moe_hip_build_config, csrc/apis/mega_dcu.hpp:28-39. */
