@@ -65,6 +65,7 @@ _SIGNATURES = {
     "mm_moe_few_tokens": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                   c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_int64, c_void_p, c_void_p]),
     "mm_block128_read_status": (c_int, [c_void_p, POINTER(c_int32)]),
+    "mm_block128_test_waits": (c_int, [c_int, c_int64]),
     "mm_set_stage_timing": (c_int, [c_int]),
     "mm_get_stage_times": (c_int, [POINTER(c_float), c_int]),
 }

@@ -6,6 +6,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <atomic>
 #include <mutex>
 
 #include "../../include/megamoe_b200.h"
@@ -49,6 +50,14 @@ int fail(int code, const char* fmt, ...) {
         mm_detail_count_launch();     \
         B_CUDA(cudaGetLastError());   \
     } while (0)
+
+// mm_block128_test_waits
+std::atomic<int> g_given_up{-1};
+std::atomic<int64_t> g_limit_ns{0};
+uint64_t wait_limit_ns() {
+    const int64_t test = g_limit_ns.load();
+    return test > 0 ? (uint64_t)test : mm_detail_pipe_timeout_ns();
+}
 
 constexpr int kMaxDevices = 64;
 constexpr int64_t kMaxDim = (int64_t)1 << 31;
@@ -323,7 +332,8 @@ int mm_fp8_gemm_block128(const void* a, int64_t a_stride, const float* sa, int64
     const int esz = out_fp32 ? 4 : 2;
     p.out_vec32 = aligned(out, 32) && (out_stride * esz) % 32 == 0;
     p.status = d->status;
-    p.timeout_ns = mm_detail_pipe_timeout_ns();
+    p.timeout_ns = wait_limit_ns();
+    p.given_up = g_given_up.load();
     p.m_tiles = (m + 127) / 128;
     p.a_box_rows = m >= 128 ? 128 : (m + 7) / 8 * 8;
     // Tile width and split of K.  A turn of the SMs with tiles of 128 columns takes 0.7 of the time of one with 256 (1024 x 4096 x 4096: 29 us in
@@ -409,7 +419,7 @@ int mm_moe_few_tokens(const void* x, int x_is_fp8, int64_t x_stride, const float
     p.y = static_cast<__nv_bfloat16*>(y);
     p.clamp = clamp;
     p.status = d->status;
-    p.timeout_ns = mm_detail_pipe_timeout_ns();
+    p.timeout_ns = wait_limit_ns();
     CUtensorMap tm1, tm2;
     if (tiled) {
         if (int rc = byte_map(w1, 128, (uint64_t)E * (I / 128) * (H / 128) * 256, 128, 0, 0, 256, &tm1)) return rc;
@@ -424,6 +434,13 @@ int mm_moe_few_tokens(const void* x, int x_is_fp8, int64_t x_stride, const float
     // starts while the first one runs: its barriers, TMEM and tensor maps need nothing of it
     B_CUDA(Launch(d->sms, mm::kMoeThreads, mm::kMoeSmemBytes, st)(mm::moe_experts_kernel, tm1, tm2, p));
     B_LAUNCHED();
+    return 0;
+}
+
+int mm_block128_test_waits(int given_up_cta, int64_t limit_ns) {
+    B_REQUIRE(given_up_cta >= -1 && limit_ns >= 0, "mm_block128_test_waits: no such CTA or limit");
+    g_given_up.store(given_up_cta);
+    g_limit_ns.store(limit_ns);
     return 0;
 }
 

@@ -42,6 +42,7 @@ struct B128GemmParams {
     int out_vec32;                             // rows and base are multiples of 32 bytes
     int* status;
     uint64_t timeout_ns;
+    int given_up;                              // CTA that counts as one whose wait has run out (mm_block128_test_waits), else -1
 };
 
 __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap* map, int32_t c0, int32_t c1, int32_t c2, uint32_t bar) {
@@ -117,6 +118,12 @@ __device__ __forceinline__ void st_global_32b(void* p, const uint32_t (&v)[8]) {
 __device__ __forceinline__ float4 ld_shared_cluster_f4(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ int ld_shared_cluster_s32(uint32_t addr) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
     return v;
 }
 
@@ -309,7 +316,7 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) { mbar_init(full_bar(s), 3); mbar_init(empty_bar(s), 1); }
         for (int a = 0; a < kAccs; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), 8); }
-        st_shared_volatile(abort_flag, 0);
+        st_shared_volatile(abort_flag, static_cast<int>(blockIdx.x) == p.given_up ? 1 : 0);
         fence_barrier_init();
         prefetch_tensormap(&tm_a);
         prefetch_tensormap(&tm_b);
@@ -482,23 +489,34 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     if (kSplit) {
         __syncwarp();
         cluster_sync_all();                                  // every part of the tile is in shared memory
-        if (warp >= 4 && ld_shared_volatile(abort_flag) == 0 && first_tile < num_tiles) {
+        if (warp >= 4 && first_tile < num_tiles) {
             int mt, nt;
             b128_tile(p, first_tile, mt, nt);
             // rows part, part + split, .. of the tile are this CTA's: a warp to a row, four columns a lane
             static_assert(!kSplit || kBN == 128, "a warp holds a row of a split tile");
             const int rows = min(128, p.m - mt * 128), col = nt * kBN + lane * 4;
-            for (int r = part + (warp - 4) * split; r < rows; r += 8 * split) {
+            int r = part + (warp - 4) * split;
+            float4 v[kB128MaxSplit];
+            auto fetch = [&]() {                                         // all on their way before the first is added
                 const uint32_t at = smem_base + static_cast<uint32_t>(r * (kBN + 4) + lane * 4) * 4;
-                float4 v[kB128MaxSplit], t = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int i = 0; i < kB128MaxSplit; ++i)                  // all on their way before the first is added
+                for (int i = 0; i < kB128MaxSplit; ++i)
                     if (i < split) v[i] = ld_shared_cluster_f4(mapa_shared(at, i));
+            };
+            // A CTA that has given up has no part there, but operands: then no CTA of the cluster writes anything of the tile.  (Asked
+            // together with the first row's parts: before them it cost 0.2 us.)
+            const int failed = lane < split ? ld_shared_cluster_s32(mapa_shared(abort_flag, lane)) : 0;
+            if (r < rows) fetch();
+            if (__any_sync(0xffffffffu, failed != 0)) r = rows;
+            while (r < rows) {
+                float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (int i = 0; i < kB128MaxSplit; ++i)
                     if (i < split) { t.x += v[i].x; t.y += v[i].y; t.z += v[i].z; t.w += v[i].w; }
                 const float f[4] = {t.x, t.y, t.z, t.w};
                 const int64_t o = (mt * 128 + r) * p.out_stride + col;
+                r += 8 * split;
+                if (r < rows) fetch();
                 if (p.out_vec32 && col + 4 <= p.n) {
                     if (p.out_fp32) *reinterpret_cast<float4*>(static_cast<float*>(p.out) + o) = t;
                     else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + o) = make_uint2(pack_bf16x2(t.x, t.y), pack_bf16x2(t.z, t.w));

@@ -188,6 +188,10 @@ int mm_moe_few_tokens(const void* x, int x_is_fp8, int64_t x_stride, const float
  * taken whole, by this read or by a later one. */
 int mm_block128_read_status(void* stream, int32_t* out5);
 
+/* Test hook (host only, no device work): how the waits of later calls of these operators end.  given_up_cta: the CTA of the products that
+ * behaves as if a wait of its had run out, although it has not (-1: none).  limit_ns: limit of their waits, 0 = that of mm_set_timeouts. */
+int mm_block128_test_waits(int given_up_cta, int64_t limit_ns);
+
 /* JSON description of the build.  Replaces get_mega_moe_hip_build_config, csrc/apis/mega_dcu.hpp:28-39. */
 int mm_build_config(char* json, int capacity);
 

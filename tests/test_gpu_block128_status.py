@@ -46,3 +46,35 @@ def test_a_read_on_another_stream_takes_each_report_whole(built_lib):
         got.append(_read(built_lib, here))
         reports = [r for r in got if r[0]]
         assert reports and all(r == [BAD_GROUP_LAYOUT, 0, 1, 0, 1] for r in reports), (turn, reports)
+
+
+@pytest.fixture
+def waits(built_lib):
+    """Sets how the waits of the calls that follow end; as ever afterwards."""
+    yield lambda given_up=-1, limit_ns=0: built_lib.mm_block128_test_waits(given_up, limit_ns)
+    built_lib.mm_block128_test_waits(-1, 0)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (77, 300, 2048)])
+@pytest.mark.parametrize("cta", [0, 1, 5])
+def test_a_split_tile_is_not_written_when_one_of_its_ctas_gave_up(built_lib, waits, m, n, k, cta):
+    """The CTAs that share a tile add up what each has left in its shared memory, and one that gave up has left operands there."""
+    import megamoe
+    g = torch.Generator().manual_seed(5)
+    a, sa = ref.random_operand(g, m, k).cuda(), ref.random_scales(g, m, ref.blocks(k)).cuda()
+    b, sb = ref.random_operand(g, n, k).cuda(), ref.random_scales(g, ref.blocks(n), ref.blocks(k)).cuda()
+    want = megamoe.fp8_gemm_nt_block128((a, sa), (b, sb), out_dtype=torch.float32)
+    megamoe.check_block128_status()
+    out = torch.full((m, n), 5.0, device="cuda")
+    waits(given_up=cta)
+    megamoe.fp8_gemm_nt_block128((a, sa), (b, sb), out=out)
+    status = _read(built_lib, torch.cuda.current_stream())
+    assert status[:3] == [PIPE_TIMEOUT, 20, cta], status
+    assert not bool((want == 5).any())
+    left = (out == 5).all(0).view(-1).cpu()
+    tiles = [left[i:i + 128] for i in range(0, n, 128)]
+    assert sum(bool(t.all()) for t in tiles) == 1 and not any(bool(t.any()) for t in tiles if not bool(t.all())), "one whole tile and nothing else"
+    assert torch.equal(out.cpu()[:, ~left], want.cpu()[:, ~left])
+    waits()
+    assert torch.equal(megamoe.fp8_gemm_nt_block128((a, sa), (b, sb), out=out), want)
+    megamoe.check_block128_status()
