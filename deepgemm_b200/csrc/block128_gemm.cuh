@@ -51,14 +51,14 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap
         ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
         : "memory");
 }
-// Bounded wait like mbar_wait, for hand-overs that follow one another every few hundred cycles: the clock is not read before the wait
-// has failed a thousand times, because reading it costs more than such a hand-over.
 __device__ __forceinline__ int ld_shared_volatile(uint32_t addr) {
     int v;
     asm volatile("ld.volatile.shared.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
     return v;
 }
 __device__ __forceinline__ void st_shared_volatile(uint32_t addr, int v) { asm volatile("st.volatile.shared.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+// Bounded wait of one thread like mbar_wait, for hand-overs that follow one another every few hundred cycles: the clock is not read before
+// the wait has failed a thousand times, because reading it costs more than such a hand-over.
 __device__ __forceinline__ bool mbar_wait_often(uint32_t bar, uint32_t parity, uint32_t abort_flag, uint64_t timeout_ns) {
     uint64_t t0 = 0;
     for (uint32_t it = 1;; ++it) {
@@ -69,6 +69,13 @@ __device__ __forceinline__ bool mbar_wait_often(uint32_t bar, uint32_t parity, u
         if (t0 == 0) t0 = t;
         else if (t - t0 > timeout_ns) { st_shared_volatile(abort_flag, 1); return false; }
     }
+}
+// The same for a converged warp, with one answer for all of its lanes.  If each lane decided for itself, one could give up while another still
+// sees the barrier complete, and what follows such a wait (tcgen05.ld, elect, votes, __syncwarp) needs all of them.  (A vote for "any failed",
+// behind the loop: written as "all came", or inside the loop, it made 644 us of the layer's 128 tokens into 735 and 47 of one token into 54.)
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, uint32_t abort_flag, uint64_t timeout_ns) {
+    const bool came = mbar_wait_often(bar, parity, abort_flag, timeout_ns);
+    return !__any_sync(0xffffffffu, !came);
 }
 __device__ __forceinline__ float ld_shared_f32(uint32_t addr) {
     float v;
@@ -411,7 +418,7 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                 const float* sa1 = p.sa + static_cast<int64_t>(min(mt * 128 + 64 + l64, p.m - 1)) * p.sa_stride;
                 const float* sb = p.sb + (static_cast<int64_t>(e) * p.n_sf + min(nt * (kBN / 128) + (l64 & 1), p.n_sf - 1)) * p.k_blocks;
                 for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!mbar_wait_often(empty_bar(stage), phase ^ 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
+                    if (!mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
                     const uint32_t dst = smem_u32(scales) + slot * S::kScaleBytes + l64 * 4;
                     cp_async_4(dst, sa0 + kb);
                     cp_async_4(dst + 256, sa1 + kb);
@@ -458,7 +465,7 @@ block128_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
 #pragma unroll 1
             for (int left = kb1 - kb0; left > 0; --left, ++n) {
                 const uint32_t acc = n % kAccs;
-                if (!mbar_wait_often(tfull_bar(acc), (n / kAccs) & 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
+                if (!mbar_wait_warp(tfull_bar(acc), (n / kAccs) & 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
                 if (kSplit && idle) {
                     if (elect_lane()) mbar_arrive(tempty_bar(acc));
                     continue;

@@ -282,17 +282,21 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
         : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
-// Bounded wait for something that takes a tile's time
+// Bounded wait of a converged warp, as mbar_wait_warp, for something that takes a tile's time
 __device__ __forceinline__ bool mbar_wait_asleep(uint32_t bar, uint32_t parity, uint32_t abort_flag, uint64_t timeout_ns) {
-    uint64_t t0 = 0;
-    while (!mbar_try_wait(bar, parity)) {
-        if (ld_shared_volatile(abort_flag) != 0) return false;
-        const uint64_t t = global_timer_ns();
-        if (t0 == 0) t0 = t;
-        else if (t - t0 > timeout_ns) { st_shared_volatile(abort_flag, 1); return false; }
-        __nanosleep(40);
-    }
-    return true;
+    const auto wait = [&]() {
+        uint64_t t0 = 0;
+        while (!mbar_try_wait(bar, parity)) {
+            if (ld_shared_volatile(abort_flag) != 0) return false;
+            const uint64_t t = global_timer_ns();
+            if (t0 == 0) t0 = t;
+            else if (t - t0 > timeout_ns) { st_shared_volatile(abort_flag, 1); return false; }
+            __nanosleep(40);
+        }
+        return true;
+    };
+    const bool came = wait();
+    return !__any_sync(0xffffffffu, !came);
 }
 __device__ __forceinline__ void st_release_cta(uint32_t addr, int v) { asm volatile("st.release.cta.shared::cta.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ int ld_acquire_cta(uint32_t addr) {
@@ -457,7 +461,7 @@ __device__ __forceinline__ void moe_combine(const MoeParams& p, const MoeSmem& s
     const bool ok = tid != 0 || moe_wait_count(p.counters + kMoeCtrUnits2, units, smem_u32(&sm.words->abort), p.timeout_ns);
     if (!__all_sync(0xffffffffu, ok)) return;
     if (lane == 0) mbar_arrive(sm.finish_bar());
-    if (!mbar_wait_often(sm.finish_bar(), 0, smem_u32(&sm.words->abort), p.timeout_ns)) return;
+    if (!mbar_wait_warp(sm.finish_bar(), 0, smem_u32(&sm.words->abort), p.timeout_ns)) return;
     // A warp takes 64 columns of a token: `group` slots side by side, 32 / group lanes to each, then a sum over the slots in a fixed order.
     // (Eight slots one after the other in each thread, unrolled, were code that every SM ran once: fetching it took 4 us.)
     int group = 1;
@@ -656,9 +660,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
     const int chunks1 = sm.words->list[0].chunks, chunks = n_blocks == 0 ? 0 : chunks1 + sm.words->list[1].chunks;
 
     struct Place { int slot = 0; uint32_t phase = 0; };              // in the ring of segments
-    auto segment_at = [&](const Place& at) -> const MoeSegment* {
-        return mbar_wait_often(sfull_bar(at.slot), at.phase, abort_flag, p.timeout_ns) ? &sm.words->segment[at.slot] : nullptr;
-    };
+    auto segment_came = [&](const Place& at) { return mbar_wait_warp(sfull_bar(at.slot), at.phase, abort_flag, p.timeout_ns); };
     auto segment_done = [&](Place& at) {                             // one thread of a warp, or the MMA thread
         mbar_arrive(sempty_bar(at.slot));
     };
@@ -733,8 +735,9 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                 Place at;
                 bool alive = true;
                 while (alive) {
-                    const MoeSegment* g = segment_at(at);
-                    if (g == nullptr || g->kind < 0) break;
+                    if (!mbar_wait_often(sfull_bar(at.slot), at.phase, abort_flag, p.timeout_ns)) break;
+                    const MoeSegment* g = &sm.words->segment[at.slot];
+                    if (g->kind < 0) break;
                     const int units = g->k1 - g->k0;
                     const uint32_t idesc = moe_lanes(g->rows) == 16 ? umma_idesc_f8(64, 256) : umma_idesc_f8(128, 256);
                     segment_done(at);
@@ -781,9 +784,9 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
             };
             while (alive) {
                 if (!__all_sync(0xffffffffu, mbar_test(sfull_bar(at.slot), at.phase))) drain();          // nothing to go on with yet
-                const MoeSegment* seg = segment_at(at);
-                if (seg == nullptr || seg->kind < 0) break;
-                const MoeSegment g = *seg;
+                if (!segment_came(at)) break;
+                const MoeSegment g = sm.words->segment[at.slot];
+                if (g.kind < 0) break;
                 __syncwarp();
                 if (lane == 0) segment_done(at);
                 step(at);
@@ -823,7 +826,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                         }
                     }
                     for (int k = g.k0; k < g.k1; ++k) {
-                        if (!mbar_wait_often(empty_bar(stage), phase ^ 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
+                        if (!mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag, p.timeout_ns)) { alive = false; break; }
                         const uint32_t sdst = smem_u32(sm.scale) + slot * kMoeScaleBytes;
                         for (int r = l64; r < rows; r += 64) {
                             const uint32_t row = kind ? first + r : token_of(sm.route[first + r]);
@@ -865,8 +868,8 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
         int buffer = 0; uint32_t buffer_phase = 0;
         Place at;
         while (true) {
-            const MoeSegment* g = segment_at(at);
-            if (g == nullptr) break;
+            if (!segment_came(at)) break;
+            const MoeSegment* g = &sm.words->segment[at.slot];
             if (g->kind < 0) {
                 if (n_blocks > 0) moe_combine(p, sm, smem, n_blocks * nt2 * kb2);
                 break;
@@ -888,8 +891,9 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
         Place at;
         bool alive = true;
         while (alive) {
-            const MoeSegment* g = segment_at(at);
-            if (g == nullptr || g->kind < 0) break;
+            if (!segment_came(at)) break;
+            const MoeSegment* g = &sm.words->segment[at.slot];
+            if (g->kind < 0) break;
             const int units = g->k1 - g->k0;
             const int lanes = moe_lanes(g->rows), et = lane < lanes ? q * lanes + lane : 127;                            // row of the tile; 127: none
             if (q * lanes < g->rows) {
@@ -904,7 +908,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                 for (int j = 0; j < 64; ++j) sum[j] = 0ull;
 #pragma unroll 1
                 for (int u = 0; u < units; ++u) {
-                    if (!mbar_wait_often(tfull_bar(acc), acc_phase, abort_flag, p.timeout_ns)) { alive = false; break; }
+                    if (!mbar_wait_warp(tfull_bar(acc), acc_phase, abort_flag, p.timeout_ns)) { alive = false; break; }
                     tc_fence_after();
                     const float* sc = sm.scale + slot * (kMoeScaleBytes / 4);
                     const float s_row = sc[et];
@@ -914,7 +918,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
                     if (++slot == kMoeScaleSlots) slot = 0;
                     if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
                 }
-                if (!alive || !mbar_wait_often(sm.turn_empty(buffer), buffer_phase ^ 1u, abort_flag, p.timeout_ns)) break;
+                if (!alive || !mbar_wait_warp(sm.turn_empty(buffer), buffer_phase ^ 1u, abort_flag, p.timeout_ns)) break;
                 // Where the sums go next: rows of activations that are finished here to shared memory if they fit; else, and parts of a
                 // tile, to work memory; whole rows of outputs straight to their place.
                 if (lane < lanes && et < g->rows) {
@@ -944,7 +948,7 @@ moe_experts_kernel(const __grid_constant__ CUtensorMap tm_w1, const __grid_const
             } else {
                 // Not ahead of the others, though: a barrier tells a phase from the one after the next by nothing.  So an idle warp is
                 // counted where the sums are handed on, and waits there, mostly asleep, until the others have come.
-                if (!mbar_wait_often(sm.turn_empty(buffer), buffer_phase ^ 1u, abort_flag, p.timeout_ns)) break;
+                if (!mbar_wait_warp(sm.turn_empty(buffer), buffer_phase ^ 1u, abort_flag, p.timeout_ns)) break;
                 if (lane == 0) mbar_arrive(sm.turn_full(buffer));
                 if (!mbar_wait_asleep(sm.turn_full(buffer), buffer_phase, abort_flag, p.timeout_ns)) break;
                 slot = (slot + units) % kMoeScaleSlots;

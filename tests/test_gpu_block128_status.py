@@ -78,3 +78,50 @@ def test_a_split_tile_is_not_written_when_one_of_its_ctas_gave_up(built_lib, wai
     waits()
     assert torch.equal(megamoe.fp8_gemm_nt_block128((a, sa), (b, sb), out=out), want)
     megamoe.check_block128_status()
+
+
+def _layer(t, e, k, h, i):
+    import megamoe
+    from test_gpu_few_tokens import make
+    g = torch.Generator().manual_seed(6)
+    x, w1, w2 = make(g, t, e, h, i)
+    l1, l2 = (megamoe.pack_weights_tiled(w1[0].cuda(), "l1"), w1[1].cuda()), (megamoe.pack_weights_tiled(w2[0].cuda(), "l2"), w2[1].cuda())
+    x, logits = x.cuda(), torch.randn((t, e), generator=g).cuda()
+    return lambda out=None: megamoe.fp8_moe_few_tokens(x, l1, l2, router_logits=logits, num_topk=k, out=out)
+
+
+@pytest.mark.parametrize("t,e,k,h,i", [(1, 16, 6, 4096, 2048), (33, 16, 4, 2048, 1024), (130, 8, 2, 1024, 512)])
+def test_a_layer_whose_waits_run_out_reports_it_and_ends(built_lib, waits, t, e, k, h, i):
+    """With a limit of a nanosecond the wait for the activations of the first product runs out in every CTA, and all other waits end by
+    that: the call returns, leaves the output as it was, and the next one is as ever."""
+    import megamoe
+    call = _layer(t, e, k, h, i)
+    want = call()
+    megamoe.check_block128_status()
+    out = torch.full((t, h), 3.0, dtype=torch.bfloat16, device="cuda")
+    for _ in range(3):
+        waits(limit_ns=1)
+        call(out)
+        status = _read(built_lib, torch.cuda.current_stream())
+        assert status[:2] == [PIPE_TIMEOUT, 30], status
+        assert bool((out == 3.0).all())
+        waits()
+        assert torch.equal(call(), want)
+        megamoe.check_block128_status()
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (2000, 3000, 4096), (600, 1500, 1024)])
+def test_a_product_with_a_limit_that_may_run_out_is_right_or_reports_it(built_lib, waits, m, n, k):
+    import megamoe
+    g = torch.Generator().manual_seed(5)
+    a, sa = ref.random_operand(g, m, k).cuda(), ref.random_scales(g, m, ref.blocks(k)).cuda()
+    b, sb = ref.random_operand(g, n, k).cuda(), ref.random_scales(g, ref.blocks(n), ref.blocks(k)).cuda()
+    want = megamoe.fp8_gemm_nt_block128((a, sa), (b, sb))
+    for _ in range(3):
+        waits(limit_ns=1)
+        got = megamoe.fp8_gemm_nt_block128((a, sa), (b, sb))
+        status = _read(built_lib, torch.cuda.current_stream())
+        assert torch.equal(got, want) if status[0] == 0 else status[:2] == [PIPE_TIMEOUT, 20], status
+        waits()
+        assert torch.equal(megamoe.fp8_gemm_nt_block128((a, sa), (b, sb)), want)
+        megamoe.check_block128_status()
