@@ -25,6 +25,7 @@ from .. import _lib
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _E4M3 = torch.float8_e4m3fn
+_DIM = 2 ** 31      # sizes pass through the library's 32-bit arguments, where ctypes would cut off a larger one without a word
 
 
 def _blocks(n: int) -> int:
@@ -89,8 +90,8 @@ def cast_to_fp8_block128(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         raise TypeError("cast_to_fp8_block128 expects a bfloat16, float16 or float32 tensor with at least one dimension")
     shape = x.shape
     k = shape[-1]
-    if k == 0 or k % 8 != 0:
-        raise ValueError("the row length must be a positive multiple of 8")
+    if k == 0 or k % 8 != 0 or k >= _DIM:
+        raise ValueError("the row length must be a positive multiple of 8" if k < _DIM else "the row length must be below 2^31")
     index = _device_index("cast_to_fp8_block128", x)
     q = torch.empty_like(x, dtype=_E4M3, memory_format=torch.contiguous_format)      # (half of new_empty's time)
     sf = x.new_empty((*shape[:-1], (k + 127) // 128), dtype=torch.float32)
@@ -111,6 +112,8 @@ def cast_weight_to_fp8_block128(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Te
     n, k = w.shape[-2:]
     if k == 0 or k % 8 != 0:
         raise ValueError("the row length must be a positive multiple of 8")
+    if max(w.shape) >= _DIM:
+        raise ValueError("each size of a weight must be below 2^31")
     index = _device_index("cast_weight_to_fp8_block128", w)
     w = w.contiguous()
     if w.data_ptr() % 16 != 0:
@@ -129,6 +132,8 @@ def _check_operands(name, a, a_sf, b, b_sf, n, k):
         raise RuntimeError(f"{name} expects fp32 scales")
     if k == 0 or k % 16 != 0:
         raise RuntimeError(f"{name}: K must be a positive multiple of 16")
+    if k >= _DIM or n >= _DIM or b.shape[0] >= _DIM:
+        raise RuntimeError(f"{name}: N, K and the number of experts must be below 2^31")
     kb = (k + 127) // 128
     if a.dim() != 2 or a.shape[1] != k or a_sf.shape != (a.shape[0], kb):
         raise RuntimeError(f"{name} expects a [M, K] with scales [M, ceil(K/128)], got {tuple(a.shape)} and {tuple(a_sf.shape)}")
@@ -291,6 +296,8 @@ def fp8_moe_few_tokens(x, l1_weights: Tuple[torch.Tensor, torch.Tensor], l2_weig
         if num_topk is not None and num_topk != k:
             raise ValueError(f"{name}: num_topk does not match topk_idx")
         topk_idx, topk_weights = topk_idx.contiguous(), topk_weights.contiguous()
+    if e >= _DIM:
+        raise ValueError(f"{name}: too many experts")
     if not 0 < k <= min(e, 32):
         raise ValueError(f"{name}: topk must be in 1..{min(e, 32)}")
     if t * k > 4096:
@@ -366,6 +373,8 @@ def norm_gate_residual(y: Optional[torch.Tensor], residual: torch.Tensor, *, pos
     t, h = residual.shape
     if h == 0 or h % 8 != 0 or h > 16384:
         raise ValueError(f"{name}: H must be a multiple of 8, at most 16384")
+    if t >= _DIM:
+        raise ValueError(f"{name}: at most 2^31 - 1 tokens")
     if y is None:
         if post_weight is not None or gate is not None or residual_scale != 1.0:
             raise ValueError(f"{name}: post_weight, gate and residual_scale need y")
