@@ -279,7 +279,7 @@ int mm_norm_gate_residual(const void* y, int y_type, int64_t y_stride, const voi
     p.tokens = tokens; p.hidden = hidden; p.quant = quant; p.alpha = alpha; p.eps = eps; p.offset = offset;
     const int vecs = hidden / 8;
     // One vector of 8 values per thread while a row has an SM to itself (one row of 4096: 3.9 us against 4.7) and for an fp32 residual, whose
-    // two would not fit the registers (4000 x 4096: 49 us against 61), else two (see the kernel).  64 registers a thread, so 1024 threads
+    // two would not fit the registers (4000 x 4096: 45 us against 56), else two (see the kernel).  64 registers a thread, so 1024 threads
     // are resident on an SM; a block more than those waits a whole turn (74 us instead of 62).
     const bool two = vecs > 1024 || (tokens > 2 * d->sms && r_type != mm::B128_FP32);
     const int threads = ((two ? (vecs + 1) / 2 : vecs) + 31) / 32 * 32;

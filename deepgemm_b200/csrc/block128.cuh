@@ -7,7 +7,9 @@
 // (2^-3) of error.  x * (448 / top) alone is not enough; one residual step makes it so (Markstein, "Computation of elementary
 // functions on the IBM RISC System/6000 processor", 1990): with a = 448 x and q0 near a / top, the residual r = fma(-q0, top, a)
 // is exact and fma(r, 1 / top, q0) rounds a value that is off by (a / top - q0) times the reciprocal's error only.
-// A group that holds an infinity or a NaN gets NaN codes and a scale that is not finite, so that it cannot pass unseen.
+// A group that holds an infinity or a NaN gets NaN codes and a scale that is not finite, so that it cannot pass unseen.  (Where the codes are
+// of values that were computed here, quantise_computed, a group with an infinity has the NaN code for that value alone and 0 for its
+// finite ones; the scale is infinite, so products with the group are NaN all the same.)
 //
 // All of this is bound by HBM: one read of the inputs, one write of the outputs, everything between in registers.
 #pragma once
@@ -277,6 +279,9 @@ constexpr int kNormMaxHidden = 16384;
 // Measured at 8192 x 4096 in bf16 with codes by blocks: 55 us, 5.5 TB/s of the bytes it must move (a plain copy: 6.5); instructions and the
 // three waits of a row share what is left.  With weights read and added up in every row 61; the first form, without the prefetch and the
 // two-wide arithmetic either, took 107; one vector per thread 68, four 69, two rows at a time 60 to 76 (all three before staging).
+// The same size with an fp32 stream: 86 us (436 MB, 5.0 TB/s).  With weights and gate in bf16, or any other types, kAny: 86 with a bf16 stream
+// and weights, 88 with an fp32 stream, 102 in fp16; its two vectors a thread do not fit the 64 registers (488 bytes of spill stores), and
+// neither do those of an fp32 stream above H = 8192 (2400 x 16384: 154 us against 79 in bf16).
 template <int kVec, int kY, int kR, int kWeight, bool kStaged>
 __global__ void __launch_bounds__(1024) norm_gate_residual_kernel(const __grid_constant__ NormParams p) {
     pdl_launch();

@@ -10,9 +10,11 @@
 // One CTA per SM, 384 threads: warp 0 = TMA, warp 1 = MMA, warps 2-3 = scales, warps 4-11 = epilogue (registers moved to them).  The
 // scales of a k block travel with its operands, copied to a ring of their own in shared memory: read from global memory by the epilogue
 // they cost it an L2 latency now and then, and every cycle of the epilogue counts.
-// What bounds it (8192 x 4096 x 4096: 134 us, 2.05 PFLOP/s, at 1.65 GHz): a k block takes 985 cycles where its MMAs take 512 and moving its 48
-// KiB into and out of shared memory 675; the promotion takes 520 to 600 cycles of a warp and the hand-overs on both sides of it 300, and
-// with two accumulators that sum is the period.
+// What bounds it (8192 x 4096 x 4096: 137 us, 2.0 PFLOP/s, at the 1.54 GHz that the power cap leaves): 800 cycles for each of a CTA's 224 k
+// blocks and 4200 for each of its seven tiles (K = 1024 to 8192 lie on that line).  An accumulator goes round through its MMAs (512), the
+// promotion (520 to 600 of a warp) and two hand-overs (300); two accumulators share the way, so a block takes 690 to 790, above the 512 of the
+// MMAs and the 675 of moving 48 KiB into and out of shared memory.  A tile's own 4200 are its beginning and its end: the warps that
+// sum also store, 32 bytes a lane, and meanwhile the MMA warp is at most two blocks ahead.
 // kSplit: the CTAs of a cluster share one tile and divide its k blocks; the fp32 parts meet in distributed shared memory
 // and are added in rank order, so the result does not depend on timing.
 #pragma once
