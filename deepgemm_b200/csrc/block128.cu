@@ -21,8 +21,9 @@ void mm_detail_count_launch();
 uint64_t mm_detail_pipe_timeout_ns();
 
 // First failed wait or bad layout of any of these operators on a device since it was last read (b128_report); written by kernels only then.
-// [8 .. 12]: what the last read took.
-__device__ int g_b128_status[16];
+// Behind its eight words, eight for each read that may be under way: what it took.
+constexpr int kStatusReads = 64;
+__device__ int g_b128_status[8 + 8 * kStatusReads];
 
 namespace {
 
@@ -449,11 +450,22 @@ int mm_block128_read_status(void* stream_, int32_t* out5) {
     Device* d;
     if (int rc = device_of(&d)) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream_);
-    static std::mutex mu;                // one reader at a time: they share the words that a read takes the report to
-    std::lock_guard<std::mutex> lk(mu);
-    mm::b128_take_status_kernel<<<1, 1, 0, st>>>(d->status, d->status + 8);
+    // Words of its own for each read, not a lock: what this stream waits for may be the work of a thread that reads its own status first.
+    struct Place {
+        std::atomic<bool>* at = nullptr;
+        int index = 0;
+        Place() {
+            static std::atomic<bool> taken[kStatusReads];
+            for (index = 0; index < kStatusReads; ++index)
+                if (!taken[index].exchange(true)) { at = &taken[index]; return; }
+        }
+        ~Place() { if (at) at->store(false); }
+    } place;
+    B_REQUIRE(place.at, "mm_block128_read_status: %d reads are under way already", kStatusReads);
+    int* taken = d->status + 8 + 8 * place.index;
+    mm::b128_take_status_kernel<<<1, 1, 0, st>>>(d->status, taken);
     B_LAUNCHED();
-    B_CUDA(cudaMemcpyAsync(out5, d->status + 8, 5 * sizeof(int32_t), cudaMemcpyDeviceToHost, st));
+    B_CUDA(cudaMemcpyAsync(out5, taken, 5 * sizeof(int32_t), cudaMemcpyDeviceToHost, st));
     B_CUDA(cudaStreamSynchronize(st));
     return 0;
 }

@@ -185,7 +185,7 @@ int mm_moe_few_tokens(const void* x, int x_is_fp8, int64_t x_stride, const float
 
 /* First failure on the current device that these operators have met since the last call, as {code, phase, block, expected, observed},
  * and clears it; code 0 = none.  Synchronises the stream.  Any stream will do, also while others run these operators: a report is
- * taken whole, by this read or by a later one. */
+ * taken whole, by this read or by a later one.  Reads of several threads do not wait for one another (64 may be under way). */
 int mm_block128_read_status(void* stream, int32_t* out5);
 
 /* Test hook (host only, no device work): how the waits of later calls of these operators end.  given_up_cta: the CTA of the products that

@@ -125,3 +125,22 @@ def test_a_product_with_a_limit_that_may_run_out_is_right_or_reports_it(built_li
         waits()
         assert torch.equal(megamoe.fp8_gemm_nt_block128((a, sa), (b, sb)), want)
         megamoe.check_block128_status()
+
+
+def test_a_read_does_not_wait_for_reads_of_other_streams(built_lib):
+    """While a read waits for its busy stream, another thread's read of an idle one returns."""
+    import threading
+    busy, idle = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    _read(built_lib, idle)
+    with torch.cuda.stream(busy):
+        torch.cuda._sleep(1_000_000_000)                             # half a second or more
+    first = threading.Thread(target=_read, args=(built_lib, busy))
+    first.start()
+    others = [threading.Thread(target=_read, args=(built_lib, idle)) for _ in range(8)]
+    for t in others:
+        t.start()
+    for t in others:
+        t.join()
+    assert first.is_alive() and not busy.query(), "the reads of the idle stream came back only with the busy one's"
+    first.join()
