@@ -22,7 +22,7 @@
 //
 // Measured: 1 token, 256 experts, top-6, 4096 / 2048: 47 us (151 MB; 3.2 TB/s over the whole call, the streams themselves run at 6); 33 tokens,
 // 64 experts, top-8, 2048 / 1024: 88 us (58 experts have a token: 365 MB, 4.1 TB/s); 128 tokens, else as the first, with 170 to 190 popular
-// experts (4.3 to 4.7 GB): 645 to 680 us alone (HBM's own rate), 730 to 790 in a loop, where the power cap sets the clock.  With native
+// experts (4.3 to 4.7 GB): 640 to 680 us alone (HBM's own rate), 730 to 800 in a loop, where the power cap sets the clock.  With native
 // weights, two copies of 16 KiB for each block: 49, 89 and 663.  What bounds it at one token are the latencies around the streams: 8 us until the first
 // copy, 8 from the last sums of the first product to its activations being known everywhere, 4 for the combine.
 //
